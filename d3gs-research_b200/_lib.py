@@ -101,8 +101,15 @@ class RefineMoments(C.Structure):
                 ("exp_avg_sq_dst", C.c_void_p * 6)]
 
 
+class GroupNorm(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("pixels", C.c_int64), ("x_batch_stride", C.c_int64), ("x_pixel_stride", C.c_int64),
+                ("dy_batch_stride", C.c_int64), ("dy_pixel_stride", C.c_int64), ("channels", C.c_int32),
+                ("groups", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("act", C.c_int32),
+                ("eps", C.c_float)]
+
+
 _STRUCTS = [Camera, OpConfig, Model, ModelGrad, SplatContext, AdamSegment, DensifyStats, PeerSet, RefineConfig,
-            RefineMoments, PeerViews]
+            RefineMoments, PeerViews, GroupNorm]
 
 _P, _I32, _I64, _F, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 
@@ -157,6 +164,9 @@ SIGNATURES = {
     "d3gs_refine_apply": (_I32, [C.POINTER(Model), C.POINTER(Model), C.POINTER(RefineConfig), C.POINTER(RefineMoments),
                                  _P, _P, _P, C.POINTER(C.c_int64), _P, _P]),
     "d3gs_reset_opacity": (_I32, [_P, _I64, _F, _I32, _P, _P, _P]),
+    "d3gs_group_norm_workspace_bytes": (_SZ, [C.POINTER(GroupNorm), _I32]),
+    "d3gs_group_norm_forward": (_I32, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "d3gs_group_norm_backward": (_I32, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "d3gs_peer_buffer_create": (_I32, [_I64, C.POINTER(_P), _P]),
     "d3gs_peer_buffer_open": (_I32, [_P, C.POINTER(_P)]),
     "d3gs_peer_buffer_close": (_I32, [_P]),

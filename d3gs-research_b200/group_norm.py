@@ -1,0 +1,147 @@
+"""Group normalisation with an activation over channels-last images.
+
+The rasteriser blends ``custom_features`` into feature images ``[B, H, W, C]``; ``group_norm_act`` is the
+normalisation layer of a network that decodes such images, in their own layout and with its gradient.  The
+reference has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {"none": 0, "silu": 1, "gelu": 2}
+
+
+def _pixel_strides(t: torch.Tensor):
+    """(image stride, pixel stride) of [B, *spatial, C] when its channels are dense and its pixels evenly spaced,
+    else None."""
+    shape, stride = t.shape, t.stride()
+    if t.numel() == 0:
+        return 0, shape[-1]
+    if shape[-1] > 1 and stride[-1] != 1:
+        return None
+    pixel, span = None, 1
+    for n, s in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
+        if n == 1:
+            continue
+        if pixel is None:
+            pixel = s
+        elif s != pixel * span:
+            return None
+        span *= n
+    return (stride[0] if shape[0] > 1 else 0), (pixel if pixel is not None else shape[-1])
+
+
+def _prepared(t: torch.Tensor):
+    strides = _pixel_strides(t)
+    if strides is None:
+        t = t.contiguous()
+        strides = _pixel_strides(t)
+    return t, strides
+
+
+def _desc(x: torch.Tensor, strides, groups: int, wdtype, act: int, eps: float) -> _lib.GroupNorm:
+    d = _lib.GroupNorm()
+    d.batch, d.channels, d.groups = x.shape[0], x.shape[-1], groups
+    d.pixels = 1
+    for n in x.shape[1:-1]:
+        d.pixels *= n
+    d.x_batch_stride, d.x_pixel_stride = strides
+    d.dtype, d.weight_dtype, d.act, d.eps = _DTYPES[x.dtype], _DTYPES[wdtype], act, eps
+    return d
+
+
+def _workspace(lib, d: _lib.GroupNorm, backward: int, device):
+    n = lib.d3gs_group_norm_workspace_bytes(C.byref(d), backward)
+    if n == 0:
+        raise RuntimeError(f"d3gs_group_norm_workspace_bytes: {_lib.last_error()}")
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def _forward(x, groups, weight, bias, eps, act):
+    lib = _lib.load()
+    x, strides = _prepared(x)
+    wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+    d = _desc(x, strides, groups, wdtype, act, eps)
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+        ws, n = _workspace(lib, d, 0, x.device)
+        _lib.check(lib.d3gs_group_norm_forward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), y.data_ptr(),
+                                               stats.data_ptr(), ws.data_ptr(), n,
+                                               torch.cuda.current_stream().cuda_stream), "d3gs_group_norm_forward")
+    return x, y, stats, d
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups: int, eps: float, act: int):
+        x, y, stats, d = _forward(x.detach(), groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.desc = d
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        lib = _lib.load()
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        d = _lib.GroupNorm.from_buffer_copy(ctx.desc)
+        dy, (d.dy_batch_stride, d.dy_pixel_stride) = _prepared(dy)
+        empty = x.numel() == 0
+        with torch.cuda.device(x.device):
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            make = torch.zeros_like if empty else torch.empty_like
+            dw = make(weight) if need_w else None
+            db = make(bias) if need_b else None
+            if not empty and (need_x or need_w or need_b):
+                ws, n = _workspace(lib, d, 1, x.device)
+                _lib.check(lib.d3gs_group_norm_backward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias),
+                                                        stats.data_ptr(), dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
+                                                        _lib.ptr(db), ws.data_ptr(), n,
+                                                        torch.cuda.current_stream().cuda_stream),
+                           "d3gs_group_norm_backward")
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, eps: float = 1e-5, act: str = "silu") -> torch.Tensor:
+    """``act(weight * (x - mean) / sqrt(var + eps) + bias)`` of a channels-last image ``x`` ``[B, *spatial, C]``.
+
+    Mean and (biased) variance go over the pixels and the ``C / num_groups`` channels of a group, per image.
+    ``act`` is ``"none"``, ``"silu"`` or ``"gelu"`` (the erf form).  ``x`` is float32, bfloat16 or float16; ``weight``
+    and ``bias`` ``[C]`` share one of these types, not necessarily that of ``x``.  Sums and statistics are float32.
+    Channels that are not dense, or pixels that are not evenly spaced, are copied first.  The result is dense and has
+    the type of ``x``; gradients flow to ``x``, ``weight`` and ``bias`` (once)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("group_norm_act: x must be a CUDA tensor")
+    if x.dim() < 2 or x.dtype not in _DTYPES:
+        raise ValueError(f"group_norm_act: x must be [B, ..., C] in float32, bfloat16 or float16, got {tuple(x.shape)} "
+                         f"{x.dtype}")
+    if act not in _ACTS:
+        raise ValueError(f"group_norm_act: act must be one of {sorted(_ACTS)}, got {act!r}")
+    c = x.shape[-1]
+    num_groups = int(num_groups)
+    if num_groups < 1 or c < 1 or c % num_groups:
+        raise ValueError(f"group_norm_act: {num_groups} groups do not divide {c} channels")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"group_norm_act: eps must be finite and not negative, got {eps}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (c,) or t.device != x.device or t.dtype not in _DTYPES:
+            raise ValueError(f"group_norm_act: {name} must be [{c}] on {x.device} in float32, bfloat16 or float16, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("group_norm_act: weight and bias must have one type")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNormAct.apply(x, weight, bias, num_groups, float(eps), _ACTS[act])
+    return _forward(x, num_groups, weight, bias, float(eps), _ACTS[act])[1]

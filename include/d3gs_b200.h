@@ -522,6 +522,33 @@ int32_t d3gs_simple_knn(const float* points, int64_t point_stride, int64_t n, in
                         const float* points_min, const float* points_max, float* out, void* workspace,
                         size_t workspace_bytes, uint32_t* status, void* stream);
 
+/* ---- group normalisation with an activation over channels-last images (custom feature images, [B, H, W, C]) ----
+ * mean and variance over the pixels and the C/groups channels of a group, per image; xhat = (x - mean) /
+ * sqrt(var + eps); y = act(weight * xhat + bias).  No counterpart in the reference.  weight and bias [C] (either may
+ * be NULL: 1 and 0) have weight_dtype, everything else dtype.  x and dy: the channels of a pixel are dense, pixels
+ * and images lie x_/dy_ *_stride values apart; y and dx are dense.  stats [batch, groups, 2] float (mean,
+ * 1/sqrt(var+eps)) is written by the forward and read by the backward.  The backward writes dx, dweight and dbias
+ * (any of them NULL: not wanted).  Sums are kept in 32 bits and joined in a fixed order.  At most 65535 images and
+ * 16384 channels.  An empty batch or image launches nothing and writes nothing. */
+#define D3GS_DTYPE_F32 0
+#define D3GS_DTYPE_BF16 1
+#define D3GS_DTYPE_F16 2
+typedef struct D3gsGroupNorm {
+    int64_t batch, pixels;
+    int64_t x_batch_stride, x_pixel_stride;
+    int64_t dy_batch_stride, dy_pixel_stride;   /* backward only */
+    int32_t channels, groups;
+    int32_t dtype, weight_dtype;                /* D3GS_DTYPE_* */
+    int32_t act;                                /* 0 none, 1 silu, 2 gelu (erf) */
+    float eps;
+} D3gsGroupNorm;
+size_t d3gs_group_norm_workspace_bytes(const D3gsGroupNorm* desc, int32_t backward);
+int32_t d3gs_group_norm_forward(const D3gsGroupNorm* desc, const void* x, const void* weight, const void* bias, void* y,
+                                float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int32_t d3gs_group_norm_backward(const D3gsGroupNorm* desc, const void* x, const void* weight, const void* bias,
+                                 const float* stats, const void* dy, void* dx, void* dweight, void* dbias,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

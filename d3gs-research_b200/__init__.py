@@ -21,7 +21,9 @@ def __getattr__(name):
         "CameraBundle": "render", "GaussianSplatOutput": "render", "GaussianSplatOpContext": "render",
         "GaussianSplatGradients": "render", "fused_ssim_loss": "fused_ssim", "l1_dssim_loss": "fused_ssim",
         "l1_loss": "fused_ssim", "GaussianAdam": "adam", "fused_step": "adam", "GaussianTrainState": "strategy",
-        "GaussianStrategyOrigin": "strategy", "group_norm_act": "group_norm", "create_origin_3dgs_optimizers": "tools", "SplatTrainer": "trainer",
+        "GaussianStrategyOrigin": "strategy", "group_norm_act": "group_norm",
+        "orthogonalize": "muon", "muon_step": "muon", "GaussianMuon": "muon",
+        "create_origin_3dgs_optimizers": "tools", "SplatTrainer": "trainer",
     }
     if name in table:
         return getattr(importlib.import_module(f"{__name__}.{table[name]}"), name)

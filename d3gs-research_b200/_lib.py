@@ -108,8 +108,21 @@ class GroupNorm(C.Structure):
                 ("eps", C.c_float)]
 
 
+NS_MAX_STEPS = 32
+
+
+class OrthoMatrix(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("momentum", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("src_row_stride", C.c_int64), ("rate", C.c_float), ("reserved_", C.c_int32)]
+
+
+class OrthoConfig(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("steps", C.c_int32), ("coefficients", C.c_float * 3 * NS_MAX_STEPS),
+                ("eps", C.c_float), ("momentum", C.c_float), ("decay", C.c_float), ("nesterov", C.c_int32)]
+
+
 _STRUCTS = [Camera, OpConfig, Model, ModelGrad, SplatContext, AdamSegment, DensifyStats, PeerSet, RefineConfig,
-            RefineMoments, PeerViews, GroupNorm]
+            RefineMoments, PeerViews, GroupNorm, OrthoMatrix, OrthoConfig]
 
 _P, _I32, _I64, _F, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 
@@ -167,6 +180,9 @@ SIGNATURES = {
     "d3gs_group_norm_workspace_bytes": (_SZ, [C.POINTER(GroupNorm), _I32]),
     "d3gs_group_norm_forward": (_I32, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "d3gs_group_norm_backward": (_I32, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "d3gs_orthogonalize_workspace_bytes": (_SZ, [C.POINTER(OrthoMatrix), _I32, C.POINTER(OrthoConfig)]),
+    "d3gs_orthogonalize": (_I32, [C.POINTER(OrthoMatrix), _I32, C.POINTER(OrthoConfig), _P, _SZ, _P]),
+    "d3gs_muon_step": (_I32, [C.POINTER(OrthoMatrix), _I32, C.POINTER(OrthoConfig), _P, _SZ, _P]),
     "d3gs_peer_buffer_create": (_I32, [_I64, C.POINTER(_P), _P]),
     "d3gs_peer_buffer_open": (_I32, [_P, C.POINTER(_P)]),
     "d3gs_peer_buffer_close": (_I32, [_P]),

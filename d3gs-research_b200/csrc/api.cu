@@ -72,6 +72,8 @@ extern "C" size_t d3gs_struct_size(int32_t which) {
         case 9: return sizeof(D3gsRefineMoments);
         case 10: return sizeof(D3gsPeerViews);
         case 11: return sizeof(D3gsGroupNorm);
+        case 12: return sizeof(D3gsOrthoMatrix);
+        case 13: return sizeof(D3gsOrthoConfig);
         default: return 0;
     }
 }

@@ -1,0 +1,205 @@
+"""Orthogonalised updates of weight matrices, and the optimizer that takes them.
+
+``GaussianAdam`` steps the per-Gaussian parameters.  The hidden matrices of a network that decodes rendered feature
+images are better served by an update whose singular values are all near one: the momentum, orthogonalised by a few
+Newton-Schulz products.  ``orthogonalize`` is that product chain, ``muon_step`` the whole update of a list of
+parameters in a handful of launches, ``GaussianMuon`` the optimizer around it.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Sequence
+
+import torch
+
+from . import _lib
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib.OrthoConfig:
+    if not 1 <= steps <= _lib.NS_MAX_STEPS:
+        raise ValueError(f"{what}: ns_steps must be 1 to {_lib.NS_MAX_STEPS}, got {steps}")
+    coefficients = list(coefficients)
+    if len(coefficients) == 3 and not isinstance(coefficients[0], (tuple, list)):
+        coefficients = [coefficients] * steps
+    if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
+        raise ValueError(f"{what}: ns_coefficients must be (a, b, c), or one such triple for each of {steps} steps")
+    if not all(math.isfinite(v) for c in coefficients for v in c):
+        raise ValueError(f"{what}: ns_coefficients must be finite")
+    if not 0.0 < eps < float("inf"):
+        raise ValueError(f"{what}: eps must be finite and positive, got {eps}")
+    cfg = _lib.OrthoConfig()
+    cfg.dtype, cfg.steps, cfg.eps = dtype, steps, eps
+    for k, c in enumerate(coefficients):
+        cfg.coefficients[k][:] = c
+    return cfg
+
+
+def _run(entry: str, mats, count: int, cfg: _lib.OrthoConfig, device):
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        n = lib.d3gs_orthogonalize_workspace_bytes(mats, count, C.byref(cfg))
+        if n == 0:
+            raise RuntimeError(f"{entry}: {_lib.last_error()}")
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        _lib.check(getattr(lib, entry)(mats, count, C.byref(cfg), ws.data_ptr(), n,
+                                       torch.cuda.current_stream().cuda_stream), entry)
+
+
+@torch.no_grad()
+def orthogonalize(update: torch.Tensor, ns_coefficients: Sequence = NS_COEFFICIENTS, eps: float = 1e-7,
+                  ns_steps: int = 5) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of a matrix ``[m, n]`` or of each matrix of a stack ``[..., m, n]``.
+
+    ``X = U / max(|U|_F, eps)``, then ``ns_steps`` times ``X = a X + (b A + c A A) X`` with ``A = X X^T``.
+    ``ns_coefficients`` is ``(a, b, c)``, or one such triple per step.  float32 or bfloat16 in, a dense tensor of the
+    same type out; every product is summed in 32 bits.  Rows that are not dense are copied first.  No gradient."""
+    if not isinstance(update, torch.Tensor) or not update.is_cuda:
+        raise ValueError("orthogonalize: update must be a CUDA tensor")
+    if update.dim() < 2 or update.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"orthogonalize: update must be [..., m, n] in float32 or bfloat16, got {tuple(update.shape)} "
+                         f"{update.dtype}")
+    cfg = _config("orthogonalize", 0 if update.dtype == torch.float32 else 1, ns_coefficients, eps, ns_steps)
+    out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
+    if update.numel() == 0:
+        return out
+    m, n = update.shape[-2:]
+    if (n > 1 and update.stride(-1) != 1) or update.dim() > 3:
+        update = update.contiguous()
+    src = update.reshape(-1, m, n)
+    count, step, size = src.shape[0], src.stride(0) * src.element_size(), src.element_size()
+    mats = (_lib.OrthoMatrix * count)()
+    for k in range(count):
+        d = mats[k]
+        d.src, d.dst = src.data_ptr() + k * step, out.data_ptr() + k * m * n * size
+        d.rows, d.cols, d.src_row_stride = m, n, src.stride(1)
+    _run("d3gs_orthogonalize", mats, count, cfg, update.device)
+    return out
+
+
+def _dense_rows(t: torch.Tensor) -> bool:
+    """Whether the first axis is the outermost of a gapless layout (contiguous or channels last): flattening the
+    rest gives the same columns, in some order, for every tensor of these strides."""
+    return (t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last))
+            or (t.dim() == 5 and t.is_contiguous(memory_format=torch.channels_last_3d)))
+
+
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Equal strides wherever an axis has more than one value."""
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
+def _adjusted_lr(lr: float, rows: int, cols: int, adjust_lr_fn: str | None) -> float:
+    if adjust_lr_fn == "match_rms_adamw":
+        return lr * 0.2 * math.sqrt(max(rows, cols))
+    return lr * math.sqrt(max(1.0, rows / cols))
+
+
+_ADJUST = (None, "original", "match_rms_adamw")
+
+
+@torch.no_grad()
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momentum_buffers: Sequence[torch.Tensor], *,
+              lr: float, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
+              ns_coefficients: Sequence = NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
+              adjust_lr_fn: str | None = None) -> None:
+    """One optimizer step of a list of float32 parameters, in place, all of them through the same launches::
+
+        buffer = momentum * buffer + (1 - momentum) * grad
+        update = momentum * buffer + (1 - momentum) * grad   if nesterov else   buffer
+        param  = (1 - lr * weight_decay) * param - lr * ratio * orthogonalize(update)
+
+    A parameter of more than two axes (a convolution's filters) is taken as ``[size(0), the rest]``.  ``ratio`` is
+    ``sqrt(max(1, rows / columns))``, or with ``adjust_lr_fn="match_rms_adamw"`` ``0.2 sqrt(max(rows, columns))``.
+    Parameters and buffers must be dense (contiguous or channels last) and must not overlap one another."""
+    params, grads, momentum_buffers = list(params), list(grads), list(momentum_buffers)
+    if not len(params) == len(grads) == len(momentum_buffers):
+        raise ValueError(f"muon_step: {len(params)} params, {len(grads)} grads, {len(momentum_buffers)} momentum_buffers")
+    if adjust_lr_fn not in _ADJUST:
+        raise ValueError(f"muon_step: adjust_lr_fn must be one of {_ADJUST}, got {adjust_lr_fn!r}")
+    for name, v in (("lr", lr), ("weight_decay", weight_decay)):
+        if not 0.0 <= v < float("inf"):
+            raise ValueError(f"muon_step: {name} must be finite and not negative, got {v}")
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError(f"muon_step: momentum must be in [0, 1), got {momentum}")
+    cfg = _config("muon_step", 0, ns_coefficients, eps, ns_steps)
+    cfg.momentum, cfg.decay, cfg.nesterov = momentum, 1.0 - lr * weight_decay, int(nesterov)
+    mats = (_lib.OrthoMatrix * max(len(params), 1))()
+    keep, spans, count, device = [], [], 0, None
+    for p, g, buf in zip(params, grads, momentum_buffers):
+        if not (p.is_cuda and p.dtype == g.dtype == buf.dtype == torch.float32 and p.dim() >= 2 and g.device == p.device
+                and buf.device == p.device and g.shape == p.shape == buf.shape and g.layout == torch.strided):
+            raise ValueError("muon_step: params, grads and momentum_buffers must be float32 CUDA tensors of two or more axes "
+                             f"with equal shapes and devices, got {tuple(p.shape)} {p.dtype} {p.device}, {tuple(g.shape)} "
+                             f"{g.dtype} {g.device}, {tuple(buf.shape)} {buf.dtype} {buf.device}")
+        if device is None:
+            device = p.device
+        if p.device != device:
+            raise ValueError(f"muon_step: parameters on {device} and {p.device} in one call")
+        if p.numel() == 0:
+            continue
+        if not _dense_rows(p) or not _same_order(p, buf):
+            raise ValueError(f"muon_step: a parameter of strides {p.stride()} or its buffer of strides {buf.stride()} is not "
+                             "dense (contiguous or channels last, the two alike)")
+        rows, cols = p.shape[0], p.numel() // p.shape[0]
+        row_stride = cols
+        if not _same_order(p, g):
+            if g.dim() == 2 and (cols == 1 or g.stride(1) == 1) and p.is_contiguous():
+                row_stride = g.stride(0)
+            else:
+                g = torch.empty_like(p).copy_(g)
+                keep.append(g)
+        d = mats[count]
+        d.src, d.momentum, d.dst = g.data_ptr(), buf.data_ptr(), p.data_ptr()
+        d.rows, d.cols, d.src_row_stride = rows, cols, row_stride
+        d.rate = _adjusted_lr(lr, rows, cols, adjust_lr_fn)
+        spans += [(d.momentum, rows * cols * 4), (d.dst, rows * cols * 4)]
+        count += 1
+    if count == 0:
+        return
+    spans.sort()
+    if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+        raise ValueError("muon_step: parameters or buffers overlap (is one given twice?)")
+    _run("d3gs_muon_step", mats, count, cfg, device)
+    torch.autograd.graph.increment_version([*params, *momentum_buffers])
+
+
+class GaussianMuon(torch.optim.Optimizer):
+    """Optimizer over ``muon_step``: one call per parameter group.  Takes float32 CUDA parameters of two or more axes;
+    biases and per-Gaussian parameters belong to ``GaussianAdam``.  The state of a parameter is ``momentum_buffer``.
+    Hyper-parameters are those of ``muon_step``."""
+
+    def __init__(self, params, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients: Sequence = NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
+                 adjust_lr_fn: str | None = None):
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                      ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
+                                      adjust_lr_fn=adjust_lr_fn))
+        for group in self.param_groups:
+            _config("GaussianMuon", 0, group["ns_coefficients"], group["eps"], group["ns_steps"])
+            for p in group["params"]:
+                if p.dim() < 2 or p.dtype != torch.float32:
+                    raise ValueError(f"GaussianMuon: parameters must be float32 with two or more axes, got {tuple(p.shape)} "
+                                     f"{p.dtype}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            for p in params:
+                state = self.state[p]
+                if len(state) == 0:
+                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            if params:
+                muon_step(params, [p.grad for p in params], [self.state[p]["momentum_buffer"] for p in params],
+                          **{k: v for k, v in group.items() if k in _HYPER})
+        return loss
+
+
+_HYPER = ("lr", "weight_decay", "momentum", "nesterov", "ns_coefficients", "eps", "ns_steps", "adjust_lr_fn")

@@ -549,6 +549,38 @@ int32_t d3gs_group_norm_backward(const D3gsGroupNorm* desc, const void* x, const
                                  const float* stats, const void* dy, void* dx, void* dweight, void* dbias,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- orthogonalised updates of weight matrices (Newton-Schulz), and the optimizer step around them -------------------
+ * X = U / max(|U|_F, eps); each step X <- a X + (b A + c A A) X with A = X X^T (on the short side): the singular values
+ * go through the polynomial a s + b s^3 + c s^5, the singular vectors stay.  No counterpart in the reference.
+ *   d3gs_orthogonalize: dst = X after all steps, U = src; src and dst have cfg->dtype.  dst may be src.
+ *   d3gs_muon_step: momentum = mu momentum + (1 - mu) src;  U = nesterov ? mu momentum + (1 - mu) src : momentum;
+ *                   dst = decay dst - rate X   (src the gradient, dst the parameter, all 32 bits)
+ * A list of matrices of any sizes shares the launches.  src: rows lie src_row_stride values apart, columns are dense;
+ * dst and momentum are dense.  No matrix's dst or momentum may overlap another's.  Short side at most 16384, long side
+ * at most 2^24, below 2^31 values.  An empty matrix is left alone; one of zeros gives zeros. */
+#define D3GS_NS_MAX_STEPS 32
+typedef struct D3gsOrthoMatrix {
+    const void* src;
+    float* momentum;          /* d3gs_muon_step only */
+    void* dst;
+    int64_t rows, cols, src_row_stride;
+    float rate;               /* d3gs_muon_step only */
+    int32_t reserved_;
+} D3gsOrthoMatrix;
+typedef struct D3gsOrthoConfig {
+    int32_t dtype;            /* D3GS_DTYPE_F32 or _BF16 (d3gs_muon_step: F32) */
+    int32_t steps;
+    float coefficients[D3GS_NS_MAX_STEPS][3];   /* a, b, c of every step */
+    float eps;
+    float momentum, decay;    /* d3gs_muon_step only: mu; 1 - lr * weight decay */
+    int32_t nesterov;
+} D3gsOrthoConfig;
+size_t d3gs_orthogonalize_workspace_bytes(const D3gsOrthoMatrix* matrices, int32_t count, const D3gsOrthoConfig* cfg);
+int32_t d3gs_orthogonalize(const D3gsOrthoMatrix* matrices, int32_t count, const D3gsOrthoConfig* cfg, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int32_t d3gs_muon_step(const D3gsOrthoMatrix* matrices, int32_t count, const D3gsOrthoConfig* cfg, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

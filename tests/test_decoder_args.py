@@ -91,6 +91,18 @@ def test_ortho_config(kw, word):
     assert word in _lib.last_error()
 
 
+def test_ortho_coefficients_that_grow_without_bound():
+    lib = _lib.load()
+    mats, cfg = ortho()
+    for k in range(5):
+        cfg.coefficients[k][:] = (5.0, 0.0, 0.0)          # 5^5 = 3125
+    assert lib.d3gs_orthogonalize(mats, 1, C.byref(cfg), 256, 1 << 40, None) == -1
+    assert "singular values grow" in _lib.last_error()
+    for k in range(5):
+        cfg.coefficients[k][:] = (0.0, 0.0, 0.0)
+    assert lib.d3gs_orthogonalize_workspace_bytes(mats, 1, C.byref(cfg)) > 0
+
+
 def test_ortho_workspace():
     lib = _lib.load()
     mats, cfg = ortho(3)

@@ -5,7 +5,9 @@ direction, by up to 3.4, so what a rounding costs depends on the matrix.  ``chai
 formula a second time with every operand of every product rounded to ``bits`` bits (with a random sign): the
 distance between the two runs is what arithmetic of that width costs on this matrix.  32-bit matrices are held to
 four times the cost of 20 bits (operands of 22 bits, and sums whose last bits are lost over long rows), 16-bit ones
-to four times the cost of 11 bits, both in the 2-norm, plus half a step of the output's type.
+to four times the cost of 11 bits, both in the 2-norm, plus half a step of the output's type.  Operands are fp16 values
+of a scale of 2^15, whose smallest step is 2^-24: an entry of X is off by 2^-25 / 2^15 = 2^-40 at least, and a small
+singular value, with the error in its direction, grows by the product of the steps' a.
 """
 import copy
 import math
@@ -43,7 +45,8 @@ def chain(u, coefs=(NS,) * 5, eps=1e-7, bits=None):
 
 def bound(u, ref, dtype, coefs=(NS,) * 5, eps=1e-7):
     cost = torch.linalg.vector_norm(chain(u, coefs, eps, 20 if dtype == F32 else 11) - ref)
-    return 4 * cost + torch.finfo(dtype).eps / 2 * torch.linalg.vector_norm(ref) + 1e-12
+    return 4 * cost + torch.finfo(dtype).eps / 2 * torch.linalg.vector_norm(ref) \
+        + 4 * math.sqrt(u.numel()) * 2.0 ** -40 * math.prod(max(1.0, abs(c[0])) for c in coefs)
 
 
 def make(m, n, seed=0, scale=1e-3):
@@ -302,5 +305,24 @@ def test_refusals(cuda_device):
             muon_step(*args, **{"lr": 0.1, **kw})
     with pytest.raises(ValueError, match="GaussianMuon"):
         GaussianMuon([torch.nn.Parameter(torch.zeros(3, device="cuda"))])
+    with pytest.raises(RuntimeError, match="singular values grow"):
+        orthogonalize(u, ns_coefficients=(9.0, 0.0, 0.0))
     with pytest.raises(RuntimeError, match="short side"):
         orthogonalize(torch.empty(16385, 1, device="cuda").expand(16385, 16385))
+
+
+def test_a_wait_that_gives_up_spoils_the_result_and_no_more(cuda_device):
+    """One CTA of every product never asks for its first tile (nothing is in flight when its waits run out): the call
+    returns, its result is NaN, and the next call is right."""
+    from d3gs_research_b200 import _lib
+    lib = _lib.load()
+    u = make(200, 300)
+    want = orthogonalize(u)
+    lib.d3gs_test_hooks(300, 0)
+    try:
+        got = orthogonalize(u)
+        torch.cuda.synchronize()
+    finally:
+        lib.d3gs_test_hooks(0, -1)
+    assert torch.isnan(got).all()
+    assert torch.equal(orthogonalize(u), want)

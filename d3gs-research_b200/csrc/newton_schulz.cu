@@ -8,9 +8,13 @@
 //
 // The products run on the tensor cores (tcgen05, 32-bit sums in TMEM).  Their operands are fp16 with a power-of-two
 // scale: X, A and B have bounded spectra (the bounds follow from the coefficients), so the 2^29 of fp16's normal range
-// hold every entry that matters.  16-bit matrices use one fp16 value per entry (11 bits: their result is rounded to 8).
-// 32-bit matrices use two, v = hi + lo (22 bits), and three products hi hi + hi lo + lo hi; the dropped lo lo is of the
-// size of the last bit.  (Two bf16 values would hold 16 bits only, and three of them need six products.)
+// hold every entry that matters.  One fp16 value keeps 11 bits, two of them, v = hi + lo, keep 22.
+//  * 32-bit matrices: all operands hi + lo, three products hi hi + hi lo + lo hi; the dropped lo lo is of the size of
+//    the last bit.  (Two bf16 values would hold 16 bits only, and three of them need six products.)
+//  * 16-bit matrices: A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
+//    and B lose turns X's singular directions by that much and no more.  What X loses is noise in all directions alike,
+//    and the next steps amplify it where X is small: with one value the result is 4e-3 off at 512 x 512 and 6e-3 at
+//    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.
 //
 // Working matrices are stored as the products read them: blocks of 128 rows x 64 columns, each the image of one shared
 // memory tile (128-byte rows, 16-byte pieces exchanged within groups of eight rows), hi and lo one after the other, zero
@@ -57,19 +61,25 @@ struct Table {
     int32_t from;         // which of x[] holds X
     float ca, cb, cc;     // this step's coefficients, by the scales of what they multiply (see scales_of)
     float out_scale;      // of a product's result; of X in the first and the last pass
+    int32_t last;         // the last step
     uint32_t* fail;       // set when a bounded wait ran out: the last pass then writes NaN
     TestHooks hooks;
 };
 
+// Launches follow one another closely: a kernel may start while its predecessor's last CTAs run, and waits here before
+// it touches memory.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // the matrix a CTA belongs to, and its number within it
-__device__ __forceinline__ int find_matrix(const Table& t, int& block) {
+__device__ __forceinline__ int find_matrix(const Table& t, int id, int& block) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if ((int)blockIdx.x >= t.first_block[mid]) lo = mid;
+        if (id >= t.first_block[mid]) lo = mid;
         else hi = mid - 1;
     }
-    block = (int)blockIdx.x - t.first_block[lo];
+    block = id - t.first_block[lo];
     return lo;
 }
 
@@ -85,9 +95,11 @@ __device__ __forceinline__ float update_of(const Table& t, float g, float buf) {
 // ---- new momentum, and the sum of squares of the update (in 64 bits: no value of a float overflows it) -----------
 __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant__ Table t) {
     __shared__ double s[kThreads / 32];
+    let_next_start();
+    wait_for_previous();
     if (blockIdx.x == 0 && threadIdx.x == 0) *t.fail = 0;
     int block;
-    const Matrix& m = t.mat[find_matrix(t, block)];
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
     const int64_t count = (int64_t)m.rows * m.cols, i0 = (int64_t)block * kNormChunk, i1 = min(count, i0 + kNormChunk);
     double sum = 0.0;
     for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) {
@@ -139,10 +151,12 @@ __device__ __forceinline__ uint32_t pack(__half a, __half b) {
 }
 
 // ---- first pass: blocks of X = U / norm, transposed when the matrix is tall; one CTA per block --------------------
-template <int PLANES> __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant__ Table t) {
-    __shared__ __align__(16) uint32_t s[PLANES * kPlane / 4];
+__global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant__ Table t) {
+    __shared__ __align__(16) uint32_t s[2 * kPlane / 4];
+    let_next_start();
+    wait_for_previous();
     int block;
-    const Matrix& m = t.mat[find_matrix(t, block)];
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
     const float inv = inverse_norm(t, m);
     const bool tall = m.rows > m.cols;
     const int r0 = block / m.nk * kRows, c0 = block % m.nk * kCols;
@@ -166,25 +180,26 @@ template <int PLANES> __global__ void __launch_bounds__(kThreads) ns_load_kernel
         split(v[1], h[1], l[1]);
         const uint32_t o = block_offset(r, c) / 4;
         s[o] = pack(h[0], h[1]);
-        if (PLANES == 2) s[kPlane / 4 + o] = pack(l[0], l[1]);
+        s[kPlane / 4 + o] = pack(l[0], l[1]);
     }
     __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(m.x[0] + (int64_t)block * PLANES * kPlane);
-    for (int i = threadIdx.x; i < PLANES * (int)kPlane / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(s)[i];
+    uint4* out = reinterpret_cast<uint4*>(m.x[0] + (int64_t)block * 2 * kPlane);
+    for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(s)[i];
 }
 
 // ---- last pass: result or parameter from the blocks of X; one CTA per block ---------------------------------------
-template <int PLANES> __global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constant__ Table t) {
+__global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constant__ Table t) {
+    wait_for_previous();
     int block;
-    const Matrix& m = t.mat[find_matrix(t, block)];
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
     const bool tall = m.rows > m.cols, failed = *t.fail != 0;
     const int r0 = block / m.nk * kRows, c0 = block % m.nk * kCols;
-    const char* x = m.x[t.from] + (int64_t)block * PLANES * kPlane;
+    const char* x = m.x[t.from] + (int64_t)block * 2 * kPlane;
     for (int i = threadIdx.x; i < kRows * kCols / 2; i += kThreads) {
         const int r = tall ? i % kRows : i / (kCols / 2), c = (tall ? i / kRows : i % (kCols / 2)) * 2;
         const uint32_t o = block_offset(r, c);
         const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(x + o));
-        const float2 lo = PLANES == 2 ? __half22float2(*reinterpret_cast<const __half2*>(x + kPlane + o)) : make_float2(0.0f, 0.0f);
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(x + kPlane + o));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t xr = r0 + r, xc = c0 + c + k;
@@ -205,25 +220,49 @@ template <int PLANES> __global__ void __launch_bounds__(kThreads) ns_store_kerne
 }
 
 // ---- tcgen05 ------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t* out, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(out)), "r"(cols) : "memory");
+// CG: 1, or 2 where a pair of CTAs works on one tile
+template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t* out, uint32_t cols) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(out)), "r"(cols) : "memory");
+    else
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(out)), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t cols) {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols));
+template <int CG> __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t cols) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols));
+    } else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols));
+    }
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// arrives at the barrier (of both CTAs of a pair) when the products issued so far are done
+template <int CG> __device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-        : "memory");
+template <int CG> __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
 }
 // 32 columns of this thread's TMEM lane
 __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
@@ -242,6 +281,56 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// the same barrier in CTA `rank` of the cluster
+__device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(rank)
+        : "memory");
+}
+// a wait for arrivals from other CTAs of the cluster, bounded like mbar_wait_bounded
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
+    const uint32_t polls = limit != 0 ? limit : (1u << 22);
+    for (uint32_t it = 0; it < polls; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (it > 64) __nanosleep(64);
+    }
+    return false;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float load_shared_of(uint32_t at, uint32_t rank) {
+    float v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %1, %2;\n\t"
+        "ld.shared::cluster.f32 %0, [a];\n\t}"
+        : "=f"(v)
+        : "r"(at), "r"(rank)
+        : "memory");
+    return v;
+}
 __device__ __forceinline__ void bulk_wait_group0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Shared-memory operand in 128-byte rows with the 16-byte pieces exchanged (swizzle mode 2).  Summed along the rows:
@@ -251,34 +340,105 @@ __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t next, uint32_t
     return (uint64_t)((at >> 4) & 0x3fffu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
+// D 32 bits, A and B fp16; B X sums its right factor across the rows (bit 16)
+__device__ __forceinline__ uint32_t instruction(bool across, uint32_t rows, uint32_t cols) {
+    return (1u << 4) | ((across ? 1u : 0u) << 16) | ((cols / 8u) << 17) | ((rows / 16u) << 24);
+}
 
-// ---- products: one 128 x 128 tile a CTA ---------------------------------------------------------------------------
-// Warp 4 brings in operand tiles by bulk copies, warp 5 issues the products, warps 0-3 (one TMEM quarter each) take the
-// sums out.  The tensor cores cut the last bits of a running sum at every step (towards zero, so that the losses add
-// up; 2e-5 of the result at 1025 x 515 when nothing is done about it).  With PLANES == 2 the sums of hi hi are therefore
-// taken out every kRunBlocks column blocks and added in registers (rounded), the products going to another part of TMEM
-// meanwhile; hi lo + lo hi, 2^-11 of their size, have a sum of their own that is taken out once.
+// ---- products -----------------------------------------------------------------------------------------------------
+// Roles of a CTA: one warp brings in operand tiles by bulk copies, one issues the products, the others take the sums
+// out of TMEM and write the result's blocks.
+//
+// The tensor cores cut the last bits of a running sum at every addition (towards zero, so that the losses add up: 2e-5
+// of the result at 1025 x 515 when nothing is done about it).  For 32-bit matrices the sums of hi hi are therefore taken
+// out after every column block and added in registers (rounded).  That costs no time: hi lo + lo hi, 2^-11 of their
+// size, go to a sum of their own, taken out once, and the tensor cores work on those meanwhile.
+//
 // A and B are symmetric: only tiles on and above the diagonal are computed, and written twice.  Rows behind the last
 // column block of A and B hold anything: nothing sums over them, and no valid row or column reads them.
 enum { kGram = 0, kSquare = 1, kApply = 2 };
-constexpr int kGemmThreads = 192, kTile = 128, kRunBlocks = 2;
-template <int PLANES> struct Stages {
-    static constexpr uint32_t kOperand = PLANES * kPlane, kStage = 2 * kOperand;
-    static constexpr int kCount = PLANES == 2 ? 3 : 6;
-    static constexpr uint32_t kBytes = kCount * kStage + 1024;   // alignment to 1024
-    static constexpr uint32_t kTmem = PLANES == 2 ? 512 : 128;   // columns: two sums of hi hi, one of the rest; one sum
+
+// What the products of a mode read: planes of the left and the right factor and of the result, and how many planes lie
+// between blocks of A and B.  RIGHT is 1 in the last step of 16-bit matrices.
+template <bool F32, int MODE, int RIGHT> struct Planes {
+    static constexpr int kLeft = F32 ? 2 : 1;
+    static constexpr int kRight = RIGHT;
+    static constexpr int kOut = F32 || MODE == kApply ? 2 : 1;
+    static constexpr uint32_t kAB = (F32 ? 2 : 1) * kPlane, kX = 2 * kPlane;   // bytes of one block
 };
 
-template <int PLANES, int MODE>
-__global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_constant__ Table t) {
-    using S = Stages<PLANES>;
+// One 16-byte piece of a result: eight columns of a row, from sums to planes.  `old`: A at the same place (kSquare).
+template <int MODE> __device__ __forceinline__ void finish(const Table& t, const float* v, const float* old, int diagonal,
+                                                           __half* hi, __half* lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float f = v[i];
+        if (MODE == kSquare) {
+            f = fmaf(t.cc, f, t.cb * old[i]);
+            if (i == diagonal) f += t.ca;
+        } else {
+            f *= t.out_scale;
+        }
+        split(f, hi[i], lo[i]);
+    }
+}
+template <bool TWO> __device__ __forceinline__ void load_old(const char* a, float* old) {
+    const uint4 h = *reinterpret_cast<const uint4*>(a);
+    const uint4 l = TWO ? *reinterpret_cast<const uint4*>(a + kPlane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
+        const float2 g = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
+        old[2 * i] = f.x + g.x;
+        old[2 * i + 1] = f.y + g.y;
+    }
+}
+__device__ __forceinline__ uint4 pack8(const __half* h) {
+    return make_uint4(pack(h[0], h[1]), pack(h[2], h[3]), pack(h[4], h[5]), pack(h[6], h[7]));
+}
+
+// ---- small matrices: one 128 x 128 tile a cluster, its CTAs share the summed axis ---------------------------------
+// With few tiles the summed axis is what takes time: the CTAs of a cluster (1, 2, 4 or 8) each sum a part of it, put
+// their sums into shared memory and each finish a part of the columns, adding the parts in the order of their ranks.
+constexpr int kSmallThreads = 192, kTile = 128;
+template <int L, int R> struct SmallStages {
+    static constexpr uint32_t kLeft = L * kPlane, kRight = R * kPlane, kStage = kLeft + kRight;
+    static constexpr int kCount = (int)(196608u / kStage);
+    static constexpr uint32_t kBytes = kCount * kStage + 1024;   // alignment to 1024
+};
+
+template <bool F32, int MODE, int RIGHT>
+__global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid_constant__ Table t) {
+    using P = Planes<F32, MODE, RIGHT>;
+    constexpr int L = P::kLeft, R = P::kRight;
+    using S = SmallStages<L, R>;
+    constexpr uint32_t kTmem = F32 ? 256 : 128;   // columns: hi hi and the rest; one sum
     extern __shared__ char raw[];
-    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum[2], s_taken[2], s_drain;
+    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum, s_taken, s_last;
     __shared__ uint32_t s_tmem;
     char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int parts = (int)cluster_size(), part = (int)cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kCount; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_empty[i], 1);
+        }
+        mbar_init(&s_sum, 1);
+        mbar_init(&s_taken, 128);
+        mbar_init(&s_last, 1);
+        fence_mbar_init();
+    }
+    if (warp == 5) tmem_alloc<1>(&s_tmem, kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
+    let_next_start();
+    wait_for_previous();
+
     int block;
-    const Matrix& m = t.mat[find_matrix(t, block)];
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x / parts, block)];
     int ti, tj;
     if (MODE == kApply) {
         const int across = (m.nk + 1) / 2;
@@ -293,53 +453,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_c
     const bool same = MODE != kApply && ti == tj;      // both operands are one tile
     const char* const left = MODE == kGram ? m.x[t.from] : MODE == kSquare ? m.a : m.b;
     const char* const right = MODE == kSquare ? m.a : m.x[t.from];
-    const int blocks = MODE == kGram ? m.nk : m.mk;    // summed over
-    const int run = PLANES == 2 ? kRunBlocks : blocks, runs = (blocks + run - 1) / run;
-    const uint32_t polls = t.hooks.poll_limit;
-
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kCount; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_sum[i], 1);
-            mbar_init(&s_taken[i], 128);
-        }
-        mbar_init(&s_drain, 1);
-        fence_mbar_init();
-    }
-    if (warp == 5) tmem_alloc(&s_tmem, S::kTmem);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    constexpr uint32_t kLeftBlock = MODE == kGram ? P::kX : P::kAB, kRightBlock = MODE == kSquare ? P::kAB : P::kX;
+    const int all = MODE == kGram ? m.nk : m.mk;       // column blocks summed over, this CTA's share of them
+    const int first = all * part / parts, blocks = all * (part + 1) / parts - first;
     bool ok = true;
 
     if (warp == 4) {
         if (lane == 0) {
             int k = 0;
-            for (; k < blocks && ok; ++k) {
+            for (; k < blocks; ++k) {
                 const int st = k % S::kCount;
                 if (k >= S::kCount) ok = mbar_wait_bounded(&s_empty[st], (k / S::kCount - 1) & 1, polls);
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
-                char* const b = a + S::kOperand;
+                char* const b = a + S::kLeft;
                 if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
+                const int kb = first + k;
                 if (MODE == kApply) {
                     const int wide = 2 * tj + 1 < m.nk ? 2 : 1;            // the last tile may be one block wide
-                    mbar_arrive_expect_tx(&s_full[st], S::kOperand + PLANES * wide * (kPlane / 2));
-                    bulk_copy_g2s(a, left + ((int64_t)ti * m.mk + k) * S::kOperand, S::kOperand, &s_full[st]);
-                    for (int p = 0; p < PLANES; ++p)
+                    mbar_arrive_expect_tx(&s_full[st], S::kLeft + R * wide * (kPlane / 2));
+                    bulk_copy_g2s(a, left + ((int64_t)ti * m.mk + kb) * kLeftBlock, S::kLeft, &s_full[st]);
+                    for (int p = 0; p < R; ++p)
                         for (int w = 0; w < wide; ++w)                     // 64 rows of a block: one half of a plane
                             bulk_copy_g2s(b + (p * 2 + w) * (kPlane / 2),
-                                          right + ((int64_t)(k >> 1) * m.nk + 2 * tj + w) * S::kOperand + p * kPlane +
-                                              (k & 1) * (kPlane / 2),
+                                          right + ((int64_t)(kb >> 1) * m.nk + 2 * tj + w) * kRightBlock + p * kPlane +
+                                              (kb & 1) * (kPlane / 2),
                                           kPlane / 2, &s_full[st]);
                 } else {
-                    mbar_arrive_expect_tx(&s_full[st], same ? S::kOperand : S::kStage);
-                    bulk_copy_g2s(a, left + ((int64_t)ti * blocks + k) * S::kOperand, S::kOperand, &s_full[st]);
-                    if (!same) bulk_copy_g2s(b, right + ((int64_t)tj * blocks + k) * S::kOperand, S::kOperand, &s_full[st]);
+                    mbar_arrive_expect_tx(&s_full[st], same ? S::kLeft : S::kStage);
+                    bulk_copy_g2s(a, left + ((int64_t)ti * all + kb) * kLeftBlock, S::kLeft, &s_full[st]);
+                    if (!same) bulk_copy_g2s(b, right + ((int64_t)tj * all + kb) * kRightBlock, S::kRight, &s_full[st]);
                 }
             }
             if (!ok)   // given up: what is on its way has to land before the CTA ends
@@ -348,140 +491,381 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_c
         }
     } else if (warp == 5) {
         if (lane == 0) {
-            // D 32 bits, A and B fp16; in B X the right factor is summed across its rows (bit 16)
-            const uint32_t idesc = (1u << 4) | ((MODE == kApply ? 1u : 0u) << 16) | ((kTile / 8u) << 17) | ((128u / 16u) << 24);
-            for (int k = 0; k < blocks && ok; ++k) {
-                const int st = k % S::kCount, r = k / run, half = r & 1;
-                if (k % run == 0 && r >= 2) ok = mbar_wait_bounded(&s_taken[half], (r / 2 - 1) & 1, polls);
-                if (ok) ok = mbar_wait_bounded(&s_full[st], (k / S::kCount) & 1, polls);
+            const uint32_t idesc = instruction(MODE == kApply, 128, kTile);
+            for (int k = 0; k < blocks; ++k) {
+                const int st = k % S::kCount;
+                ok = mbar_wait_bounded(&s_full[st], (k / S::kCount) & 1, polls);
+                if (F32 && ok && k > 0) ok = mbar_wait_bounded(&s_taken, (k - 1) & 1, polls);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kOperand;
-                const uint32_t d = tmem + half * kTile;
+                const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kLeft;
+                auto at_a = [&](int p, int q) { return operand(a + p * kPlane + q * 32, 16, 1024); };
+                auto at_b = [&](int p, int q) {
+                    return MODE == kApply ? operand(b + p * kPlane + q * 2048, kPlane / 2, 1024)
+                                          : operand(b + p * kPlane + q * 32, 16, 1024);
+                };
 #pragma unroll
-                for (int q = 0; q < kCols / 16; ++q) {
-                    const bool add = k % run != 0 || q != 0;
-                    uint64_t da[PLANES], db[PLANES];
+                for (int q = 0; q < kCols / 16; ++q) tc_mma<1>(tmem, at_a(0, q), at_b(0, q), idesc, (!F32 && k != 0) || q != 0);
+                if (F32) {
+                    tc_commit<1>(&s_sum);
 #pragma unroll
-                    for (int p = 0; p < PLANES; ++p) {
-                        da[p] = operand(a + p * kPlane + q * 32, 16, 1024);
-                        db[p] = MODE == kApply ? operand(b + p * kPlane + q * 2048, kPlane / 2, 1024)
-                                               : operand(b + p * kPlane + q * 32, 16, 1024);
+                    for (int q = 0; q < kCols / 16; ++q) {
+                        tc_mma<1>(tmem + kTile, at_a(0, q), at_b(1, q), idesc, k != 0 || q != 0);
+                        tc_mma<1>(tmem + kTile, at_a(L - 1, q), at_b(0, q), idesc, true);
                     }
-                    tc_mma(d, da[0], db[0], idesc, add);
-                    if (PLANES == 2) {
-                        tc_mma(tmem + 2 * kTile, da[0], db[PLANES - 1], idesc, k != 0 || q != 0);
-                        tc_mma(tmem + 2 * kTile, da[PLANES - 1], db[0], idesc, true);
-                    }
+                } else if (R == 2) {
+#pragma unroll
+                    for (int q = 0; q < kCols / 16; ++q) tc_mma<1>(tmem, at_a(0, q), at_b(R - 1, q), idesc, true);
                 }
-                tc_commit(&s_empty[st]);
-                if (k % run == run - 1 || k == blocks - 1) tc_commit(&s_sum[half]);
+                tc_commit<1>(&s_empty[st]);
             }
-            if (!ok) {   // given up: the products that were issued end before TMEM is handed back
-                tc_commit(&s_drain);
-                mbar_wait_bounded(&s_drain, 0, polls);
-            }
+            // everything issued so far, in the good case the whole sum
+            tc_commit<1>(&s_last);
+            if (!ok) mbar_wait_bounded(&s_last, 0);
         }
     } else {
         float v[kTile];
 #pragma unroll
         for (int c = 0; c < kTile; ++c) v[c] = 0.0f;
-        for (int r = 0; r < runs && ok; ++r) {
-            ok = __all_sync(~0u, mbar_wait_bounded(&s_sum[r & 1], (r / 2) & 1, polls));
-            if (!ok) break;
-            tc_fence_after();
+        auto take = [&](uint32_t from) {
 #pragma unroll
             for (int c = 0; c < kTile; c += 32) {
                 float w[32];
-                tmem_load32(tmem + (r & 1) * kTile + c + ((uint32_t)warp << 21), w);
+                tmem_load32(tmem + from + c + ((uint32_t)warp << 21), w);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[c + i] += w[i];
             }
-            if (PLANES == 2 && r == runs - 1) {
-#pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    float w[32];
-                    tmem_load32(tmem + 2 * kTile + c + ((uint32_t)warp << 21), w);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c + i] += w[i];
-                }
+        };
+        if (F32)
+            for (int k = 0; k < blocks; ++k) {
+                ok = __all_sync(~0u, mbar_wait_bounded(&s_sum, k & 1, polls));
+                if (!ok) break;
+                tc_fence_after();
+                take(0);
+                tc_fence_before();
+                mbar_arrive(&s_taken);
             }
-            tc_fence_before();
-            mbar_arrive(&s_taken[r & 1]);
-        }
-        // every product has read its operands by now: their shared memory takes the finished tile
+        if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&s_last, 0, polls));
+        tc_fence_after();
+        if (ok && blocks > 0) take(F32 ? kTile : 0);
+        // every product has read its operands by now: their shared memory is free
         const uint32_t r = threadIdx.x;
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
         char* const out = MODE == kGram ? m.a : MODE == kSquare ? m.b : m.x[t.from ^ 1];
-        if (ok) {
+        constexpr uint32_t kOutBlock = MODE == kApply ? P::kX : P::kAB;
+        float* const sums = reinterpret_cast<float*>(smem);
+        if (parts > 1) {
 #pragma unroll
-            for (int c = 0; c < kTile; c += 8) {
-                if (2 * tj + c / kCols >= wide) continue;
-                const uint32_t o = (c / kCols) * S::kOperand + block_offset(r, c % kCols);
-                float old[8];
-                if (MODE == kSquare) {
-                    const char* a = m.a + ((int64_t)ti * m.mk + 2 * tj) * S::kOperand + o;
-                    const uint4 h = *reinterpret_cast<const uint4*>(a);
-                    const uint4 l = PLANES == 2 ? *reinterpret_cast<const uint4*>(a + kPlane) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
-                        const float2 g = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
-                        old[2 * i] = f.x + g.x;
-                        old[2 * i + 1] = f.y + g.y;
-                    }
-                }
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    __half h[2], l[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float f = v[c + i + j];
-                        if (MODE == kSquare) {
-                            f = fmaf(t.cc, f, t.cb * old[i + j]);
-                            if (same && (int)r == c + i + j && ti * kRows + (int)r < m.m) f += t.ca;
-                        } else {
-                            f *= t.out_scale;
-                        }
-                        split(f, h[j], l[j]);
-                        if (MODE != kApply && !same) {   // the mirrored tile: this thread's row is a column
-                            const uint32_t w = 2 * S::kOperand + (r / kCols) * S::kOperand + block_offset(c + i + j, r % kCols);
-                            *reinterpret_cast<__half*>(smem + w) = h[j];
-                            if (PLANES == 2) *reinterpret_cast<__half*>(smem + w + kPlane) = l[j];
-                        }
-                    }
-                    hi[i / 2] = pack(h[0], h[1]);
-                    lo[i / 2] = pack(l[0], l[1]);
-                }
-                *reinterpret_cast<uint4*>(smem + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (PLANES == 2) *reinterpret_cast<uint4*>(smem + o + kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-            fence_proxy_async_smem();
-        } else {
-            *t.fail = 1;
+            for (int c = 0; c < kTile; ++c) sums[c * 128 + r] = v[c];
         }
-        const bool all = __syncthreads_and(ok);   // (the other two warps join below)
-        if (all && threadIdx.x == 0) {
-            for (int c = 0; c < 2; ++c) {
-                if (2 * tj + c < wide)
-                    bulk_copy_s2g(out + ((int64_t)ti * wide + 2 * tj + c) * S::kOperand, smem + c * S::kOperand, S::kOperand);
-                if (MODE != kApply && !same && 2 * ti + c < wide)
-                    bulk_copy_s2g(out + ((int64_t)tj * wide + 2 * ti + c) * S::kOperand, smem + (2 + c) * S::kOperand, S::kOperand);
+        if (!ok) *t.fail = 1;
+        if (parts > 1) cluster_sync();
+        const int share = kTile / parts, from = part * share;   // columns this CTA finishes
+        // eight columns at a time; with one CTA they are in registers, where only constants can index
+        auto piece = [&](int c, const float* w) {
+            if (2 * tj + c / kCols >= wide) return;
+            char* const to = out + ((int64_t)ti * wide + 2 * tj + c / kCols) * kOutBlock + block_offset(r, c % kCols);
+            float old[8];
+            if (MODE == kSquare) load_old<F32>(m.a + (to - out), old);
+            __half hi[8], lo[8];
+            const int d = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;
+            finish<MODE>(t, w, old, d, hi, lo);
+            *reinterpret_cast<uint4*>(to) = pack8(hi);
+            if (P::kOut == 2) *reinterpret_cast<uint4*>(to + kPlane) = pack8(lo);
+            if (MODE != kApply && !same) {   // the mirrored tile: this thread's row is a column
+                char* const mirror = out + ((int64_t)tj * wide + 2 * ti + r / kCols) * kOutBlock;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t o = block_offset(c + i, r % kCols);
+                    *reinterpret_cast<__half*>(mirror + o) = hi[i];
+                    if (P::kOut == 2) *reinterpret_cast<__half*>(mirror + o + kPlane) = lo[i];
+                }
             }
-            bulk_commit_group();
-            bulk_wait_group0();
+        };
+        if (parts == 1) {
+#pragma unroll
+            for (int c = 0; c < kTile; c += 8) piece(c, v + c);
+        } else {
+            for (int c = from; c < from + share; c += 8) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = 0.0f;
+                for (int q = 0; q < parts; ++q)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] += load_shared_of(smem_u32(sums + (c + i) * 128 + r), q);
+                piece(c, w);
+            }
+            cluster_sync();   // no CTA leaves while another reads its sums
         }
     }
     if (warp >= 4) {
         if (!ok) *t.fail = 1;
         __syncwarp();
-        (void)__syncthreads_and(ok);
+        if (parts > 1) {
+            cluster_sync();
+            cluster_sync();
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_free(tmem, S::kTmem);
+    if (warp == 5) tmem_free<1>(tmem, kTmem);
+}
+
+// ---- large matrices: one 256 x N tile a pair of CTAs --------------------------------------------------------------
+// A 128 x 128 tile reads 8 KB of shared memory for every 64 cycles of products and takes 64 KB in for every 768, more
+// than its 128 bytes a cycle.  In a pair each CTA holds 128 rows of the left and N / 2 columns of the right factor, and
+// both are read by the products of both: at N = 256, 8 KB in 128 cycles.  CTA 0 issues; CTA 1's second warp passes on
+// that its tiles have arrived.
+constexpr int kPairThreads = 320;
+template <int L, int R, int N> struct PairStages {
+    static constexpr uint32_t kLeft = L * kPlane, kRight = R * (uint32_t)N / 2 * 128, kStage = kLeft + kRight;
+    static constexpr int kCount = (int)(196608u / kStage);
+    static constexpr uint32_t kBytes = kCount * kStage + 1024;
+};
+
+template <bool F32, int MODE, int RIGHT, int N>
+__global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_constant__ Table t) {
+    using P = Planes<F32, MODE, RIGHT>;
+    constexpr int L = P::kLeft, R = P::kRight, kWide = N / kCols;   // column blocks of the tile
+    using S = PairStages<L, R, N>;
+    constexpr uint32_t kTmem = F32 ? 2 * N : N;
+    extern __shared__ char raw[];
+    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum, s_taken, s_last;
+    __shared__ uint32_t s_tmem;
+    char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kCount; ++i) {
+            mbar_init(&s_full[i], rank == 0 ? 2 : 1);   // CTA 0: its own tiles, and word from CTA 1
+            mbar_init(&s_empty[i], 1);
+        }
+        mbar_init(&s_sum, 1);
+        mbar_init(&s_taken, 16);                        // the eight warps of both CTAs
+        mbar_init(&s_last, 1);
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc<2>(&s_tmem, kTmem);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
+    let_next_start();
+    wait_for_previous();
+
+    int block;
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x / 2, block)];
+    const int pairs = (m.mb + 1) / 2;                   // 256-row tiles
+    int ti, tj;
+    if (MODE == kApply) {
+        ti = block % pairs;                             // neighbours share the columns of X, the larger factor
+        tj = block / pairs;
+    } else if (N == 256) {                              // column tj of the upper triangle holds tj + 1 tiles
+        tj = (int)((sqrtf(8.0f * (float)block + 1.0f) - 1.0f) * 0.5f);
+        while ((tj + 1) * (tj + 2) / 2 <= block) ++tj;
+        while (tj * (tj + 1) / 2 > block) --tj;
+        ti = block - tj * (tj + 1) / 2;
+    } else {                                            // columns 2 h and 2 h + 1 hold h + 1 tiles each
+        int h = (int)(sqrtf((float)block + 0.25f) - 0.5f);
+        while ((h + 1) * (h + 2) <= block) ++h;
+        while (h * (h + 1) > block) --h;
+        const int in = block - h * (h + 1);
+        tj = 2 * h + in / (h + 1);
+        ti = in % (h + 1);
+    }
+    const bool same = MODE != kApply && N == 256 && ti == tj;   // both operands are one tile
+    const int row = 2 * ti + rank;                              // this CTA's block of rows
+    const char* const left = MODE == kGram ? m.x[t.from] : MODE == kSquare ? m.a : m.b;
+    const char* const right = MODE == kSquare ? m.a : m.x[t.from];
+    constexpr uint32_t kLeftBlock = MODE == kGram ? P::kX : P::kAB, kRightBlock = MODE == kSquare ? P::kAB : P::kX;
+    const int blocks = MODE == kGram ? m.nk : m.mk;
+    bool ok = true;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            // blocks behind the matrix's end are taken from its last ones; what they give is not written
+            const int lrow = min(row, m.mb - 1);
+            int k = 0;
+            for (; k < blocks; ++k) {
+                const int st = k % S::kCount;
+                if (k >= S::kCount) ok = mbar_wait_cluster(&s_empty[st], (k / S::kCount - 1) & 1, polls);
+                if (!ok) break;
+                char* const a = smem + st * S::kStage;
+                char* const b = a + S::kLeft;
+                if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
+                mbar_arrive_expect_tx(&s_full[st], same ? S::kLeft : S::kStage);
+                bulk_copy_g2s(a, left + ((int64_t)lrow * blocks + k) * kLeftBlock, S::kLeft, &s_full[st]);
+                if (MODE == kApply) {
+                    for (int p = 0; p < R; ++p)
+                        for (int w = 0; w < kWide / 2; ++w)                // 64 rows of a block: one half of a plane
+                            bulk_copy_g2s(b + (p * (kWide / 2) + w) * (kPlane / 2),
+                                          right + ((int64_t)(k >> 1) * m.nk + min(kWide * tj + kWide / 2 * rank + w, m.nk - 1)) * kRightBlock +
+                                              p * kPlane + (k & 1) * (kPlane / 2),
+                                          kPlane / 2, &s_full[st]);
+                } else if (N == 256) {
+                    if (!same)
+                        bulk_copy_g2s(b, right + ((int64_t)min(2 * tj + rank, m.mb - 1) * blocks + k) * kRightBlock, S::kRight, &s_full[st]);
+                } else {
+                    for (int p = 0; p < R; ++p)
+                        bulk_copy_g2s(b + p * (kPlane / 2),
+                                      right + ((int64_t)min(tj, m.mb - 1) * blocks + k) * kRightBlock + p * kPlane + rank * (kPlane / 2),
+                                      kPlane / 2, &s_full[st]);
+                }
+            }
+            if (!ok)
+                for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
+                    mbar_wait_cluster(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && rank == 1) {
+            for (int k = 0; k < blocks && ok; ++k) {
+                ok = mbar_wait_bounded(&s_full[k % S::kCount], (k / S::kCount) & 1, polls);
+                if (ok) mbar_arrive_at(&s_full[k % S::kCount], 0);
+            }
+        } else if (lane == 0) {
+            const uint32_t idesc = instruction(MODE == kApply, 256, N);
+            constexpr uint32_t kPlaneB = (uint32_t)N / 2 * 128;
+            for (int k = 0; k < blocks; ++k) {
+                const int st = k % S::kCount;
+                ok = mbar_wait_cluster(&s_full[st], (k / S::kCount) & 1, polls);
+                if (F32 && ok && k > 0) ok = mbar_wait_cluster(&s_taken, (k - 1) & 1, polls);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kLeft;
+                auto at_a = [&](int p, int q) { return operand(a + p * kPlane + q * 32, 16, 1024); };
+                auto at_b = [&](int p, int q) {
+                    return MODE == kApply ? operand(b + p * kPlaneB + q * 2048, kPlane / 2, 1024)
+                                          : operand(b + p * kPlaneB + q * 32, 16, 1024);
+                };
+#pragma unroll
+                for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(tmem, at_a(0, q), at_b(0, q), idesc, (!F32 && k != 0) || q != 0);
+                if (F32) {
+                    tc_commit<2>(&s_sum);
+#pragma unroll
+                    for (int q = 0; q < kCols / 16; ++q) {
+                        tc_mma<2>(tmem + N, at_a(0, q), at_b(1, q), idesc, k != 0 || q != 0);
+                        tc_mma<2>(tmem + N, at_a(L - 1, q), at_b(0, q), idesc, true);
+                    }
+                } else if (R == 2) {
+#pragma unroll
+                    for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(tmem, at_a(0, q), at_b(R - 1, q), idesc, true);
+                }
+                tc_commit<2>(&s_empty[st]);
+            }
+            tc_commit<2>(&s_last);
+            if (!ok) mbar_wait_cluster(&s_last, 0, 0);
+        }
+    } else {
+        constexpr int kPart = N / 2;                     // columns of a thread; the warps' upper half takes the right ones
+        const int half = warp >> 2;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, r = threadIdx.x & 127;
+        float v[kPart];
+#pragma unroll
+        for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
+        auto take = [&](uint32_t from) {
+#pragma unroll
+            for (int c = 0; c < kPart; c += 32) {
+                float w[32];
+                tmem_load32(tmem + from + half * kPart + c + lanes, w);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[c + i] += w[i];
+            }
+        };
+        if (F32)
+            for (int k = 0; k < blocks; ++k) {
+                ok = __all_sync(~0u, mbar_wait_cluster(&s_sum, k & 1, polls));
+                if (!ok) break;
+                tc_fence_after();
+                take(0);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(&s_taken, 0);
+            }
+        if (ok) ok = __all_sync(~0u, mbar_wait_cluster(&s_last, 0, polls));
+        tc_fence_after();
+        if (ok) take(F32 ? N : 0);
+        if (!ok) *t.fail = 1;
+        // Every product has read its operands by now: their shared memory takes the finished blocks, from where they
+        // leave as whole blocks.
+        const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
+        char* const out = MODE == kGram ? m.a : MODE == kSquare ? m.b : m.x[t.from ^ 1];
+        constexpr uint32_t kOutBlock = MODE == kApply ? P::kX : P::kAB, kOutBytes = P::kOut * kPlane;
+        const int col = kWide * tj + half * (kPart / kCols);   // first block column of this thread
+        const bool mirrored = MODE != kApply && (N == 256 ? tj > ti : tj > 2 * ti + 1);
+        // space: kPart / 64 blocks and as many mirrored ones for each half; what does not fit side by side takes turns
+        constexpr uint32_t kMine = kPart / kCols * kOutBytes, kSpace = MODE == kApply ? kMine : 2 * kMine;
+        constexpr bool kTurns = 2 * kSpace > 196608u;
+        char* const space = smem + (kTurns ? 0 : half * (N == 256 ? kSpace : kMine));
+        auto write = [&]() {
+#pragma unroll
+            for (int c = 0; c < kPart; c += 8) {
+                if (col + c / kCols >= wide || row >= m.mb) continue;
+                const uint32_t o = block_offset(r, c % kCols);
+                float old[8];
+                if (MODE == kSquare) load_old<F32>(m.a + ((int64_t)row * wide + col + c / kCols) * kOutBlock + o, old);
+                __half hi[8], lo[8];
+                const int d = (int)r + row * kRows - (col * kCols + c);   // the diagonal's place in this piece
+                finish<MODE>(t, v + c, old, row * kRows + (int)r < m.m ? d : -1, hi, lo);
+                *reinterpret_cast<uint4*>(space + (c / kCols) * kOutBytes + o) = pack8(hi);
+                if (P::kOut == 2) *reinterpret_cast<uint4*>(space + (c / kCols) * kOutBytes + o + kPlane) = pack8(lo);
+                if (MODE != kApply && mirrored) {
+                    // N 256: rows of one block, columns of the two blocks that the rows r belong to.  N 128: a half's 64
+                    // columns are 64 rows of a block, the two halves' rows follow one another.
+                    char* const to = N == 256 ? space + kMine + (r / kCols) * kOutBytes
+                                              : smem + 2 * kMine + (r / kCols) * kOutBytes;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t w = block_offset((N == 256 ? 0 : half * kCols) + c + i, r % kCols);
+                        *reinterpret_cast<__half*>(to + w) = hi[i];
+                        if (P::kOut == 2) *reinterpret_cast<__half*>(to + w + kPlane) = lo[i];
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+        };
+        // one thread of each half sends its blocks
+        auto send = [&]() {
+            for (int c = 0; c < kPart / kCols; ++c)
+                if (col + c < wide) bulk_copy_s2g(out + ((int64_t)row * wide + col + c) * kOutBlock, space + c * kOutBytes, kOutBytes);
+            if (MODE != kApply && mirrored) {
+                if (N == 256) {
+                    const int to = 2 * tj + half;
+                    for (int c = 0; c < 2; ++c)
+                        if (to < m.mb)
+                            bulk_copy_s2g(out + ((int64_t)to * wide + 2 * row + c) * kOutBlock, space + kMine + c * kOutBytes, kOutBytes);
+                } else if (tj < m.mb) {   // this half's block column of the mirrored tile
+                    bulk_copy_s2g(out + ((int64_t)tj * wide + 2 * row + half) * kOutBlock, smem + 2 * kMine + half * kOutBytes, kOutBytes);
+                }
+            }
+            bulk_commit_group();
+            bulk_wait_group0();
+        };
+        auto all_warps = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        const bool sender = ok && (threadIdx.x & 127) == 0 && row < m.mb;
+        if (kTurns) {
+            for (int turn = 0; turn < 2; ++turn) {
+                if (half == turn) write();
+                all_warps();
+                if (half == turn && sender) send();
+                all_warps();
+            }
+        } else {
+            write();
+            all_warps();
+            if (sender) send();
+        }
+    }
+    if (warp >= 8) {
+        if (!ok) *t.fail = 1;
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // neither CTA leaves, or frees TMEM, while the other may still use it
+    tc_fence_after();
+    if (warp == 9) tmem_free<2>(tmem, kTmem);
+    cluster_sync();
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -498,7 +882,7 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.mb = (p.m + kRows - 1) / kRows;
     p.mk = (p.m + kCols - 1) / kCols;
     p.nk = (p.n + kCols - 1) / kCols;
-    p.x = (size_t)p.mb * p.nk * planes * kPlane;
+    p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
     p.norms = up256((size_t)div_up64(d.rows * d.cols, kNormChunk) * 8);
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.norms;
@@ -574,15 +958,79 @@ int32_t check(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     return D3GS_OK;
 }
 
-template <int PLANES, int MODE> int32_t launch_product(const Table& t, unsigned grid, cudaStream_t st) {
-    D3GS_CUDA(cudaFuncSetAttribute(ns_gemm_kernel<PLANES, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)Stages<PLANES>::kBytes));
-    ns_gemm_kernel<PLANES, MODE><<<grid, kGemmThreads, Stages<PLANES>::kBytes, st>>>(t);
-    D3GS_LAUNCH_CHECK("ns_gemm_kernel");
+template <typename K>
+int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
+               const Table& t) {
+    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = 2;
+    D3GS_CUDA(cudaLaunchKernelEx(&c, kernel, t));
+    D3GS_LAUNCH_CHECK(name);
     return D3GS_OK;
 }
 
-template <int PLANES>
+// How the products of a list of matrices are cut.  Pairs of CTAs when the largest short side is above kPairFrom.
+constexpr int kPairFrom = 384;
+struct Shape {
+    bool pair;
+};
+Shape shape_of(const Table& t) {
+    Shape s{};
+    for (int k = 0; k < t.count; ++k) s.pair |= t.mat[k].m > kPairFrom;
+    return s;
+}
+
+template <bool F32, int MODE, int RIGHT, typename B>
+int32_t product_of(const Table& t, const Shape& shape, B& blocks, cudaStream_t st) {
+    constexpr int L = Planes<F32, MODE, RIGHT>::kLeft;
+    if (!shape.pair) {
+        const unsigned tiles = blocks([](const Matrix& m) {
+            return MODE == kApply ? (int64_t)m.mb * ((m.nk + 1) / 2) : (int64_t)m.mb * (m.mb + 1) / 2;
+        });
+        // as many CTAs a tile as the machine has room for, none without four blocks to sum
+        int longest = 0;
+        for (int k = 0; k < t.count; ++k) longest = max(longest, MODE == kGram ? t.mat[k].nk : t.mat[k].mk);
+        unsigned parts = 1;
+        while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
+        return launch(ns_small_kernel<F32, MODE, RIGHT>, "ns_small_kernel", tiles * parts, kSmallThreads,
+                      SmallStages<L, RIGHT>::kBytes, parts, st, t);
+    }
+    // 256 x 256 tiles move the least; 256 x 128 ones when those would leave SMs idle
+    const unsigned tiles = blocks([](const Matrix& m) {
+        const int64_t pairs = (m.mb + 1) / 2;
+        return MODE == kApply ? pairs * ((m.nk + 3) / 4) : pairs * (pairs + 1) / 2;
+    });
+    if (tiles * 2 > 100)
+        return launch(ns_pair_kernel<F32, MODE, RIGHT, 256>, "ns_pair_kernel", tiles * 2, kPairThreads,
+                      PairStages<L, RIGHT, 256>::kBytes, 2, st, t);
+    const unsigned narrow = blocks([](const Matrix& m) {
+        const int64_t pairs = (m.mb + 1) / 2;
+        return MODE == kApply ? pairs * ((m.nk + 1) / 2) : pairs * (pairs + 1);
+    });
+    return launch(ns_pair_kernel<F32, MODE, RIGHT, 128>, "ns_pair_kernel", narrow * 2, kPairThreads,
+                  PairStages<L, RIGHT, 128>::kBytes, 2, st, t);
+}
+template <bool F32, int MODE, typename B>
+int32_t product(Table& t, const Shape& shape, B& blocks, cudaStream_t st) {
+    // (blocks writes the table's first_block)
+    if constexpr (F32) return product_of<true, MODE, 2>(t, shape, blocks, st);
+    else if constexpr (MODE == kApply)
+        return t.last ? product_of<false, MODE, 1>(t, shape, blocks, st) : product_of<false, MODE, 2>(t, shape, blocks, st);
+    else return product_of<false, MODE, 1>(t, shape, blocks, st);
+}
+
+template <bool F32>
 int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg, bool muon, const Scales& sc, void* ws,
             cudaStream_t st) {
     char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
@@ -601,7 +1049,7 @@ int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& c
         for (; i < count && t.count < kMaxMatrices; ++i) {
             const D3gsOrthoMatrix& d = mats[i];
             if (d.rows == 0 || d.cols == 0) continue;
-            const Parts p = parts_of(d, PLANES);
+            const Parts p = parts_of(d, F32 ? 2 : 1);
             Matrix& m = t.mat[t.count++];
             m.src = d.src;
             m.momentum = muon ? d.momentum : nullptr;
@@ -635,29 +1083,26 @@ int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& c
         auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
         t.from = 0;
         unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * m.cols, kNormChunk); });
-        ns_norm_kernel<<<grid, kThreads, 0, st>>>(t);
-        D3GS_LAUNCH_CHECK("ns_norm_kernel");
+        if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, t)) return rc;
         t.out_scale = sc.x[0];
         grid = blocks(every_block);
-        ns_load_kernel<PLANES><<<grid, kThreads, 0, st>>>(t);
-        D3GS_LAUNCH_CHECK("ns_load_kernel");
+        if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, t)) return rc;
+        const Shape shape = shape_of(t);
         for (int s = 0; s < cfg.steps; ++s) {
-            grid = blocks([](const Matrix& m) { return (int64_t)m.mb * (m.mb + 1) / 2; });
+            t.last = s == cfg.steps - 1;
             t.out_scale = sc.a[s] / (sc.x[s] * sc.x[s]);
-            if (int32_t rc = launch_product<PLANES, kGram>(t, grid, st)) return rc;
+            if (int32_t rc = product<F32, kGram>(t, shape, blocks, st)) return rc;
             t.ca = cfg.coefficients[s][0] * sc.b[s];
             t.cb = cfg.coefficients[s][1] * (sc.b[s] / sc.a[s]);
             t.cc = cfg.coefficients[s][2] * (sc.b[s] / sc.a[s] / sc.a[s]);
-            if (int32_t rc = launch_product<PLANES, kSquare>(t, grid, st)) return rc;
+            if (int32_t rc = product<F32, kSquare>(t, shape, blocks, st)) return rc;
             t.out_scale = sc.x[s + 1] / sc.b[s] / sc.x[s];
-            grid = blocks([](const Matrix& m) { return (int64_t)m.mb * ((m.nk + 1) / 2); });
-            if (int32_t rc = launch_product<PLANES, kApply>(t, grid, st)) return rc;
+            if (int32_t rc = product<F32, kApply>(t, shape, blocks, st)) return rc;
             t.from ^= 1;
         }
         t.out_scale = 1.0f / sc.x[cfg.steps];
         grid = blocks(every_block);
-        ns_store_kernel<PLANES><<<grid, kThreads, 0, st>>>(t);
-        D3GS_LAUNCH_CHECK("ns_store_kernel");
+        if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, t)) return rc;
     }
     return D3GS_OK;
 }
@@ -672,7 +1117,8 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     D3GS_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= workspace_of(mats, count, *cfg),
                  "%s: workspace missing, unaligned or smaller than d3gs_orthogonalize_workspace_bytes", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return planes_of(*cfg) == 2 ? run<2>(mats, count, *cfg, muon, sc, ws, st) : run<1>(mats, count, *cfg, muon, sc, ws, st);
+    return cfg->dtype == D3GS_DTYPE_F32 ? run<true>(mats, count, *cfg, muon, sc, ws, st)
+                                        : run<false>(mats, count, *cfg, muon, sc, ws, st);
 }
 
 }  // namespace

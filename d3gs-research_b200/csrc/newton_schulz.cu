@@ -281,31 +281,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// the same barrier in CTA `rank` of the cluster
+// The same barrier in CTA `rank` of the cluster.  What it orders are tensor-core and bulk-copy accesses, never plain
+// ones, so no cluster-wide release is asked for (the fence that it costs held the products of a pair up by a factor of
+// two: 1.6 k cycles a column block of 512 cycles of products).
 __device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
     asm volatile(
         "{\n\t.reg .b32 a;\n\t"
         "mapa.shared::cluster.u32 a, %0, %1;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)),
+        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)),
         "r"(rank)
         : "memory");
-}
-// a wait for arrivals from other CTAs of the cluster, bounded like mbar_wait_bounded
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
-    const uint32_t polls = limit != 0 ? limit : (1u << 22);
-    for (uint32_t it = 0; it < polls; ++it) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if (it > 64) __nanosleep(64);
-    }
-    return false;
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -689,7 +674,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             int k = 0;
             for (; k < blocks; ++k) {
                 const int st = k % S::kCount;
-                if (k >= S::kCount) ok = mbar_wait_cluster(&s_empty[st], (k / S::kCount - 1) & 1, polls);
+                if (k >= S::kCount) ok = mbar_wait_bounded(&s_empty[st], (k / S::kCount - 1) & 1, polls);
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
@@ -715,7 +700,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             }
             if (!ok)
                 for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
-                    mbar_wait_cluster(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+                    mbar_wait_bounded(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
         }
     } else if (warp == 9) {
         if (lane == 0 && rank == 1) {
@@ -728,8 +713,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             constexpr uint32_t kPlaneB = (uint32_t)N / 2 * 128;
             for (int k = 0; k < blocks; ++k) {
                 const int st = k % S::kCount;
-                ok = mbar_wait_cluster(&s_full[st], (k / S::kCount) & 1, polls);
-                if (F32 && ok && k > 0) ok = mbar_wait_cluster(&s_taken, (k - 1) & 1, polls);
+                ok = mbar_wait_bounded(&s_full[st], (k / S::kCount) & 1, polls);
+                if (F32 && ok && k > 0) ok = mbar_wait_bounded(&s_taken, (k - 1) & 1, polls);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kLeft;
@@ -754,7 +739,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 tc_commit<2>(&s_empty[st]);
             }
             tc_commit<2>(&s_last);
-            if (!ok) mbar_wait_cluster(&s_last, 0, 0);
+            if (!ok) mbar_wait_bounded(&s_last, 0, 0);
         }
     } else {
         constexpr int kPart = N / 2;                     // columns of a thread; the warps' upper half takes the right ones
@@ -774,7 +759,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         };
         if (F32)
             for (int k = 0; k < blocks; ++k) {
-                ok = __all_sync(~0u, mbar_wait_cluster(&s_sum, k & 1, polls));
+                ok = __all_sync(~0u, mbar_wait_bounded(&s_sum, k & 1, polls));
                 if (!ok) break;
                 tc_fence_after();
                 take(0);
@@ -782,7 +767,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(&s_taken, 0);
             }
-        if (ok) ok = __all_sync(~0u, mbar_wait_cluster(&s_last, 0, polls));
+        if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&s_last, 0, polls));
         tc_fence_after();
         if (ok) take(F32 ? N : 0);
         if (!ok) *t.fail = 1;

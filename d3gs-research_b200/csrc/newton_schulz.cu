@@ -4,6 +4,11 @@
 //   each step: A = X X^T,  B = a I + b A + c A A,  X <- B X
 //   result X, or param <- decay param - rate X
 //
+// B - a I is one product: with V = A + b/c I it is c A V, so that nothing but products and a shifted diagonal is needed.
+// V is A but for the blocks on its diagonal, which are kept twice.  (c = 0: B = a I + b A, and no second product.)
+// Shifting both factors, c S S with S = A + b/(2c) I, would need no second blocks, but its sums are of size one where
+// b A + c A A is small, and lost twice the accuracy of 32-bit matrices up to 256 x 256.
+//
 // All matrices of a call go through the same launches: a table in the kernel arguments maps CTAs to matrices.
 //
 // The products run on the tensor cores (tcgen05, 32-bit sums in TMEM).  Their operands are fp16 with a power-of-two
@@ -45,6 +50,7 @@ struct Matrix {
     void* dst;
     int64_t src_stride;   // values between rows
     char *x[2], *a, *b;   // blocks of X (two buffers), A, B
+    char* v;              // V's blocks on the diagonal: two for each block of rows
     double* norms;        // sums of squares of the norm pass
     int32_t rows, cols;
     int32_t m, n;         // short and long side
@@ -59,9 +65,9 @@ struct Table {
     float eps, mu, decay;
     int32_t nesterov;
     int32_t from;         // which of x[] holds X
-    float ca, cb, cc;     // this step's coefficients, by the scales of what they multiply (see scales_of)
     float out_scale;      // of a product's result; of X in the first and the last pass
-    int32_t last;         // the last step
+    float shift;          // added on the diagonal of V or B
+    int32_t cubic;        // c = 0: the first product gives B
     uint32_t* fail;       // set when a bounded wait ran out: the last pass then writes NaN
     TestHooks hooks;
 };
@@ -316,14 +322,21 @@ __device__ __forceinline__ float load_shared_of(uint32_t at, uint32_t rank) {
         : "memory");
     return v;
 }
-__device__ __forceinline__ void bulk_wait_group0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// mbar_wait_bounded without its sleep: a wait here is a link of the chain that every column block goes through.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint32_t limit = 0) {
+    const uint32_t polls = limit != 0 ? limit : (1u << 24);
+    for (uint32_t it = 0; it < polls; ++it)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
+}
 
 // Shared-memory operand in 128-byte rows with the 16-byte pieces exchanged (swizzle mode 2).  Summed along the rows:
-// eight rows are 1024 bytes apart (`group`), `next` is not used.  Summed across the rows: `group` is the distance of
-// the next eight summed rows, `next` that of the next 64 columns.
-__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t next, uint32_t group) {
-    return (uint64_t)((at >> 4) & 0x3fffu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
+// eight rows are 1024 bytes apart, `next` is not used.  Summed across the rows: the next eight summed rows are 1024
+// bytes apart, the next 64 columns `next`.  The low word holds the address: moving by n bytes adds n / 16 to it.
+__device__ __forceinline__ uint32_t operand_low(uint32_t at, uint32_t next) { return (at >> 4) | ((next >> 4) << 16); }
+__device__ __forceinline__ uint64_t operand(uint32_t low) {
+    return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | low;
 }
 // D 32 bits, A and B fp16; B X sums its right factor across the rows (bit 16)
 __device__ __forceinline__ uint32_t instruction(bool across, uint32_t rows, uint32_t cols) {
@@ -343,7 +356,7 @@ __device__ __forceinline__ uint32_t instruction(bool across, uint32_t rows, uint
 // column block of A and B hold anything: nothing sums over them, and no valid row or column reads them.
 enum { kGram = 0, kSquare = 1, kApply = 2 };
 
-// What the products of a mode read: planes of the left and the right factor and of the result, and how many planes lie
+// What the products of a mode of large matrices read: planes of the left and the right factor and of the result, and how many planes lie
 // between blocks of A and B.  RIGHT is 1 in the last step of 16-bit matrices.
 template <bool F32, int MODE, int RIGHT> struct Planes {
     static constexpr int kLeft = F32 ? 2 : 1;
@@ -352,54 +365,61 @@ template <bool F32, int MODE, int RIGHT> struct Planes {
     static constexpr uint32_t kAB = (F32 ? 2 : 1) * kPlane, kX = 2 * kPlane;   // bytes of one block
 };
 
-// One 16-byte piece of a result: eight columns of a row, from sums to planes.  `old`: A at the same place (kSquare).
-template <int MODE> __device__ __forceinline__ void finish(const Table& t, const float* v, const float* old, int diagonal,
-                                                           __half* hi, __half* lo) {
+// A pair of values as pairs of fp16: hi and what hi's rounding left.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// One 16-byte piece of a result: eight columns of a row, from sums to planes; `diagonal`: which of them takes the shift.
+__device__ __forceinline__ void finish(const Table& t, const float* v, int diagonal, uint32_t* hi, uint32_t* lo) {
+    float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float f = v[i];
-        if (MODE == kSquare) {
-            f = fmaf(t.cc, f, t.cb * old[i]);
-            if (i == diagonal) f += t.ca;
-        } else {
-            f *= t.out_scale;
+    for (int i = 0; i < 8; ++i) f[i] = fmaf(v[i], t.out_scale, i == diagonal ? t.shift : 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(f[2 * i], f[2 * i + 1], hi[i], lo[i]);
+}
+template <bool TWO> __device__ __forceinline__ void put(char* at, const uint32_t* hi, const uint32_t* lo) {
+    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (TWO) *reinterpret_cast<uint4*>(at + kPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+// Eight columns of this thread's row into the mirrored tile, where they are eight rows.  Neighbouring threads hold
+// neighbouring columns there: they exchange values and write two at a time.  row0: the first of the eight rows, even.
+template <bool TWO> __device__ __forceinline__ void write_mirrored(char* block, uint32_t row0, uint32_t col, const uint32_t* hi,
+                                                                   const uint32_t* lo) {
+    const bool odd = col & 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // rows row0 + 2 i and the next one
+        const uint32_t o = block_offset(row0 + 2 * i + (odd ? 1 : 0), col & ~1u);
+        // an even thread keeps its first value and takes the neighbour's first, an odd one the second ones
+        const uint32_t h = __shfl_xor_sync(~0u, hi[i], 1);
+        *reinterpret_cast<uint32_t*>(block + o) = odd ? __byte_perm(h, hi[i], 0x7632) : __byte_perm(hi[i], h, 0x5410);
+        if (TWO) {
+            const uint32_t l = __shfl_xor_sync(~0u, lo[i], 1);
+            *reinterpret_cast<uint32_t*>(block + kPlane + o) = odd ? __byte_perm(l, lo[i], 0x7632) : __byte_perm(lo[i], l, 0x5410);
         }
-        split(f, hi[i], lo[i]);
     }
-}
-template <bool TWO> __device__ __forceinline__ void load_old(const char* a, float* old) {
-    const uint4 h = *reinterpret_cast<const uint4*>(a);
-    const uint4 l = TWO ? *reinterpret_cast<const uint4*>(a + kPlane) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
-        const float2 g = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
-        old[2 * i] = f.x + g.x;
-        old[2 * i + 1] = f.y + g.y;
-    }
-}
-__device__ __forceinline__ uint4 pack8(const __half* h) {
-    return make_uint4(pack(h[0], h[1]), pack(h[2], h[3]), pack(h[4], h[5]), pack(h[6], h[7]));
 }
 
 // ---- small matrices: one 128 x 128 tile a cluster, its CTAs share the summed axis ---------------------------------
 // With few tiles the summed axis is what takes time: the CTAs of a cluster (1, 2, 4 or 8) each sum a part of it, put
 // their sums into shared memory and each finish a part of the columns, adding the parts in the order of their ranks.
 constexpr int kSmallThreads = 192, kTile = 128;
-template <int L, int R> struct SmallStages {
-    static constexpr uint32_t kLeft = L * kPlane, kRight = R * kPlane, kStage = kLeft + kRight;
-    static constexpr int kCount = (int)(196608u / kStage);
+struct SmallStages {
+    static constexpr uint32_t kLeft = 2 * kPlane, kRight = 2 * kPlane, kStage = kLeft + kRight;
+    static constexpr int kCount = 3;
     static constexpr uint32_t kBytes = kCount * kStage + 1024;   // alignment to 1024
 };
 
-template <bool F32, int MODE, int RIGHT>
+template <int MODE>
 __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid_constant__ Table t) {
-    using P = Planes<F32, MODE, RIGHT>;
-    constexpr int L = P::kLeft, R = P::kRight;
-    using S = SmallStages<L, R>;
-    constexpr uint32_t kTmem = F32 ? 256 : 128;   // columns: hi hi and the rest; one sum
+    using S = SmallStages;
+    constexpr uint32_t kBlock = 2 * kPlane;   // every operand has two planes
+    constexpr uint32_t kTmem = 512;           // columns: hi hi twice, and the rest
     extern __shared__ char raw[];
-    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum, s_taken, s_last;
+    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum[2], s_taken[2], s_last;
     __shared__ uint32_t s_tmem;
     char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -409,8 +429,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             mbar_init(&s_full[i], 1);
             mbar_init(&s_empty[i], 1);
         }
-        mbar_init(&s_sum, 1);
-        mbar_init(&s_taken, 128);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_sum[i], 1);
+            mbar_init(&s_taken[i], 128);
+        }
         mbar_init(&s_last, 1);
         fence_mbar_init();
     }
@@ -419,9 +441,6 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
-    let_next_start();
-    wait_for_previous();
-
     int block;
     const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x / parts, block)];
     int ti, tj;
@@ -438,17 +457,18 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     const bool same = MODE != kApply && ti == tj;      // both operands are one tile
     const char* const left = MODE == kGram ? m.x[t.from] : MODE == kSquare ? m.a : m.b;
     const char* const right = MODE == kSquare ? m.a : m.x[t.from];
-    constexpr uint32_t kLeftBlock = MODE == kGram ? P::kX : P::kAB, kRightBlock = MODE == kSquare ? P::kAB : P::kX;
     const int all = MODE == kGram ? m.nk : m.mk;       // column blocks summed over, this CTA's share of them
     const int first = all * part / parts, blocks = all * (part + 1) / parts - first;
     bool ok = true;
+    let_next_start();
+    wait_for_previous();
 
     if (warp == 4) {
         if (lane == 0) {
             int k = 0;
             for (; k < blocks; ++k) {
                 const int st = k % S::kCount;
-                if (k >= S::kCount) ok = mbar_wait_bounded(&s_empty[st], (k / S::kCount - 1) & 1, polls);
+                if (k >= S::kCount) ok = wait_for(&s_empty[st], (k / S::kCount - 1) & 1, polls);
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
@@ -456,57 +476,56 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 const int kb = first + k;
                 if (MODE == kApply) {
                     const int wide = 2 * tj + 1 < m.nk ? 2 : 1;            // the last tile may be one block wide
-                    mbar_arrive_expect_tx(&s_full[st], S::kLeft + R * wide * (kPlane / 2));
-                    bulk_copy_g2s(a, left + ((int64_t)ti * m.mk + kb) * kLeftBlock, S::kLeft, &s_full[st]);
-                    for (int p = 0; p < R; ++p)
+                    mbar_arrive_expect_tx(&s_full[st], S::kLeft + 2 * wide * (kPlane / 2));
+                    bulk_copy_g2s(a, left + ((int64_t)ti * m.mk + kb) * kBlock, S::kLeft, &s_full[st]);
+                    for (int p = 0; p < 2; ++p)
                         for (int w = 0; w < wide; ++w)                     // 64 rows of a block: one half of a plane
                             bulk_copy_g2s(b + (p * 2 + w) * (kPlane / 2),
-                                          right + ((int64_t)(kb >> 1) * m.nk + 2 * tj + w) * kRightBlock + p * kPlane +
+                                          right + ((int64_t)(kb >> 1) * m.nk + 2 * tj + w) * kBlock + p * kPlane +
                                               (kb & 1) * (kPlane / 2),
                                           kPlane / 2, &s_full[st]);
                 } else {
-                    mbar_arrive_expect_tx(&s_full[st], same ? S::kLeft : S::kStage);
-                    bulk_copy_g2s(a, left + ((int64_t)ti * all + kb) * kLeftBlock, S::kLeft, &s_full[st]);
-                    if (!same) bulk_copy_g2s(b, right + ((int64_t)tj * all + kb) * kRightBlock, S::kRight, &s_full[st]);
+                    const bool v = MODE == kSquare && kb >> 1 == tj, shared = same && !v;
+                    mbar_arrive_expect_tx(&s_full[st], shared ? S::kLeft : S::kStage);
+                    bulk_copy_g2s(a, left + ((int64_t)ti * all + kb) * kBlock, S::kLeft, &s_full[st]);
+                    if (!shared)
+                        bulk_copy_g2s(b, v ? m.v + (int64_t)kb * kBlock : right + ((int64_t)tj * all + kb) * kBlock, S::kRight,
+                                      &s_full[st]);
                 }
             }
             if (!ok)   // given up: what is on its way has to land before the CTA ends
                 for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
-                    mbar_wait_bounded(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+                    wait_for(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
         }
     } else if (warp == 5) {
         if (lane == 0) {
             const uint32_t idesc = instruction(MODE == kApply, 128, kTile);
+            constexpr uint32_t kStep = (MODE == kApply ? 2048 : 32) / 16, kNext = MODE == kApply ? kPlane / 2 : 16;
+            const uint32_t a0 = operand_low(smem_u32(smem), 16), b0 = operand_low(smem_u32(smem) + S::kLeft, kNext);
+            int st = 0, phase = 0;
             for (int k = 0; k < blocks; ++k) {
-                const int st = k % S::kCount;
-                ok = mbar_wait_bounded(&s_full[st], (k / S::kCount) & 1, polls);
-                if (F32 && ok && k > 0) ok = mbar_wait_bounded(&s_taken, (k - 1) & 1, polls);
+                const int buf = k & 1;
+                ok = wait_for(&s_full[st], phase, polls);
+                if (ok && k > 1) ok = wait_for(&s_taken[buf], ((k >> 1) - 1) & 1, polls);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kLeft;
-                auto at_a = [&](int p, int q) { return operand(a + p * kPlane + q * 32, 16, 1024); };
-                auto at_b = [&](int p, int q) {
-                    return MODE == kApply ? operand(b + p * kPlane + q * 2048, kPlane / 2, 1024)
-                                          : operand(b + p * kPlane + q * 32, 16, 1024);
-                };
+                const bool shared = same && !(MODE == kSquare && (first + k) >> 1 == tj);
+                const uint32_t a = a0 + st * (S::kStage / 16), b = shared ? a : b0 + st * (S::kStage / 16);
+                const uint32_t d = tmem + buf * kTile;
 #pragma unroll
-                for (int q = 0; q < kCols / 16; ++q) tc_mma<1>(tmem, at_a(0, q), at_b(0, q), idesc, (!F32 && k != 0) || q != 0);
-                if (F32) {
-                    tc_commit<1>(&s_sum);
+                for (int q = 0; q < kCols / 16; ++q) tc_mma<1>(d, operand(a + q * 2), operand(b + q * kStep), idesc, q != 0);
+                tc_commit<1>(&s_sum[buf]);
 #pragma unroll
-                    for (int q = 0; q < kCols / 16; ++q) {
-                        tc_mma<1>(tmem + kTile, at_a(0, q), at_b(1, q), idesc, k != 0 || q != 0);
-                        tc_mma<1>(tmem + kTile, at_a(L - 1, q), at_b(0, q), idesc, true);
-                    }
-                } else if (R == 2) {
-#pragma unroll
-                    for (int q = 0; q < kCols / 16; ++q) tc_mma<1>(tmem, at_a(0, q), at_b(R - 1, q), idesc, true);
+                for (int q = 0; q < kCols / 16; ++q) {
+                    tc_mma<1>(tmem + 2 * kTile, operand(a + q * 2), operand(b + kPlane / 16 + q * kStep), idesc, k != 0 || q != 0);
+                    tc_mma<1>(tmem + 2 * kTile, operand(a + kPlane / 16 + q * 2), operand(b + q * kStep), idesc, true);
                 }
                 tc_commit<1>(&s_empty[st]);
+                if (++st == S::kCount) st = 0, phase ^= 1;
             }
             // everything issued so far, in the good case the whole sum
             tc_commit<1>(&s_last);
-            if (!ok) mbar_wait_bounded(&s_last, 0);
+            if (!ok) wait_for(&s_last, 0);
         }
     } else {
         float v[kTile];
@@ -521,24 +540,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 for (int i = 0; i < 32; ++i) v[c + i] += w[i];
             }
         };
-        if (F32)
-            for (int k = 0; k < blocks; ++k) {
-                ok = __all_sync(~0u, mbar_wait_bounded(&s_sum, k & 1, polls));
-                if (!ok) break;
-                tc_fence_after();
-                take(0);
-                tc_fence_before();
-                mbar_arrive(&s_taken);
-            }
-        if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&s_last, 0, polls));
+        for (int k = 0; k < blocks; ++k) {
+            ok = __all_sync(~0u, wait_for(&s_sum[k & 1], (k >> 1) & 1, polls));
+            if (!ok) break;
+            tc_fence_after();
+            take((k & 1) * kTile);
+            tc_fence_before();
+            mbar_arrive(&s_taken[k & 1]);
+        }
+        if (ok) ok = __all_sync(~0u, wait_for(&s_last, 0, polls));
         tc_fence_after();
-        if (ok && blocks > 0) take(F32 ? kTile : 0);
+        if (ok && blocks > 0) take(2 * kTile);
         // every product has read its operands by now: their shared memory is free
         const uint32_t r = threadIdx.x;
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
-        char* const out = MODE == kGram ? m.a : MODE == kSquare ? m.b : m.x[t.from ^ 1];
-        constexpr uint32_t kOutBlock = MODE == kApply ? P::kX : P::kAB;
-        float* const sums = reinterpret_cast<float*>(smem);
+        char* const out = MODE == kGram && !t.cubic ? m.a : MODE != kApply ? m.b : m.x[t.from ^ 1];
+            float* const sums = reinterpret_cast<float*>(smem);
         if (parts > 1) {
 #pragma unroll
             for (int c = 0; c < kTile; ++c) sums[c * 128 + r] = v[c];
@@ -549,23 +566,18 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         // eight columns at a time; with one CTA they are in registers, where only constants can index
         auto piece = [&](int c, const float* w) {
             if (2 * tj + c / kCols >= wide) return;
-            char* const to = out + ((int64_t)ti * wide + 2 * tj + c / kCols) * kOutBlock + block_offset(r, c % kCols);
-            float old[8];
-            if (MODE == kSquare) load_old<F32>(m.a + (to - out), old);
-            __half hi[8], lo[8];
-            const int d = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;
-            finish<MODE>(t, w, old, d, hi, lo);
-            *reinterpret_cast<uint4*>(to) = pack8(hi);
-            if (P::kOut == 2) *reinterpret_cast<uint4*>(to + kPlane) = pack8(lo);
-            if (MODE != kApply && !same) {   // the mirrored tile: this thread's row is a column
-                char* const mirror = out + ((int64_t)tj * wide + 2 * ti + r / kCols) * kOutBlock;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t o = block_offset(c + i, r % kCols);
-                    *reinterpret_cast<__half*>(mirror + o) = hi[i];
-                    if (P::kOut == 2) *reinterpret_cast<__half*>(mirror + o + kPlane) = lo[i];
-                }
+            char* const to = out + ((int64_t)ti * wide + 2 * tj + c / kCols) * kBlock + block_offset(r, c % kCols);
+            uint32_t hi[4], lo[4];
+            const int on = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;   // diagonal
+            finish(t, w, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+            put<true>(to, hi, lo);
+            if (MODE == kGram && same && !t.cubic) {
+                uint32_t vh[4], vl[4];
+                finish(t, w, on, vh, vl);
+                put<true>(m.v + (int64_t)(2 * ti + c / kCols) * kBlock + block_offset(r, c % kCols), vh, vl);
             }
+            if (MODE != kApply && !same)   // the mirrored tile: this thread's row is a column
+                write_mirrored<true>(out + ((int64_t)tj * wide + 2 * ti + r / kCols) * kBlock, c, r % kCols, hi, lo);
         };
         if (parts == 1) {
 #pragma unroll
@@ -605,7 +617,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
 constexpr int kPairThreads = 320;
 template <int L, int R, int N> struct PairStages {
     static constexpr uint32_t kLeft = L * kPlane, kRight = R * (uint32_t)N / 2 * 128, kStage = kLeft + kRight;
-    static constexpr int kCount = (int)(196608u / kStage);
+    // A commit takes the issuing thread about 400 cycles.  Where a column block is 256 or 512 cycles of products one
+    // commit hands back two stages.
+    static constexpr int kGroup = L == 1 && R == 1 ? 2 : 1;
+    static constexpr int kCount = (int)(196608u / kStage) / kGroup * kGroup;
     static constexpr uint32_t kBytes = kCount * kStage + 1024;
 };
 
@@ -614,9 +629,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     using P = Planes<F32, MODE, RIGHT>;
     constexpr int L = P::kLeft, R = P::kRight, kWide = N / kCols;   // column blocks of the tile
     using S = PairStages<L, R, N>;
-    constexpr uint32_t kTmem = F32 ? 2 * N : N;
+    constexpr int kSums = N == 128 ? 2 : 1;              // sums of hi hi in TMEM: as many as it has room for
+    // With two of them a commit says both that a block's hi hi is there and that the stage of the block before is free.
+    // The loading thread may look at it late: one barrier a stage, so that none completes twice before it has looked.
+    constexpr bool kOneCommit = F32 && kSums == 2;
+    constexpr int kSumBars = kOneCommit ? S::kCount : 1;
+    constexpr uint32_t kTmem = F32 ? 512 : N;
     extern __shared__ char raw[];
-    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum, s_taken, s_last;
+    __shared__ uint64_t s_full[S::kCount], s_empty[S::kCount], s_sum[kSumBars], s_taken[kSums], s_last;
     __shared__ uint32_t s_tmem;
     char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
@@ -625,8 +645,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             mbar_init(&s_full[i], rank == 0 ? 2 : 1);   // CTA 0: its own tiles, and word from CTA 1
             mbar_init(&s_empty[i], 1);
         }
-        mbar_init(&s_sum, 1);
-        mbar_init(&s_taken, 16);                        // the eight warps of both CTAs
+        for (int i = 0; i < kSumBars; ++i) mbar_init(&s_sum[i], 1);
+        for (int i = 0; i < kSums; ++i) mbar_init(&s_taken[i], 16);   // the eight warps of both CTAs
         mbar_init(&s_last, 1);
         fence_mbar_init();
     }
@@ -636,9 +656,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
-    let_next_start();
-    wait_for_previous();
-
     int block;
     const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x / 2, block)];
     const int pairs = (m.mb + 1) / 2;                   // 256-row tiles
@@ -666,6 +683,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     constexpr uint32_t kLeftBlock = MODE == kGram ? P::kX : P::kAB, kRightBlock = MODE == kSquare ? P::kAB : P::kX;
     const int blocks = MODE == kGram ? m.nk : m.mk;
     bool ok = true;
+    let_next_start();
+    wait_for_previous();
 
     if (warp == 8) {
         if (lane == 0) {
@@ -674,12 +693,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             int k = 0;
             for (; k < blocks; ++k) {
                 const int st = k % S::kCount;
-                if (k >= S::kCount) ok = mbar_wait_bounded(&s_empty[st], (k / S::kCount - 1) & 1, polls);
+                if (k >= S::kCount) {
+                    if (kOneCommit) {   // block k - kCount is done with when the block after it has been committed
+                        const int j = k - S::kCount + 1;
+                        ok = wait_for(&s_sum[j % kSumBars], (j / kSumBars) & 1, polls);
+                    } else if (st % S::kGroup == 0) {
+                        ok = wait_for(&s_empty[st / S::kGroup], (k / S::kCount - 1) & 1, polls);
+                    }
+                }
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
                 if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
-                mbar_arrive_expect_tx(&s_full[st], same ? S::kLeft : S::kStage);
+                const bool shared = same && !(MODE == kSquare && k >> 2 == tj);
+                mbar_arrive_expect_tx(&s_full[st], shared ? S::kLeft : S::kStage);
                 bulk_copy_g2s(a, left + ((int64_t)lrow * blocks + k) * kLeftBlock, S::kLeft, &s_full[st]);
                 if (MODE == kApply) {
                     for (int p = 0; p < R; ++p)
@@ -689,57 +716,78 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                                               p * kPlane + (k & 1) * (kPlane / 2),
                                           kPlane / 2, &s_full[st]);
                 } else if (N == 256) {
-                    if (!same)
-                        bulk_copy_g2s(b, right + ((int64_t)min(2 * tj + rank, m.mb - 1) * blocks + k) * kRightBlock, S::kRight, &s_full[st]);
+                    const int j = min(2 * tj + rank, m.mb - 1);
+                    const bool v = MODE == kSquare && k >> 1 == j;
+                    if (!shared)
+                        bulk_copy_g2s(b, v ? m.v + (int64_t)k * kRightBlock : right + ((int64_t)j * blocks + k) * kRightBlock, S::kRight,
+                                      &s_full[st]);
                 } else {
+                    const int j = min(tj, m.mb - 1);
+                    const bool v = MODE == kSquare && k >> 1 == j;
+                    const char* from = v ? m.v + (int64_t)k * kRightBlock : right + ((int64_t)j * blocks + k) * kRightBlock;
                     for (int p = 0; p < R; ++p)
-                        bulk_copy_g2s(b + p * (kPlane / 2),
-                                      right + ((int64_t)min(tj, m.mb - 1) * blocks + k) * kRightBlock + p * kPlane + rank * (kPlane / 2),
-                                      kPlane / 2, &s_full[st]);
+                        bulk_copy_g2s(b + p * (kPlane / 2), from + p * kPlane + rank * (kPlane / 2), kPlane / 2, &s_full[st]);
                 }
             }
             if (!ok)
                 for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
-                    mbar_wait_bounded(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+                    wait_for(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
         }
     } else if (warp == 9) {
         if (lane == 0 && rank == 1) {
             for (int k = 0; k < blocks && ok; ++k) {
-                ok = mbar_wait_bounded(&s_full[k % S::kCount], (k / S::kCount) & 1, polls);
+                ok = wait_for(&s_full[k % S::kCount], (k / S::kCount) & 1, polls);
                 if (ok) mbar_arrive_at(&s_full[k % S::kCount], 0);
             }
         } else if (lane == 0) {
             const uint32_t idesc = instruction(MODE == kApply, 256, N);
-            constexpr uint32_t kPlaneB = (uint32_t)N / 2 * 128;
+            constexpr uint32_t kStep = (MODE == kApply ? 2048 : 32) / 16, kNext = MODE == kApply ? kPlane / 2 : 16;
+            constexpr uint32_t kLowB = (uint32_t)N / 2 * 128 / 16;   // from hi to lo of the right factor
+            const uint32_t a0 = operand_low(smem_u32(smem), 16), b0 = operand_low(smem_u32(smem) + S::kLeft, kNext);
+            auto left_of = [&](int st) { return a0 + st * (S::kStage / 16); };
+            auto right_of = [&](int k, int st) {
+                const bool shared = same && !(MODE == kSquare && k >> 2 == tj);
+                return shared ? left_of(st) : b0 + st * (S::kStage / 16);
+            };
+            auto rest = [&](int k, int st) {   // hi lo + lo hi
+                const uint32_t a = left_of(st), b = right_of(k, st);
+#pragma unroll
+                for (int q = 0; q < kCols / 16; ++q) {
+                    tc_mma<2>(tmem + kSums * N, operand(a + q * 2), operand(b + kLowB + q * kStep), idesc, k != 0 || q != 0);
+                    tc_mma<2>(tmem + kSums * N, operand(a + kPlane / 16 + q * 2), operand(b + q * kStep), idesc, true);
+                }
+            };
+            int st = 0, phase = 0, before = 0;
             for (int k = 0; k < blocks; ++k) {
-                const int st = k % S::kCount;
-                ok = mbar_wait_bounded(&s_full[st], (k / S::kCount) & 1, polls);
-                if (F32 && ok && k > 0) ok = mbar_wait_bounded(&s_taken, (k - 1) & 1, polls);
+                const int buf = k % kSums;
+                ok = wait_for(&s_full[st], phase, polls);
+                if (F32 && ok && k >= kSums) ok = wait_for(&s_taken[buf], (k / kSums - 1) & 1, polls);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t a = smem_u32(smem + st * S::kStage), b = same ? a : a + S::kLeft;
-                auto at_a = [&](int p, int q) { return operand(a + p * kPlane + q * 32, 16, 1024); };
-                auto at_b = [&](int p, int q) {
-                    return MODE == kApply ? operand(b + p * kPlaneB + q * 2048, kPlane / 2, 1024)
-                                          : operand(b + p * kPlaneB + q * 32, 16, 1024);
-                };
+                const uint32_t a = left_of(st), b = right_of(k, st);
+                const uint32_t d = F32 ? tmem + buf * N : tmem;
 #pragma unroll
-                for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(tmem, at_a(0, q), at_b(0, q), idesc, (!F32 && k != 0) || q != 0);
-                if (F32) {
-                    tc_commit<2>(&s_sum);
+                for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(d, operand(a + q * 2), operand(b + q * kStep), idesc, (!F32 && k != 0) || q != 0);
+                if (kOneCommit) {
+                    if (k > 0) rest(k - 1, before);
+                    tc_commit<2>(&s_sum[k % kSumBars]);
+                    before = st;
+                } else if (F32) {
+                    tc_commit<2>(&s_sum[0]);
+                    rest(k, st);
+                    tc_commit<2>(&s_empty[st]);
+                } else {
+                    if (R == 2) {
 #pragma unroll
-                    for (int q = 0; q < kCols / 16; ++q) {
-                        tc_mma<2>(tmem + N, at_a(0, q), at_b(1, q), idesc, k != 0 || q != 0);
-                        tc_mma<2>(tmem + N, at_a(L - 1, q), at_b(0, q), idesc, true);
+                        for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(d, operand(a + q * 2), operand(b + kLowB + q * kStep), idesc, true);
                     }
-                } else if (R == 2) {
-#pragma unroll
-                    for (int q = 0; q < kCols / 16; ++q) tc_mma<2>(tmem, at_a(0, q), at_b(R - 1, q), idesc, true);
+                    if (st % S::kGroup == S::kGroup - 1) tc_commit<2>(&s_empty[st / S::kGroup]);
                 }
-                tc_commit<2>(&s_empty[st]);
+                if (++st == S::kCount) st = 0, phase ^= 1;
             }
+            if (kOneCommit && ok) rest(blocks - 1, before);
             tc_commit<2>(&s_last);
-            if (!ok) mbar_wait_bounded(&s_last, 0, 0);
+            if (!ok) wait_for(&s_last, 0, 0);
         }
     } else {
         constexpr int kPart = N / 2;                     // columns of a thread; the warps' upper half takes the right ones
@@ -759,25 +807,27 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         };
         if (F32)
             for (int k = 0; k < blocks; ++k) {
-                ok = __all_sync(~0u, mbar_wait_bounded(&s_sum, k & 1, polls));
+                ok = __all_sync(~0u, wait_for(&s_sum[k % kSumBars], (k / kSumBars) & 1, polls));
                 if (!ok) break;
                 tc_fence_after();
-                take(0);
+                take(k % kSums * N);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_at(&s_taken, 0);
+                if (lane == 0) mbar_arrive_at(&s_taken[k % kSums], 0);
             }
-        if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&s_last, 0, polls));
+        if (ok) ok = __all_sync(~0u, wait_for(&s_last, 0, polls));
         tc_fence_after();
-        if (ok) take(F32 ? N : 0);
+        if (ok) take(F32 ? kSums * N : 0);
         if (!ok) *t.fail = 1;
         // Every product has read its operands by now: their shared memory takes the finished blocks, from where they
         // leave as whole blocks.
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
-        char* const out = MODE == kGram ? m.a : MODE == kSquare ? m.b : m.x[t.from ^ 1];
+        char* const out = MODE == kGram && !t.cubic ? m.a : MODE != kApply ? m.b : m.x[t.from ^ 1];
         constexpr uint32_t kOutBlock = MODE == kApply ? P::kX : P::kAB, kOutBytes = P::kOut * kPlane;
         const int col = kWide * tj + half * (kPart / kCols);   // first block column of this thread
         const bool mirrored = MODE != kApply && (N == 256 ? tj > ti : tj > 2 * ti + 1);
+        // V's blocks take the place of mirrored ones, which tiles on the diagonal do not have
+        const bool keeps_v = MODE == kGram && !t.cubic && (N == 256 ? col == 2 * row : tj == row);
         // space: kPart / 64 blocks and as many mirrored ones for each half; what does not fit side by side takes turns
         constexpr uint32_t kMine = kPart / kCols * kOutBytes, kSpace = MODE == kApply ? kMine : 2 * kMine;
         constexpr bool kTurns = 2 * kSpace > 196608u;
@@ -787,24 +837,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             for (int c = 0; c < kPart; c += 8) {
                 if (col + c / kCols >= wide || row >= m.mb) continue;
                 const uint32_t o = block_offset(r, c % kCols);
-                float old[8];
-                if (MODE == kSquare) load_old<F32>(m.a + ((int64_t)row * wide + col + c / kCols) * kOutBlock + o, old);
-                __half hi[8], lo[8];
-                const int d = (int)r + row * kRows - (col * kCols + c);   // the diagonal's place in this piece
-                finish<MODE>(t, v + c, old, row * kRows + (int)r < m.m ? d : -1, hi, lo);
-                *reinterpret_cast<uint4*>(space + (c / kCols) * kOutBytes + o) = pack8(hi);
-                if (P::kOut == 2) *reinterpret_cast<uint4*>(space + (c / kCols) * kOutBytes + o + kPlane) = pack8(lo);
+                uint32_t hi[4], lo[4];
+                const int in = row * kRows + (int)r, on = in < m.m ? in - (col * kCols + c) : -1;   // diagonal
+                finish(t, v + c, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+                put<P::kOut == 2>(space + (c / kCols) * kOutBytes + o, hi, lo);
+                if (MODE == kGram && keeps_v) {
+                    finish(t, v + c, on, hi, lo);
+                    put<P::kOut == 2>((N == 256 ? space + kMine : smem + (2 + half) * kMine) + (c / kCols) * kOutBytes + o, hi, lo);
+                }
                 if (MODE != kApply && mirrored) {
                     // N 256: rows of one block, columns of the two blocks that the rows r belong to.  N 128: a half's 64
                     // columns are 64 rows of a block, the two halves' rows follow one another.
                     char* const to = N == 256 ? space + kMine + (r / kCols) * kOutBytes
                                               : smem + 2 * kMine + (r / kCols) * kOutBytes;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t w = block_offset((N == 256 ? 0 : half * kCols) + c + i, r % kCols);
-                        *reinterpret_cast<__half*>(to + w) = hi[i];
-                        if (P::kOut == 2) *reinterpret_cast<__half*>(to + w + kPlane) = lo[i];
-                    }
+                    write_mirrored<P::kOut == 2>(to, (N == 256 ? 0 : half * kCols) + c, r % kCols, hi, lo);
                 }
             }
             fence_proxy_async_smem();
@@ -823,8 +869,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                     bulk_copy_s2g(out + ((int64_t)tj * wide + 2 * row + half) * kOutBlock, smem + 2 * kMine + half * kOutBytes, kOutBytes);
                 }
             }
+            if (MODE == kGram && keeps_v)
+                for (int c = 0; c < kPart / kCols; ++c)
+                    if (col + c < wide)
+                        bulk_copy_s2g(m.v + (int64_t)(col + c) * kOutBlock,
+                                      (N == 256 ? space + kMine : smem + (2 + half) * kMine) + c * kOutBytes, kOutBytes);
             bulk_commit_group();
-            bulk_wait_group0();
+            bulk_wait_group_read0();   // (what leaves is in memory when the grid has ended)
         };
         auto all_warps = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         const bool sender = ok && (threadIdx.x & 127) == 0 && row < m.mb;
@@ -850,7 +901,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     cluster_sync();   // neither CTA leaves, or frees TMEM, while the other may still use it
     tc_fence_after();
     if (warp == 9) tmem_free<2>(tmem, kTmem);
-    cluster_sync();
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -858,7 +908,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Parts {
     int m, n, mb, mk, nk;
-    size_t x, a, norms, total;   // bytes
+    size_t x, a, v, norms, total;   // bytes
 };
 Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     Parts p;
@@ -870,54 +920,70 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
     p.norms = up256((size_t)div_up64(d.rows * d.cols, kNormChunk) * 8);
-    p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.norms;
+    p.v = (size_t)p.mb * 2 * planes * kPlane;
+    p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
 }
-int planes_of(const D3gsOrthoConfig& cfg) { return cfg.dtype == D3GS_DTYPE_F32 ? 2 : 1; }
+// How the products of a list of matrices are cut: pairs of CTAs when the largest short side is above kPairFrom.
+constexpr int kPairFrom = 384;
+bool large(const D3gsOrthoMatrix* mats, int32_t count) {
+    for (int32_t i = 0; i < count; ++i)
+        if ((mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols) > kPairFrom && mats[i].rows > 0 && mats[i].cols > 0) return true;
+    return false;
+}
+// Planes of A and B.  Small matrices take two for 16-bit types too: with them it is not the products that take time, and
+// one plane would cost an 8 x 8 matrix up to twice the error of its own rounding.
+int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
+    return cfg.dtype == D3GS_DTYPE_F32 || !large(mats, count) ? 2 : 1;
+}
 size_t workspace_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
     size_t need = 512;   // alignment, the failure word
-    for (int32_t i = 0; i < count; ++i) need += parts_of(mats[i], planes_of(cfg)).total;
+    const int planes = planes_of(mats, count, cfg);
+    for (int32_t i = 0; i < count; ++i) need += parts_of(mats[i], planes).total;
     return need;
 }
 
-// Scales of the operands.  The singular values of X lie in [0, s]: s = 1 at the start, and after a step the largest
-// |a x + b x^3 + c x^5| over [0, s], found at s or where the derivative a + 3 b x^2 + 5 c x^4 vanishes.  No entry of X
-// exceeds s, none of A s^2, none of B the largest |a + b y + c y^2| over y in [0, s^2].  Each is scaled to at most 2^15
-// by a power of two, so that scaling loses nothing.
+// Scales of the operands.  The singular values of X lie in [0, x]: x = 1 at the start, and after a step the largest
+// |a s + b s^3 + c s^5| over [0, x], found at x or where the derivative a + 3 b s^2 + 5 c s^4 vanishes.  No entry of X
+// exceeds x, none of A and V = A + b/c I the largest of x^2, |b/c| and |x^2 + b/c|, none of B the largest
+// |a + b y + c y^2| over y in [0, x^2].  Each is scaled to at most 2^15 by a power of two, so that scaling loses nothing.
 struct Scales {
-    float x[D3GS_NS_MAX_STEPS + 1], a[D3GS_NS_MAX_STEPS], b[D3GS_NS_MAX_STEPS];
+    float x[D3GS_NS_MAX_STEPS + 1], v[D3GS_NS_MAX_STEPS], b[D3GS_NS_MAX_STEPS];
 };
 float scale_for(double most) {
     int e;
-    std::frexp(most * 1.001, &e);   // most * 1.001 <= 2^e
+    std::frexp(std::fmax(most, 1.0 / kMaxSpectrum) * 1.001, &e);   // at most 2^e; zeros are held by any scale
     return std::ldexp(1.0f, 15 - e);
 }
+// Fails when singular values would pass kMaxSpectrum, or where b / c would: A shares V's scale.
 bool scales_of(const D3gsOrthoConfig& cfg, Scales& out) {
-    double s = 1.0;
-    out.x[0] = scale_for(s);
+    double x = 1.0;
+    out.x[0] = scale_for(x);
     for (int k = 0; k < cfg.steps; ++k) {
-        const double a = cfg.coefficients[k][0], b = cfg.coefficients[k][1], c = cfg.coefficients[k][2], top = s * s;
+        const double a = cfg.coefficients[k][0], b = cfg.coefficients[k][1], c = cfg.coefficients[k][2], top = x * x;
+        if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c) || (c != 0.0 && std::fabs(b) > kMaxSpectrum * std::fabs(c))) return false;
         auto f = [&](double y) { return std::fabs(std::sqrt(y) * (a + y * (b + y * c))); };
         double next = f(top), poly = std::fmax(std::fabs(a), std::fabs(a + top * (b + top * c)));
         auto inside = [&](double y) {
             if (y > 0.0 && y < top) next = std::fmax(next, f(y));
         };
+        double shift = 0.0;
         if (c != 0.0) {
             const double d = 9.0 * b * b - 20.0 * a * c;
             if (d >= 0.0) {
                 inside((-3.0 * b + std::sqrt(d)) / (10.0 * c));
                 inside((-3.0 * b - std::sqrt(d)) / (10.0 * c));
             }
-            const double v = -b / (2.0 * c);
-            if (v > 0.0 && v < top) poly = std::fmax(poly, std::fabs(a + v * (b + v * c)));
+            shift = b / c;
+            if (-0.5 * shift > 0.0 && -0.5 * shift < top) poly = std::fmax(poly, std::fabs(a - b * b / (4.0 * c)));
         } else if (b != 0.0) {
             inside(-a / (3.0 * b));
         }
-        out.a[k] = scale_for(top);
-        out.b[k] = scale_for(std::fmax(poly, 1.0 / kMaxSpectrum));
-        s = std::fmax(next, 1.0 / kMaxSpectrum);   // coefficients of zeros: any scale holds a zero
-        if (!(s <= kMaxSpectrum) || !(poly <= kMaxSpectrum * kMaxSpectrum)) return false;
-        out.x[k + 1] = scale_for(s);
+        out.v[k] = scale_for(std::fmax(top, std::fmax(std::fabs(shift), std::fabs(top + shift))));
+        out.b[k] = scale_for(poly);
+        x = std::fmax(next, 1.0 / kMaxSpectrum);
+        if (!(x <= kMaxSpectrum) || !(poly <= kMaxSpectrum * kMaxSpectrum)) return false;
+        out.x[k + 1] = scale_for(x);
     }
     return true;
 }
@@ -929,7 +995,7 @@ int32_t check(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     D3GS_REQUIRE(cfg->steps >= 1 && cfg->steps <= D3GS_NS_MAX_STEPS, "%s: %d steps (1 to %d)", what, cfg->steps,
                  D3GS_NS_MAX_STEPS);
     D3GS_REQUIRE(cfg->eps > 0.0f, "%s: eps must be positive", what);
-    D3GS_REQUIRE(scales_of(*cfg, scales), "%s: with these coefficients singular values grow past %g", what, kMaxSpectrum);
+    D3GS_REQUIRE(scales_of(*cfg, scales), "%s: with these coefficients singular values grow past %g, or b / c does", what, kMaxSpectrum);
     for (int32_t i = 0; i < count; ++i) {
         const D3gsOrthoMatrix& m = mats[i];
         const int64_t small = m.rows < m.cols ? m.rows : m.cols, large = m.rows < m.cols ? m.cols : m.rows;
@@ -965,32 +1031,19 @@ int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size
     return D3GS_OK;
 }
 
-// How the products of a list of matrices are cut.  Pairs of CTAs when the largest short side is above kPairFrom.
-constexpr int kPairFrom = 384;
-struct Shape {
-    bool pair;
-};
-Shape shape_of(const Table& t) {
-    Shape s{};
-    for (int k = 0; k < t.count; ++k) s.pair |= t.mat[k].m > kPairFrom;
-    return s;
+template <int MODE, typename B> int32_t small_product(const Table& t, B& blocks, cudaStream_t st) {
+    const unsigned tiles = blocks([](const Matrix& m) {
+        return MODE == kApply ? (int64_t)m.mb * ((m.nk + 1) / 2) : (int64_t)m.mb * (m.mb + 1) / 2;
+    });
+    // as many CTAs a tile as the machine has room for, none without four blocks to sum
+    int longest = 0;
+    for (int k = 0; k < t.count; ++k) longest = max(longest, MODE == kGram ? t.mat[k].nk : t.mat[k].mk);
+    unsigned parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
+    return launch(ns_small_kernel<MODE>, "ns_small_kernel", tiles * parts, kSmallThreads, SmallStages::kBytes, parts, st, t);
 }
-
-template <bool F32, int MODE, int RIGHT, typename B>
-int32_t product_of(const Table& t, const Shape& shape, B& blocks, cudaStream_t st) {
+template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const Table& t, B& blocks, cudaStream_t st) {
     constexpr int L = Planes<F32, MODE, RIGHT>::kLeft;
-    if (!shape.pair) {
-        const unsigned tiles = blocks([](const Matrix& m) {
-            return MODE == kApply ? (int64_t)m.mb * ((m.nk + 1) / 2) : (int64_t)m.mb * (m.mb + 1) / 2;
-        });
-        // as many CTAs a tile as the machine has room for, none without four blocks to sum
-        int longest = 0;
-        for (int k = 0; k < t.count; ++k) longest = max(longest, MODE == kGram ? t.mat[k].nk : t.mat[k].mk);
-        unsigned parts = 1;
-        while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
-        return launch(ns_small_kernel<F32, MODE, RIGHT>, "ns_small_kernel", tiles * parts, kSmallThreads,
-                      SmallStages<L, RIGHT>::kBytes, parts, st, t);
-    }
     // 256 x 256 tiles move the least; 256 x 128 ones when those would leave SMs idle
     const unsigned tiles = blocks([](const Matrix& m) {
         const int64_t pairs = (m.mb + 1) / 2;
@@ -1006,16 +1059,16 @@ int32_t product_of(const Table& t, const Shape& shape, B& blocks, cudaStream_t s
     return launch(ns_pair_kernel<F32, MODE, RIGHT, 128>, "ns_pair_kernel", narrow * 2, kPairThreads,
                   PairStages<L, RIGHT, 128>::kBytes, 2, st, t);
 }
-template <bool F32, int MODE, typename B>
-int32_t product(Table& t, const Shape& shape, B& blocks, cudaStream_t st) {
-    // (blocks writes the table's first_block)
-    if constexpr (F32) return product_of<true, MODE, 2>(t, shape, blocks, st);
+// one product of every matrix of the table; `blocks` writes its first_block
+template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table& t, bool last, B& blocks, cudaStream_t st) {
+    if constexpr (!PAIR) return small_product<MODE>(t, blocks, st);
+    else if constexpr (F32) return pair_product<true, MODE, 2>(t, blocks, st);
     else if constexpr (MODE == kApply)
-        return t.last ? product_of<false, MODE, 1>(t, shape, blocks, st) : product_of<false, MODE, 2>(t, shape, blocks, st);
-    else return product_of<false, MODE, 1>(t, shape, blocks, st);
+        return last ? pair_product<false, MODE, 1>(t, blocks, st) : pair_product<false, MODE, 2>(t, blocks, st);
+    else return pair_product<false, MODE, 1>(t, blocks, st);
 }
 
-template <bool F32>
+template <bool F32, bool PAIR>
 int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg, bool muon, const Scales& sc, void* ws,
             cudaStream_t st) {
     char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
@@ -1052,7 +1105,8 @@ int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& c
             m.x[1] = at + p.x;
             m.a = at + 2 * p.x;
             m.b = at + 2 * p.x + p.a;
-            m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a);
+            m.v = at + 2 * p.x + 2 * p.a;
+            m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a + p.v);
             at += p.total;
         }
         if (t.count == 0) break;
@@ -1072,17 +1126,21 @@ int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& c
         t.out_scale = sc.x[0];
         grid = blocks(every_block);
         if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, t)) return rc;
-        const Shape shape = shape_of(t);
         for (int s = 0; s < cfg.steps; ++s) {
-            t.last = s == cfg.steps - 1;
-            t.out_scale = sc.a[s] / (sc.x[s] * sc.x[s]);
-            if (int32_t rc = product<F32, kGram>(t, shape, blocks, st)) return rc;
-            t.ca = cfg.coefficients[s][0] * sc.b[s];
-            t.cb = cfg.coefficients[s][1] * (sc.b[s] / sc.a[s]);
-            t.cc = cfg.coefficients[s][2] * (sc.b[s] / sc.a[s] / sc.a[s]);
-            if (int32_t rc = product<F32, kSquare>(t, shape, blocks, st)) return rc;
+            const bool last = s == cfg.steps - 1;
+            const double a = cfg.coefficients[s][0], b = cfg.coefficients[s][1], c = cfg.coefficients[s][2];
+            const double sx = sc.x[s], sv = sc.v[s], sb = sc.b[s];
+            t.cubic = c == 0.0;
+            t.out_scale = (float)(t.cubic ? b * (sb / (sx * sx)) : sv / (sx * sx));
+            t.shift = (float)(t.cubic ? a * sb : b / c * sv);
+            if (int32_t rc = product<F32, PAIR, kGram>(t, last, blocks, st)) return rc;
+            if (!t.cubic) {
+                t.out_scale = (float)(c * (sb / (sv * sv)));
+                t.shift = (float)(a * sb);
+                if (int32_t rc = product<F32, PAIR, kSquare>(t, last, blocks, st)) return rc;
+            }
             t.out_scale = sc.x[s + 1] / sc.b[s] / sc.x[s];
-            if (int32_t rc = product<F32, kApply>(t, shape, blocks, st)) return rc;
+            if (int32_t rc = product<F32, PAIR, kApply>(t, last, blocks, st)) return rc;
             t.from ^= 1;
         }
         t.out_scale = 1.0f / sc.x[cfg.steps];
@@ -1102,8 +1160,9 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     D3GS_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= workspace_of(mats, count, *cfg),
                  "%s: workspace missing, unaligned or smaller than d3gs_orthogonalize_workspace_bytes", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return cfg->dtype == D3GS_DTYPE_F32 ? run<true>(mats, count, *cfg, muon, sc, ws, st)
-                                        : run<false>(mats, count, *cfg, muon, sc, ws, st);
+    if (!large(mats, count)) return run<true, false>(mats, count, *cfg, muon, sc, ws, st);
+    return cfg->dtype == D3GS_DTYPE_F32 ? run<true, true>(mats, count, *cfg, muon, sc, ws, st)
+                                        : run<false, true>(mats, count, *cfg, muon, sc, ws, st);
 }
 
 }  // namespace

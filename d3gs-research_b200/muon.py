@@ -55,7 +55,8 @@ def orthogonalize(update: torch.Tensor, ns_coefficients: Sequence = NS_COEFFICIE
 
     ``X = U / max(|U|_F, eps)``, then ``ns_steps`` times ``X = a X + (b A + c A A) X`` with ``A = X X^T``.
     ``ns_coefficients`` is ``(a, b, c)``, or one such triple per step.  float32 or bfloat16 in, a dense tensor of the
-    same type out; every product is summed in 32 bits.  Rows that are not dense are copied first.  No gradient."""
+    same type out; every product is summed in 32 bits.  Rows that are not dense are copied first.  No gradient.
+    Coefficients with which singular values in [0, 1] grow past 1024, or with ``0 < 1024 |c| < |b|``, are refused."""
     if not isinstance(update, torch.Tensor) or not update.is_cuda:
         raise ValueError("orthogonalize: update must be a CUDA tensor")
     if update.dim() < 2 or update.dtype not in (torch.float32, torch.bfloat16):

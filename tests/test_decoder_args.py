@@ -99,6 +99,10 @@ def test_ortho_coefficients_that_grow_without_bound():
     assert lib.d3gs_orthogonalize(mats, 1, C.byref(cfg), 256, 1 << 40, None) == -1
     assert "singular values grow" in _lib.last_error()
     for k in range(5):
+        cfg.coefficients[k][:] = (1.5, -0.5, 1e-4)
+    assert lib.d3gs_orthogonalize(mats, 1, C.byref(cfg), 256, 1 << 40, None) == -1
+    assert "b / c" in _lib.last_error()
+    for k in range(5):
         cfg.coefficients[k][:] = (0.0, 0.0, 0.0)
     assert lib.d3gs_orthogonalize_workspace_bytes(mats, 1, C.byref(cfg)) > 0
 

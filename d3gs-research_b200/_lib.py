@@ -226,3 +226,10 @@ def check(rc: int, what: str):
 def ptr(t):
     """Device pointer of a torch tensor (None -> NULL)."""
     return None if t is None else t.data_ptr()
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of CUDA device ``index`` as an integer (``torch.cuda.current_stream`` without the object
+    around it, which takes longer to make than a small launch)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)

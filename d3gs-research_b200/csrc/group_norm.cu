@@ -22,10 +22,11 @@ namespace d3gs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;                // rows in flight per thread and input
+constexpr int kUnroll = 4, kUnroll2 = 2;   // rows in flight per thread: kernels that read x, that read x and dy
+constexpr int kCtas = 4, kCtas2 = 3;       // and their CTAs per SM, which the registers are bounded for
 constexpr int kMaxChannels = 16384;       // per-channel sums of one CTA stay in shared memory
 constexpr int64_t kTurnBytes = 48 << 20;  // inputs of one turn, to be found in L2 (126 MB) by the second pass
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kMaxChunks = 1024;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2 };
 
@@ -50,8 +51,12 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int i, float v) 
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T v[V]; };
 
-// The logistic function: ex2 and reciprocal of the special-function unit, about 2e-7 relative; u -> -inf gives 0.
-__device__ __forceinline__ float logistic(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+// The logistic function by ex2 and reciprocal of the special-function unit, about 2e-7 relative; u -> -inf gives 0.
+__device__ __forceinline__ float logistic(float u) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-u)));
+    return r;
+}
 
 template <int ACT> __device__ __forceinline__ float act_value(float u) {
     if (ACT == kActSilu) return u * logistic(u);
@@ -66,6 +71,11 @@ template <int ACT> __device__ __forceinline__ float act_slope(float u) {
     if (ACT == kActGelu) return fmaf(u * 0.39894228f, __expf(-0.5f * u * u), 0.5f * (1.0f + erff(u * 0.70710678f)));
     return 1.0f;
 }
+
+// Launches follow one another closely: a kernel may start while its predecessor's last CTAs run, and waits here before
+// it touches memory.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 struct Args {
     const void *x, *dy, *weight, *bias;
@@ -121,8 +131,10 @@ template <int V> __device__ __forceinline__ int64_t whole_rows(const Args& a, in
 // that k came from are themselves far from it and the variance is at least kUnroll/n of that distance squared, so
 // the cancellation in q - s^2/n costs at most n/kUnroll units of the last place, whatever the mean.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) gn_stats_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a) {
     extern __shared__ float sh[];
+    let_next_start();
+    wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = blockIdx.x;
     const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
@@ -139,46 +151,41 @@ __global__ void __launch_bounds__(kThreads) gn_stats_kernel(const Args a) {
         float k[V], s[V], q[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = q[j] = k[j] = 0.0f;
-        int n = 0;
-        for (int64_t r = r0 + w.lane_row; r < end; r += kUnroll * w.rp) {
-            Vec<T, V> v[kUnroll];
-            int got = 0;
+        int64_t r = r0 + w.lane_row;
+        const int64_t step = w.rp * a.x_row;
+        p += r * a.x_row;
+        const int got = r < end ? (int)min((int64_t)kUnroll, (end - r + w.rp - 1) / w.rp) : 0;
+        for (int u = 0; u < got; ++u) {
+            const Vec<T, V> f = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-                    v[u] = *reinterpret_cast<const Vec<T, V>*>(p + (r + u * w.rp) * a.x_row);
-                    ++got;
-                }
-            if (n == 0) {
-                const float inv = 1.0f / got;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float t = 0.0f;
-#pragma unroll
-                    for (int u = 0; u < kUnroll; ++u)
-                        if (u < got) t += to_f(v[u].v[j]);
-                    k[j] = t * inv;
-                }
-            }
-            n += got;
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (u < got) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float d = to_f(v[u].v[j]) - k[j];
-                        s[j] += d;
-                        q[j] = fmaf(d, d, q[j]);
-                    }
-                }
+            for (int j = 0; j < V; ++j) k[j] += to_f(f.v[j]);
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) k[j] /= (float)max(got, 1);
+        auto add = [&](const Vec<T, V>& x) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = to_f(x.v[j]) - k[j];
+                s[j] += d;
+                q[j] = fmaf(d, d, q[j]);
+            }
+        };
+        int n = 0;
+        for (; r + (kUnroll - 1) * w.rp < end; r += kUnroll * w.rp, p += kUnroll * step, n += kUnroll) {
+            Vec<T, V> v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) add(v[u]);
+        }
+        for (; r < end; r += w.rp, p += step, ++n) add(*reinterpret_cast<const Vec<T, V>*>(p));
         // the short row at the image's end belongs to the thread whose turn it is
         const bool mine = tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             int nj = n;
             if (mine && j < tail) {
-                const float v = to_f(p[end * a.x_row + j]);
+                const float v = to_f(p[j]);   // r == end
                 if (n == 0) k[j] = v;
                 const float d = v - k[j];
                 s[j] += d;
@@ -235,52 +242,65 @@ __device__ __forceinline__ float chunk_count(const Args& a, int chunk) {
     return (float)((e1 - e0) / a.C * a.cpg);
 }
 
-// ---- forward, join: one warp per (image, group) over the chunks ---------------------------------------------------
-__global__ void __launch_bounds__(kJoinThreads) gn_stats_join_kernel(const Args a, int images) {
-    const int i = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (i >= images * a.G) return;
-    const int64_t bg = (int64_t)a.first * a.G + i;
-    const float2* part = reinterpret_cast<const float2*>(a.part) + bg * a.chunks;
-    const float total = (float)(a.elems / a.C * a.cpg);
-    float t = 0.0f;
-    const float near = part[0].x;
-    for (int k = lane; k < a.chunks; k += 32) t = fmaf(chunk_count(a, k) / total, part[k].x - near, t);
+// ---- forward, join: one CTA per (image, group) over the chunks ----------------------------------------------------
+__device__ __forceinline__ float cta_sum(float v, float* sh) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-    t += near;
-    float m2 = 0.0f;
-    for (int k = lane; k < a.chunks; k += 32) {
-        const float2 p = part[k];
-        const float d = p.x - t;
-        m2 += fmaf(chunk_count(a, k) * d, d, p.y);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinThreads / 32; ++k) v += sh[k];
+    return v;
+}
+__global__ void __launch_bounds__(kJoinThreads) gn_stats_join_kernel(const Args a) {
+    __shared__ float sh[2][kJoinThreads / 32];
+    let_next_start();
+    wait_for_previous();
+    const int64_t bg = (int64_t)a.first * a.G + blockIdx.x;
+    const float2* part = reinterpret_cast<const float2*>(a.part) + bg * a.chunks;
+    const float total = (float)(a.elems / a.C * a.cpg), near = part[0].x;
+    float2 mine[kMaxChunks / kJoinThreads];
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / kJoinThreads; ++i) {
+        const int k = threadIdx.x + i * kJoinThreads;
+        mine[i] = k < a.chunks ? part[k] : make_float2(near, 0.0f);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o);
-    if (lane == 0) {
-        a.stats[bg * 2] = t;
+    for (int i = 0; i < kMaxChunks / kJoinThreads; ++i) {
+        const int k = threadIdx.x + i * kJoinThreads;
+        if (k < a.chunks) t = fmaf(chunk_count(a, k) / total, mine[i].x - near, t);
+    }
+    const float mean = near + cta_sum(t, sh[0]);
+    float m2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / kJoinThreads; ++i) {
+        const int k = threadIdx.x + i * kJoinThreads;
+        if (k < a.chunks) {
+            const float d = mine[i].x - mean;
+            m2 += fmaf(chunk_count(a, k) * d, d, mine[i].y);
+        }
+    }
+    m2 = cta_sum(m2, sh[1]);
+    if (threadIdx.x == 0) {
+        a.stats[bg * 2] = mean;
         a.stats[bg * 2 + 1] = 1.0f / sqrtf(m2 / total + a.eps);
     }
 }
 
-// mean, rstd, weight, bias of the V values of a vector
-template <int V> struct Coef { float mean[V], rstd[V], w[V], b[V]; };
-template <int V> __device__ __forceinline__ Coef<V> load_coef(const Args& a, int b, int vec) {
-    Coef<V> c;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int ch = (vec * V + j) % a.C;
-        const float* st = a.stats + ((int64_t)b * a.G + ch / a.cpg) * 2;
-        c.mean[j] = st[0];
-        c.rstd[j] = st[1];
-        c.w[j] = a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f;
-        c.b[j] = a.bias ? load_param(a.bias, a.wdtype, ch) : 0.0f;
-    }
-    return c;
+// mean, rstd, weight and bias of channel `ch` of image b
+__device__ __forceinline__ float4 load_coef(const Args& a, int b, int ch) {
+    const float2 st = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + ch / a.cpg];
+    return make_float4(st.x, st.y, a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f,
+                       a.bias ? load_param(a.bias, a.wdtype, ch) : 0.0f);
 }
 
 // ---- forward, pass 2 -----------------------------------------------------------------------------------------------
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a) {
+    let_next_start();
+    wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = a.chunks - 1 - blockIdx.x;   // last read first: still in L2
     const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
@@ -292,40 +312,45 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(const Args a) {
         const int vec = walk_vec(a, tile);
         int tail;
         const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        const Coef<V> c = load_coef<V>(a, b, vec);
-        const T* p = x + (int64_t)vec * V;
-        T* o = y + (int64_t)vec * V;
-        for (int64_t r = r0 + w.lane_row; r < end; r += kUnroll * w.rp) {
+        float k[V], q[V];   // u = k x + q; q is rounded at the size of mean rstd, as mean itself is
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float4 c = load_coef(a, b, (vec * V + j) % a.C);
+            k[j] = c.y * c.z;
+            q[j] = fmaf(-c.x, k[j], c.w);
+        }
+        auto value = [&](T v, int j) { return from_f<T>(act_value<ACT>(fmaf(to_f(v), k[j], q[j]))); };
+        int64_t r = r0 + w.lane_row;
+        const T* p = x + r * a.x_row + (int64_t)vec * V;
+        T* o = y + r * a.L + (int64_t)vec * V;
+        const int64_t step = w.rp * a.x_row, ostep = (int64_t)w.rp * a.L;
+        auto write = [&](T* to, const Vec<T, V>& v) {
+            Vec<T, V> res;
+#pragma unroll
+            for (int j = 0; j < V; ++j) res.v[j] = value(v.v[j], j);
+            *reinterpret_cast<Vec<T, V>*>(to) = res;
+        };
+        for (; r + (kUnroll - 1) * w.rp < end; r += kUnroll * w.rp, p += kUnroll * step, o += kUnroll * ostep) {
             Vec<T, V> v[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) v[u] = *reinterpret_cast<const Vec<T, V>*>(p + (r + u * w.rp) * a.x_row);
+            for (int u = 0; u < kUnroll; ++u) v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-                    Vec<T, V> res;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float xhat = (to_f(v[u].v[j]) - c.mean[j]) * c.rstd[j];
-                        res.v[j] = from_f<T>(act_value<ACT>(fmaf(xhat, c.w[j], c.b[j])));
-                    }
-                    *reinterpret_cast<Vec<T, V>*>(o + (r + u * w.rp) * a.L) = res;
-                }
+            for (int u = 0; u < kUnroll; ++u) write(o + u * ostep, v[u]);
         }
-        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)
+        for (; r < end; r += w.rp, p += step, o += ostep) write(o, *reinterpret_cast<const Vec<T, V>*>(p));
+        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)   // r == end: the short row
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (j < tail) {
-                    const float xhat = (to_f(p[end * a.x_row + j]) - c.mean[j]) * c.rstd[j];
-                    o[end * a.L + j] = from_f<T>(act_value<ACT>(fmaf(xhat, c.w[j], c.b[j])));
-                }
+                if (j < tail) o[j] = value(p[j], j);
     }
 }
 
 // ---- backward, pass 1: sum of du and of du xhat per channel over one chunk ----------------------------------------
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) gn_grad_sums_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Args a) {
     extern __shared__ float sh[];
+    let_next_start();
+    wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = blockIdx.x;
     const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
@@ -339,39 +364,48 @@ __global__ void __launch_bounds__(kThreads) gn_grad_sums_kernel(const Args a) {
         const int vec = walk_vec(a, tile);
         int tail;
         const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        const Coef<V> c = load_coef<V>(a, b, vec);
-        const T* p = x + (int64_t)vec * V;
-        const T* d = dy + (int64_t)vec * V;
-        float s1[V], s2[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-        auto add = [&](float xv, float dv, int j) {
-            const float xhat = (xv - c.mean[j]) * c.rstd[j];
-            const float du = dv * act_slope<ACT>(fmaf(xhat, c.w[j], c.b[j]));
-            s1[j] += du;
-            s2[j] = fmaf(du, xhat, s2[j]);
-        };
-        for (int64_t r = r0 + w.lane_row; r < end; r += kUnroll * w.rp) {
-            Vec<T, V> v[kUnroll], g[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-                    v[u] = *reinterpret_cast<const Vec<T, V>*>(p + (r + u * w.rp) * a.x_row);
-                    g[u] = *reinterpret_cast<const Vec<T, V>*>(d + (r + u * w.rp) * a.dy_row);
-                }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) add(to_f(v[u].v[j]), to_f(g[u].v[j]), j);
-                }
-        }
-        const bool mine = tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row;
+        float mean[V], k[V], q[V], s1[V], s2[V];   // u = k (x - mean) + q; s2 sums du (x - mean)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (mine && j < tail) add(to_f(p[end * a.x_row + j]), to_f(d[end * a.dy_row + j]), j);
+            const float4 c = load_coef(a, b, (vec * V + j) % a.C);
+            mean[j] = c.x;
+            k[j] = c.y * c.z;
+            q[j] = c.w;
+            s1[j] = s2[j] = 0.0f;
+        }
+        auto add = [&](T xv, T dv, int j) {
+            const float d = to_f(xv) - mean[j];
+            const float du = to_f(dv) * act_slope<ACT>(fmaf(d, k[j], q[j]));
+            s1[j] += du;
+            s2[j] = fmaf(du, d, s2[j]);
+        };
+        int64_t r = r0 + w.lane_row;
+        const T* p = x + r * a.x_row + (int64_t)vec * V;
+        const T* d = dy + r * a.dy_row + (int64_t)vec * V;
+        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row;
+        for (; r + (kUnroll2 - 1) * w.rp < end; r += kUnroll2 * w.rp, p += kUnroll2 * step, d += kUnroll2 * dstep) {
+            Vec<T, V> v[kUnroll2], g[kUnroll2];
+#pragma unroll
+            for (int u = 0; u < kUnroll2; ++u) {
+                v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+                g[u] = *reinterpret_cast<const Vec<T, V>*>(d + u * dstep);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll2; ++u)
+#pragma unroll
+                for (int j = 0; j < V; ++j) add(v[u].v[j], g[u].v[j], j);
+        }
+        for (; r < end; r += w.rp, p += step, d += dstep) {
+            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p), g = *reinterpret_cast<const Vec<T, V>*>(d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) add(v.v[j], g.v[j], j);
+        }
+        const bool mine = tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row;   // r == end: the short row
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (mine && j < tail) add(p[j], d[j], j);
             s_1[w.lane_row * a.L + vec * V + j] = s1[j];
-            s_2[w.lane_row * a.L + vec * V + j] = s2[j];
+            s_2[w.lane_row * a.L + vec * V + j] = s2[j] * load_coef(a, b, (vec * V + j) % a.C).y;
         }
     }
     __syncthreads();
@@ -386,34 +420,41 @@ __global__ void __launch_bounds__(kThreads) gn_grad_sums_kernel(const Args a) {
     }
 }
 
-// ---- backward, join: sums of every (image, channel) over the chunks; 32 channels x 8 lanes per CTA ----------------
-__global__ void __launch_bounds__(kJoinThreads) gn_grad_join_kernel(const Args a) {
-    __shared__ float2 sh[8][32];
-    const int ch = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5, b = a.first + blockIdx.y;
+// ---- backward, join: sums of every (image, channel) over the chunks; 16 channels x 64 lanes per CTA ---------------
+__global__ void __launch_bounds__(1024) gn_grad_join_kernel(const Args a) {
+    __shared__ float2 sh[64][16];
+    let_next_start();
+    wait_for_previous();
+    const int in = threadIdx.x & 15, ch = blockIdx.x * 16 + in, part = threadIdx.x >> 4, b = a.first + blockIdx.y;
     float2 t = make_float2(0.0f, 0.0f);
     if (ch < a.C) {
         const float2* p = reinterpret_cast<const float2*>(a.part) + (int64_t)b * a.chunks * a.C + ch;
-        for (int k = part; k < a.chunks; k += 8) {
+#pragma unroll 4
+        for (int k = part; k < a.chunks; k += 64) {
             const float2 v = p[(int64_t)k * a.C];
             t.x += v.x;
             t.y += v.y;
         }
     }
-    sh[part][threadIdx.x & 31] = t;
+    sh[part][in] = t;
     __syncthreads();
-    if (part == 0 && ch < a.C) {
-        for (int k = 1; k < 8; ++k) {
-            t.x += sh[k][threadIdx.x].x;
-            t.y += sh[k][threadIdx.x].y;
+#pragma unroll
+    for (int half = 32; half > 0; half >>= 1) {
+        if (part < half) {
+            sh[part][in].x += sh[part + half][in].x;
+            sh[part][in].y += sh[part + half][in].y;
         }
-        reinterpret_cast<float2*>(a.sums)[(int64_t)b * a.C + ch] = t;
+        __syncthreads();
     }
+    if (part == 0 && ch < a.C) reinterpret_cast<float2*>(a.sums)[(int64_t)b * a.C + ch] = sh[0][in];
 }
 
 // ---- backward, pass 2: dx, and (last turn) the parameter gradients ------------------------------------------------
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) gn_grad_apply_kernel(const Args a, int params) {
+__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const Args a, int params) {
     extern __shared__ float sh[];   // [G][2] group means of w du and w du xhat
+    let_next_start();
+    wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = a.chunks - 1 - blockIdx.x;
     const float2* sums = reinterpret_cast<const float2*>(a.sums);
     const float inv = 1.0f / (float)(a.elems / a.C * a.cpg);
@@ -460,44 +501,48 @@ __global__ void __launch_bounds__(kThreads) gn_grad_apply_kernel(const Args a, i
         const int vec = walk_vec(a, tile);
         int tail;
         const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        const Coef<V> c = load_coef<V>(a, b, vec);
-        float m1[V], m2[V];
+        float k[V], q[V], kx[V], kc[V];   // u = k x + q, dx = k du + kx x + kc
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int g = (vec * V + j) % a.C / a.cpg;
-            m1[j] = sh[g * 2];
-            m2[j] = sh[g * 2 + 1];
+            const int ch = (vec * V + j) % a.C;
+            const float4 c = load_coef(a, b, ch);
+            const float m1 = sh[ch / a.cpg * 2], m2 = sh[ch / a.cpg * 2 + 1];
+            k[j] = c.y * c.z;
+            q[j] = fmaf(-c.x, k[j], c.w);
+            kx[j] = -c.y * c.y * m2;
+            kc[j] = fmaf(-c.x, kx[j], -c.y * m1);
         }
-        const T* p = x + (int64_t)vec * V;
-        const T* d = dy + (int64_t)vec * V;
-        T* o = dx + (int64_t)vec * V;
-        auto value = [&](float xv, float dv, int j) {
-            const float xhat = (xv - c.mean[j]) * c.rstd[j];
-            const float du = dv * act_slope<ACT>(fmaf(xhat, c.w[j], c.b[j]));
-            return c.rstd[j] * (fmaf(c.w[j], du, -m1[j]) - xhat * m2[j]);
+        auto value = [&](T xv, T dv, int j) {
+            const float x = to_f(xv), du = to_f(dv) * act_slope<ACT>(fmaf(x, k[j], q[j]));
+            return from_f<T>(fmaf(k[j], du, fmaf(kx[j], x, kc[j])));
         };
-        for (int64_t r = r0 + w.lane_row; r < end; r += kUnroll * w.rp) {
-            Vec<T, V> v[kUnroll], g[kUnroll];
+        int64_t r = r0 + w.lane_row;
+        const T* p = x + r * a.x_row + (int64_t)vec * V;
+        const T* d = dy + r * a.dy_row + (int64_t)vec * V;
+        T* o = dx + r * a.L + (int64_t)vec * V;
+        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row, ostep = (int64_t)w.rp * a.L;
+        auto write = [&](T* to, const Vec<T, V>& v, const Vec<T, V>& g) {
+            Vec<T, V> res;
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-                    v[u] = *reinterpret_cast<const Vec<T, V>*>(p + (r + u * w.rp) * a.x_row);
-                    g[u] = *reinterpret_cast<const Vec<T, V>*>(d + (r + u * w.rp) * a.dy_row);
-                }
+            for (int j = 0; j < V; ++j) res.v[j] = value(v.v[j], g.v[j], j);
+            *reinterpret_cast<Vec<T, V>*>(to) = res;
+        };
+        for (; r + (kUnroll2 - 1) * w.rp < end; r += kUnroll2 * w.rp, p += kUnroll2 * step, d += kUnroll2 * dstep, o += kUnroll2 * ostep) {
+            Vec<T, V> v[kUnroll2], g[kUnroll2];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * w.rp < end) {
-                    Vec<T, V> res;
+            for (int u = 0; u < kUnroll2; ++u) {
+                v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+                g[u] = *reinterpret_cast<const Vec<T, V>*>(d + u * dstep);
+            }
 #pragma unroll
-                    for (int j = 0; j < V; ++j) res.v[j] = from_f<T>(value(to_f(v[u].v[j]), to_f(g[u].v[j]), j));
-                    *reinterpret_cast<Vec<T, V>*>(o + (r + u * w.rp) * a.L) = res;
-                }
+            for (int u = 0; u < kUnroll2; ++u) write(o + u * ostep, v[u], g[u]);
         }
-        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)
+        for (; r < end; r += w.rp, p += step, d += dstep, o += ostep)
+            write(o, *reinterpret_cast<const Vec<T, V>*>(p), *reinterpret_cast<const Vec<T, V>*>(d));
+        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)   // r == end: the short row
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (j < tail)
-                    o[end * a.L + j] = from_f<T>(value(to_f(p[end * a.x_row + j]), to_f(d[end * a.dy_row + j]), j));
+                if (j < tail) o[j] = value(p[j], d[j], j);
     }
 }
 
@@ -538,13 +583,13 @@ int images_per_turn(const D3gsGroupNorm& d, bool backward) {
     return (int)(n < 1 ? 1 : n);
 }
 
-// Chunks of one image: enough CTAs in a turn for four on every SM, none with less than 16 rows a thread, at most 1024.
+// Chunks of one image: as many CTAs in a turn as run at once, none with less than two vectors a thread.
 int chunks_of(const D3gsGroupNorm& d, bool backward) {
     const int turn = images_per_turn(d, backward);
-    const int64_t want = div_up64(4 * 148, turn), values = d.pixels * d.channels;
+    const int64_t want = div_up64((backward ? kCtas2 : kCtas) * 148, turn), values = d.pixels * d.channels;
     const int64_t most = div_up64(values, (int64_t)kThreads * (16 / elem_size(d.dtype)) * 2);
     int64_t n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+    return (int)(n < 1 ? 1 : n > kMaxChunks ? kMaxChunks : n);
 }
 
 int32_t check(const D3gsGroupNorm* d, const char* what) {
@@ -602,9 +647,21 @@ Args make_args(const D3gsGroupNorm& d, int v, bool backward, void* ws) {
     return a;
 }
 
-// more than 48 KB of shared memory is asked for once per kernel and device, before its launch
-template <typename K> int32_t allow_smem(K kernel, size_t bytes) {
-    if (bytes > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+template <typename K, typename... A>
+int32_t launch(K kernel, const char* name, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = 1;
+    D3GS_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
+    D3GS_LAUNCH_CHECK(name);
     return D3GS_OK;
 }
 
@@ -612,17 +669,13 @@ template <typename T, int V, int ACT>
 int32_t run_forward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, false);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
-    const size_t smem = slots * 12;
-    if (int32_t rc = allow_smem(gn_stats_kernel<T, V>, smem)) return rc;
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;
-        gn_stats_kernel<T, V><<<dim3(a.chunks, images), kThreads, smem, st>>>(a);
-        D3GS_LAUNCH_CHECK("gn_stats_kernel");
-        gn_stats_join_kernel<<<(unsigned)div_up64((int64_t)images * a.G, kJoinThreads / 32), kJoinThreads, 0, st>>>(a, images);
-        D3GS_LAUNCH_CHECK("gn_stats_join_kernel");
-        gn_apply_kernel<T, V, ACT><<<dim3(a.chunks, images), kThreads, 0, st>>>(a);
-        D3GS_LAUNCH_CHECK("gn_apply_kernel");
+        const dim3 grid(a.chunks, images);
+        if (int32_t rc = launch(gn_stats_kernel<T, V>, "gn_stats_kernel", grid, kThreads, slots * 12, st, a)) return rc;
+        if (int32_t rc = launch(gn_stats_join_kernel, "gn_stats_join_kernel", dim3(images * a.G), kJoinThreads, 0, st, a)) return rc;
+        if (int32_t rc = launch(gn_apply_kernel<T, V, ACT>, "gn_apply_kernel", grid, kThreads, 0, st, a)) return rc;
     }
     return D3GS_OK;
 }
@@ -631,18 +684,15 @@ template <typename T, int V, int ACT>
 int32_t run_backward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, true);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
-    if (int32_t rc = allow_smem(gn_grad_sums_kernel<T, V, ACT>, slots * 8)) return rc;
-    if (int32_t rc = allow_smem(gn_grad_apply_kernel<T, V, ACT>, (size_t)a.G * 8)) return rc;
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;
-        gn_grad_sums_kernel<T, V, ACT><<<dim3(a.chunks, images), kThreads, slots * 8, st>>>(a);
-        D3GS_LAUNCH_CHECK("gn_grad_sums_kernel");
-        gn_grad_join_kernel<<<dim3((a.C + 31) / 32, images), kJoinThreads, 0, st>>>(a);
-        D3GS_LAUNCH_CHECK("gn_grad_join_kernel");
+        const dim3 grid(a.chunks, images);
+        if (int32_t rc = launch(gn_grad_sums_kernel<T, V, ACT>, "gn_grad_sums_kernel", grid, kThreads, slots * 8, st, a)) return rc;
+        if (int32_t rc = launch(gn_grad_join_kernel, "gn_grad_join_kernel", dim3((a.C + 15) / 16, images), 1024, 0, st, a)) return rc;
         const int params = b + images == a.batch && (a.dweight || a.dbias);
-        gn_grad_apply_kernel<T, V, ACT><<<dim3(a.chunks, images), kThreads, (size_t)a.G * 8, st>>>(a, params);
-        D3GS_LAUNCH_CHECK("gn_grad_apply_kernel");
+        if (int32_t rc = launch(gn_grad_apply_kernel<T, V, ACT>, "gn_grad_apply_kernel", grid, kThreads, (size_t)a.G * 8, st, a, params))
+            return rc;
     }
     return D3GS_OK;
 }

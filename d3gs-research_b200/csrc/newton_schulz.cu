@@ -36,7 +36,7 @@
 namespace d3gs {
 namespace {
 
-constexpr int kMaxMatrices = 64;   // per launch; longer lists are cut
+constexpr int kMaxMatrices = 32;   // per launch, a table of less than 4 KB; longer lists are cut
 constexpr int kThreads = 256;
 constexpr int kNormChunk = 8192;   // values per CTA of the norm pass
 constexpr int kMaxShort = 16384, kMaxLong = 1 << 24;

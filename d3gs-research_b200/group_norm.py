@@ -7,6 +7,7 @@ reference has no counterpart.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -19,7 +20,11 @@ _ACTS = {"none": 0, "silu": 1, "gelu": 2}
 def _pixel_strides(t: torch.Tensor):
     """(image stride, pixel stride) of [B, *spatial, C] when its channels are dense and its pixels evenly spaced,
     else None."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
+    if t.is_contiguous():
+        n = t.numel()
+        return (n // shape[0] if n else 0), shape[-1]
+    stride = t.stride()
     if t.numel() == 0:
         return 0, shape[-1]
     if shape[-1] > 1 and stride[-1] != 1:
@@ -44,17 +49,6 @@ def _prepared(t: torch.Tensor):
     return t, strides
 
 
-def _desc(x: torch.Tensor, strides, groups: int, wdtype, act: int, eps: float) -> _lib.GroupNorm:
-    d = _lib.GroupNorm()
-    d.batch, d.channels, d.groups = x.shape[0], x.shape[-1], groups
-    d.pixels = 1
-    for n in x.shape[1:-1]:
-        d.pixels *= n
-    d.x_batch_stride, d.x_pixel_stride = strides
-    d.dtype, d.weight_dtype, d.act, d.eps = _DTYPES[x.dtype], _DTYPES[wdtype], act, eps
-    return d
-
-
 def _workspace(lib, d: _lib.GroupNorm, backward: int, device):
     n = lib.d3gs_group_norm_workspace_bytes(C.byref(d), backward)
     if n == 0:
@@ -63,50 +57,58 @@ def _workspace(lib, d: _lib.GroupNorm, backward: int, device):
 
 
 def _forward(x, groups, weight, bias, eps, act):
+    device = x.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _forward(x, groups, weight, bias, eps, act)
     lib = _lib.load()
-    x, strides = _prepared(x)
+    x, (image, pixel) = _prepared(x)
+    shape = x.shape
     wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    d = _desc(x, strides, groups, wdtype, act, eps)
-    with torch.cuda.device(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
-        ws, n = _workspace(lib, d, 0, x.device)
-        _lib.check(lib.d3gs_group_norm_forward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), y.data_ptr(),
-                                               stats.data_ptr(), ws.data_ptr(), n,
-                                               torch.cuda.current_stream().cuda_stream), "d3gs_group_norm_forward")
+    d = _lib.GroupNorm(shape[0], math.prod(shape[1:-1]), image, pixel, 0, 0, shape[-1], groups, _DTYPES[x.dtype],
+                       _DTYPES[wdtype], act, eps)
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    stats = torch.empty((shape[0], groups, 2), dtype=torch.float32, device=device)
+    ws, n = _workspace(lib, d, 0, device)
+    _lib.check(lib.d3gs_group_norm_forward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), y.data_ptr(),
+                                           stats.data_ptr(), ws.data_ptr(), n, _lib.raw_stream(device.index)),
+               "d3gs_group_norm_forward")
     return x, y, stats, d
+
+
+def _backward(d, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b: bool):
+    device = x.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _backward(d, x, weight, bias, stats, dy, need_x, need_w, need_b)
+    lib = _lib.load()
+    d = _lib.GroupNorm.from_buffer_copy(d)
+    dy, (d.dy_batch_stride, d.dy_pixel_stride) = _prepared(dy)
+    empty = x.numel() == 0
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+    make = torch.zeros_like if empty else torch.empty_like
+    dw = make(weight) if need_w else None
+    db = make(bias) if need_b else None
+    if not empty and (need_x or need_w or need_b):
+        ws, n = _workspace(lib, d, 1, device)
+        _lib.check(lib.d3gs_group_norm_backward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias),
+                                                stats.data_ptr(), dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
+                                                _lib.ptr(db), ws.data_ptr(), n, _lib.raw_stream(device.index)),
+                   "d3gs_group_norm_backward")
+    return dx, dw, db
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups: int, eps: float, act: int):
-        x, y, stats, d = _forward(x.detach(), groups, weight, bias, eps, act)
+        x, y, stats, ctx.desc = _forward(x.detach(), groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.desc = d
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        lib = _lib.load()
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        d = _lib.GroupNorm.from_buffer_copy(ctx.desc)
-        dy, (d.dy_batch_stride, d.dy_pixel_stride) = _prepared(dy)
-        empty = x.numel() == 0
-        with torch.cuda.device(x.device):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            make = torch.zeros_like if empty else torch.empty_like
-            dw = make(weight) if need_w else None
-            db = make(bias) if need_b else None
-            if not empty and (need_x or need_w or need_b):
-                ws, n = _workspace(lib, d, 1, x.device)
-                _lib.check(lib.d3gs_group_norm_backward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias),
-                                                        stats.data_ptr(), dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
-                                                        _lib.ptr(db), ws.data_ptr(), n,
-                                                        torch.cuda.current_stream().cuda_stream),
-                           "d3gs_group_norm_backward")
-        return dx, dw, db, None, None, None
+        return (*_backward(ctx.desc, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
@@ -132,9 +134,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"group_norm_act: eps must be finite and not negative, got {eps}")
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if tuple(t.shape) != (c,) or t.device != x.device or t.dtype not in _DTYPES:
+        if t is not None and (t.dim() != 1 or t.shape[0] != c or t.device != x.device or t.dtype not in _DTYPES):
             raise ValueError(f"group_norm_act: {name} must be [{c}] on {x.device} in float32, bfloat16 or float16, got "
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:

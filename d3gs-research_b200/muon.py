@@ -38,14 +38,15 @@ def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib
 
 
 def _run(entry: str, mats, count: int, cfg: _lib.OrthoConfig, device):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _run(entry, mats, count, cfg, device)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        n = lib.d3gs_orthogonalize_workspace_bytes(mats, count, C.byref(cfg))
-        if n == 0:
-            raise RuntimeError(f"{entry}: {_lib.last_error()}")
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
-        _lib.check(getattr(lib, entry)(mats, count, C.byref(cfg), ws.data_ptr(), n,
-                                       torch.cuda.current_stream().cuda_stream), entry)
+    n = lib.d3gs_orthogonalize_workspace_bytes(mats, count, C.byref(cfg))
+    if n == 0:
+        raise RuntimeError(f"{entry}: {_lib.last_error()}")
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    _lib.check(getattr(lib, entry)(mats, count, C.byref(cfg), ws.data_ptr(), n, _lib.raw_stream(device.index)), entry)
 
 
 @torch.no_grad()
@@ -73,9 +74,7 @@ def orthogonalize(update: torch.Tensor, ns_coefficients: Sequence = NS_COEFFICIE
     count, step, size = src.shape[0], src.stride(0) * src.element_size(), src.element_size()
     mats = (_lib.OrthoMatrix * count)()
     for k in range(count):
-        d = mats[k]
-        d.src, d.dst = src.data_ptr() + k * step, out.data_ptr() + k * m * n * size
-        d.rows, d.cols, d.src_row_stride = m, n, src.stride(1)
+        mats[k] = (src.data_ptr() + k * step, None, out.data_ptr() + k * m * n * size, m, n, src.stride(1), 0.0, 0)
     _run("d3gs_orthogonalize", mats, count, cfg, update.device)
     return out
 
@@ -141,27 +140,26 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
             raise ValueError(f"muon_step: parameters on {device} and {p.device} in one call")
         if p.numel() == 0:
             continue
-        if not _dense_rows(p) or not _same_order(p, buf):
+        plain = p.is_contiguous()
+        if not (plain and buf.is_contiguous()) and (not _dense_rows(p) or not _same_order(p, buf)):
             raise ValueError(f"muon_step: a parameter of strides {p.stride()} or its buffer of strides {buf.stride()} is not "
                              "dense (contiguous or channels last, the two alike)")
         rows, cols = p.shape[0], p.numel() // p.shape[0]
         row_stride = cols
-        if not _same_order(p, g):
+        if not (plain and g.is_contiguous()) and not _same_order(p, g):
             if g.dim() == 2 and (cols == 1 or g.stride(1) == 1) and p.is_contiguous():
                 row_stride = g.stride(0)
             else:
                 g = torch.empty_like(p).copy_(g)
                 keep.append(g)
-        d = mats[count]
-        d.src, d.momentum, d.dst = g.data_ptr(), buf.data_ptr(), p.data_ptr()
-        d.rows, d.cols, d.src_row_stride = rows, cols, row_stride
-        d.rate = _adjusted_lr(lr, rows, cols, adjust_lr_fn)
-        spans += [(d.momentum, rows * cols * 4), (d.dst, rows * cols * 4)]
+        at, state, size = p.data_ptr(), buf.data_ptr(), rows * cols * 4
+        mats[count] = (g.data_ptr(), state, at, rows, cols, row_stride, _adjusted_lr(lr, rows, cols, adjust_lr_fn), 0)
+        spans += [(state, state + size), (at, at + size)]
         count += 1
     if count == 0:
         return
     spans.sort()
-    if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("muon_step: parameters or buffers overlap (is one given twice?)")
     _run("d3gs_muon_step", mats, count, cfg, device)
     torch.autograd.graph.increment_version([*params, *momentum_buffers])

@@ -16,16 +16,21 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace d3gs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4, kUnroll2 = 2;   // rows in flight per thread: kernels that read x, that read x and dy
-constexpr int kCtas = 4, kCtas2 = 3;       // and their CTAs per SM, which the registers are bounded for
+// Rows in flight per thread in the kernels that read x, and in those that read x and dy, and their CTAs per SM, which
+// the registers are bounded for.  Few CTAs with many loads each do better than many with few: 4 x 1080p x 32 channels
+// in 16 bits, forward 413 us with 4 rows and 4 CTAs, 343 us with 8 and 2; backward 664 us with 2 and 3, 544 with 4 and 2.
+constexpr int kUnroll = 8, kUnroll2 = 4;
+constexpr int kCtas = 2, kCtas2 = 2;
 constexpr int kMaxChannels = 16384;       // per-channel sums of one CTA stay in shared memory
-constexpr int64_t kTurnBytes = 48 << 20;  // inputs of one turn, to be found in L2 (126 MB) by the second pass
+constexpr int64_t kTurnBytes = 72 << 20;  // inputs of one turn, to be found in L2 (126 MB) by the second pass
 constexpr int kJoinThreads = 256, kMaxChunks = 1024;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2 };
@@ -49,27 +54,109 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int i, float v) 
     else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T v[V]; };
-
-// The logistic function by ex2 and reciprocal of the special-function unit, about 2e-7 relative; u -> -inf gives 0.
-__device__ __forceinline__ float logistic(float u) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-u)));
+// ---- values in pairs: the packed 32-bit operations of sm_100 take two per instruction -----------------------------
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ float2 split(Two v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
 
-template <int ACT> __device__ __forceinline__ float act_value(float u) {
-    if (ACT == kActSilu) return u * logistic(u);
-    if (ACT == kActGelu) return 0.5f * u * (1.0f + erff(u * 0.70710678f));
+// V neighbouring values as they lie in memory; `pair(i)` gives values 2 i and 2 i + 1 (a single value comes twice).
+template <typename T, int V> struct alignas(sizeof(T) * V) Vec {
+    T v[V];
+    __device__ __forceinline__ Two pair(int i) const {
+        if constexpr (V == 1) return both(to_f(v[0]));
+        else if constexpr (sizeof(T) == 4) return two(to_f(v[2 * i]), to_f(v[2 * i + 1]));
+        else {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(v)[i];
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+            else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                return two(f.x, f.y);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(int i, Two x) {
+        const float2 f = split(x);
+        if constexpr (V == 1) v[0] = from_f<T>(f.x);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(v)[i] = __floats2bfloat162_rn(f.x, f.y);
+        else if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(v)[i] = __floats2half2_rn(f.x, f.y);
+        else {
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+// The first pass over an image reads it plainly, for the second to find in L2; what the second reads and writes is not
+// looked at again and should not drive the rest out.
+template <typename T, int V> __device__ __forceinline__ Vec<T, V> load(const T* p) { return *reinterpret_cast<const Vec<T, V>*>(p); }
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+template <> struct Raw<4> { typedef uint32_t type; };
+template <> struct Raw<2> { typedef unsigned short type; };
+template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_last(const T* p) {
+    typedef typename Raw<sizeof(T) * V>::type R;
+    const R r = __ldcs(reinterpret_cast<const R*>(p));
+    return *reinterpret_cast<const Vec<T, V>*>(&r);
+}
+template <typename T, int V> __device__ __forceinline__ void store_last(T* p, const Vec<T, V>& v) {
+    typedef typename Raw<sizeof(T) * V>::type R;
+    __stcs(reinterpret_cast<R*>(p), *reinterpret_cast<const R*>(&v));
+}
+
+// The logistic function by ex2 and reciprocal of the special-function unit, about 2e-7 relative; u -> -inf gives 0.
+__device__ __forceinline__ Two logistic(Two u) {
+    float2 e = split(mul2(u, both(-1.44269504f)));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    e = split(add2(two(e.x, e.y), both(1.0f)));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    return two(e.x, e.y);
+}
+// twice the normal distribution function
+__device__ __forceinline__ Two gauss2(Two u) {
+    const float2 f = split(mul2(u, both(0.70710678f)));
+    return add2(two(erff(f.x), erff(f.y)), both(1.0f));
+}
+template <int ACT> __device__ __forceinline__ Two act_value(Two u) {
+    if (ACT == kActSilu) return mul2(u, logistic(u));
+    if (ACT == kActGelu) return mul2(mul2(u, both(0.5f)), gauss2(u));
     return u;
 }
-template <int ACT> __device__ __forceinline__ float act_slope(float u) {
+template <int ACT> __device__ __forceinline__ Two act_slope(Two u) {
     if (ACT == kActSilu) {
-        const float s = logistic(u);
-        return s * fmaf(u, 1.0f - s, 1.0f);
+        const Two s = logistic(u);
+        return mul2(s, fma2(u, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
     }
-    if (ACT == kActGelu) return fmaf(u * 0.39894228f, __expf(-0.5f * u * u), 0.5f * (1.0f + erff(u * 0.70710678f)));
-    return 1.0f;
+    if (ACT == kActGelu) {
+        const float2 f = split(mul2(mul2(u, u), both(-0.5f)));
+        return fma2(mul2(u, both(0.39894228f)), two(__expf(f.x), __expf(f.y)), mul2(gauss2(u), both(0.5f)));
+    }
+    return both(1.0f);
 }
 
 // Launches follow one another closely: a kernel may start while its predecessor's last CTAs run, and waits here before
@@ -83,15 +170,17 @@ struct Args {
     float* stats;                // [B,G,2] mean, rstd
     float* part;                 // forward [B,G,chunks,2] mean, M2; backward [B,chunks,C,2] sum du, sum du xhat
     float* sums;                 // backward [B,C,2]
+    float* coef;                 // forward [B,C,2] k, q; backward [B,C,4] k, q, kx, kc: see the second passes
     int64_t elems;               // values of one image
     int64_t rows;                // rows of one image (the last may be short)
-    int64_t chunk_rows;
+    int tiles, tile_rows, whole_tiles;   // of an image; whole_tiles: those in which every row is whole
     int64_t x_batch, x_row, dy_batch, dy_row, y_batch;   // strides in values
     int batch, chunks, C, G, cpg;
     int L, P;                    // values and vectors per row
     int first;                   // first image of this turn
     int wdtype, act;
-    float eps;
+    float eps, share;            // share: 1 / G, of a pixel's values that belong to one group
+    float per_cpg;               // 1 / cpg: (c + 1/2) / cpg cut to an integer is c's group
 };
 
 // What a thread of the walk owns: vector `vec` of rows r0 + lane_row, step rows apart.
@@ -99,7 +188,7 @@ struct Walk {
     int rp, lane_row;            // rows the CTA takes at once, this thread's row among them
     bool on;
 };
-__device__ __forceinline__ Walk make_walk(const Args& a, int tile) {
+__device__ __forceinline__ Walk make_walk(const Args& a, int v0) {
     Walk w;
     if (a.P <= kThreads) {
         w.rp = kThreads / a.P;
@@ -108,22 +197,31 @@ __device__ __forceinline__ Walk make_walk(const Args& a, int tile) {
     } else {
         w.rp = 1;
         w.lane_row = 0;
-        w.on = tile * kThreads + (int)threadIdx.x < a.P;
+        w.on = v0 + (int)threadIdx.x < a.P;
     }
     return w;
 }
-__device__ __forceinline__ int walk_vec(const Args& a, int tile) {
-    return a.P <= kThreads ? (int)threadIdx.x % a.P : tile * kThreads + (int)threadIdx.x;
-}
 
-// Rows of [r0, r1) in which vector `vec` is whole, and how many of its values the row after them holds (0: none).
-template <int V> __device__ __forceinline__ int64_t whole_rows(const Args& a, int64_t r1, int vec, int& tail) {
-    tail = 0;
-    if (r1 < a.rows) return r1;
-    const int64_t left = a.elems - (a.rows - 1) * (int64_t)a.L - (int64_t)vec * V;   // in the last row, from this vector on
-    if (left >= V) return r1;
-    tail = left > 0 ? (int)left : 0;
-    return r1 - 1;
+// An image's rows are cut into tiles of rp * unroll rows, and a CTA takes every chunks-th of them: at any time the whole
+// grid reads one window of the image.  The second passes go through the tiles from the last to the first, the order in
+// which L2 still holds them: of a 133 MB image half is found there.
+__device__ __forceinline__ int tiles_of(const Args& a, int chunk) { return (a.tiles - 1 - chunk) / a.chunks + 1; }
+// values of vector `vec` that row `row` has: V, or fewer at the image's end
+template <int V> __device__ __forceinline__ int valid(const Args& a, int64_t row, int vec) {
+    const int64_t left = a.elems - row * a.L - (int64_t)vec * V;
+    return left >= V ? V : left > 0 ? (int)left : 0;
+}
+template <typename T, int V> __device__ __forceinline__ Vec<T, V> load_some(const T* p, int n) {
+    Vec<T, V> v{};
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) v.v[j] = p[j];
+    return v;
+}
+template <typename T, int V> __device__ __forceinline__ void store_some(T* p, const Vec<T, V>& v, int n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) p[j] = v.v[j];
 }
 
 // ---- forward, pass 1: mean and centred square sum of every group over one chunk of one image ----------------------
@@ -136,56 +234,80 @@ __global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a)
     let_next_start();
     wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = blockIdx.x;
-    const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const int slots = (a.P <= kThreads ? kThreads / a.P : 1) * a.L;   // entries of the CTA: [row][value of the row]
     float *s_n = sh, *s_mean = sh + slots, *s_m2 = sh + 2 * slots;
-    const int tiles = a.P <= kThreads ? 1 : (a.P + kThreads - 1) / kThreads;
-    for (int tile = 0; tile < tiles; ++tile) {
-        const Walk w = make_walk(a, tile);
+    for (int v0 = 0; v0 < a.P; v0 += kThreads) {
+        const Walk w = make_walk(a, v0);
         if (!w.on) continue;
-        const int vec = walk_vec(a, tile);
-        int tail;
-        const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        const T* p = x + (int64_t)vec * V;
-        float k[V], s[V], q[V];
+        const int vec = v0 + (a.P <= kThreads ? (int)threadIdx.x % a.P : (int)threadIdx.x);
+        constexpr int H = (V + 1) / 2;
+        const int64_t step = w.rp * a.x_row, next = (int64_t)a.chunks * a.tile_rows * a.x_row;
+        const int64_t row0 = (int64_t)chunk * a.tile_rows + w.lane_row;
+        const T* p = x + row0 * a.x_row + (int64_t)vec * V;
+        Two minus[H], sum[H], square[H];   // minus: -k
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = q[j] = k[j] = 0.0f;
-        int64_t r = r0 + w.lane_row;
-        const int64_t step = w.rp * a.x_row;
-        p += r * a.x_row;
-        const int got = r < end ? (int)min((int64_t)kUnroll, (end - r + w.rp - 1) / w.rp) : 0;
-        for (int u = 0; u < got; ++u) {
-            const Vec<T, V> f = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+        for (int i = 0; i < H; ++i) minus[i] = sum[i] = square[i] = both(0.0f);
+        int got = 0;
+        Vec<T, V> f[kUnroll];
 #pragma unroll
-            for (int j = 0; j < V; ++j) k[j] += to_f(f.v[j]);
-        }
+        for (int u = 0; u < kUnroll; ++u)
+            if (valid<V>(a, row0 + u * w.rp, vec) == V) {
+                f[u] = load<T, V>(p + u * step);
+                ++got;
+            }
 #pragma unroll
-        for (int j = 0; j < V; ++j) k[j] /= (float)max(got, 1);
+        for (int u = 0; u < kUnroll; ++u)
+            if (u < got) {
+#pragma unroll
+                for (int i = 0; i < H; ++i) minus[i] = add2(minus[i], f[u].pair(i));
+            }
+#pragma unroll
+        for (int i = 0; i < H; ++i) minus[i] = mul2(minus[i], both(-1.0f / max(got, 1)));
         auto add = [&](const Vec<T, V>& x) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = to_f(x.v[j]) - k[j];
-                s[j] += d;
-                q[j] = fmaf(d, d, q[j]);
+            for (int i = 0; i < H; ++i) {
+                const Two d = add2(x.pair(i), minus[i]);
+                sum[i] = add2(sum[i], d);
+                square[i] = fma2(d, d, square[i]);
             }
         };
-        int n = 0;
-        for (; r + (kUnroll - 1) * w.rp < end; r += kUnroll * w.rp, p += kUnroll * step, n += kUnroll) {
-            Vec<T, V> v[kUnroll];
+        int n = 0, tail = 0;        // rows, and values of the short row when it is this thread's
+        const T* short_row = p;
+        for (int i = tiles_of(a, chunk), tile = chunk; i > 0; --i, tile += a.chunks, p += next) {
+            if (tile < a.whole_tiles) {
+                Vec<T, V> v[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+                for (int u = 0; u < kUnroll; ++u) v[u] = load<T, V>(p + u * step);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) add(v[u]);
+                for (int u = 0; u < kUnroll; ++u) add(v[u]);
+                n += kUnroll;
+            } else {
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int has = valid<V>(a, (int64_t)tile * a.tile_rows + w.lane_row + u * w.rp, vec);
+                    if (has == V) {
+                        add(load<T, V>(p + u * step));
+                        ++n;
+                    } else if (has > 0) {
+                        tail = has;
+                        short_row = p + u * step;
+                    }
+                }
+            }
         }
-        for (; r < end; r += w.rp, p += step, ++n) add(*reinterpret_cast<const Vec<T, V>*>(p));
-        // the short row at the image's end belongs to the thread whose turn it is
-        const bool mine = tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row;
+        float k[V], s[V], q[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 m = split(minus[j / 2]), t = split(sum[j / 2]), z = split(square[j / 2]);
+            k[j] = j & 1 ? -m.y : -m.x;
+            s[j] = j & 1 ? t.y : t.x;
+            q[j] = j & 1 ? z.y : z.x;
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             int nj = n;
-            if (mine && j < tail) {
-                const float v = to_f(p[j]);   // r == end
+            if (j < tail) {
+                const float v = to_f(short_row[j]);
                 if (n == 0) k[j] = v;
                 const float d = v - k[j];
                 s[j] += d;
@@ -201,45 +323,55 @@ __global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a)
         }
     }
     __syncthreads();
-    // one warp per group joins its entries: first the mean, then the squares around it
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int pixels = slots / a.C, items = pixels * a.cpg;
-    for (int g = warp; g < a.G; g += kThreads / 32) {
+    // `lanes` threads join the entries of a group: first the mean, then the squares around it
+    int lanes = 32;
+    while (lanes > 1 && lanes * a.G > kThreads) lanes >>= 1;
+    const int lane = threadIdx.x & (lanes - 1), pixels = slots / a.C;
+    const int px0 = lane / a.cpg, ci0 = lane % a.cpg, dpx = lanes / a.cpg, dci = lanes % a.cpg;
+    auto each = [&](int g, auto f) {
+        for (int px = px0, ci = ci0; px < pixels;) {
+            f(px * a.C + g * a.cpg + ci);
+            px += dpx;
+            ci += dci;
+            if (ci >= a.cpg) {
+                ci -= a.cpg;
+                ++px;
+            }
+        }
+    };
+    auto lanes_sum = [&](float v) {
+        for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        return v;
+    };
+    for (int g0 = 0; g0 < a.G; g0 += kThreads / lanes) {
+        const int g = min(g0 + (int)threadIdx.x / lanes, a.G - 1);   // (whole warps take part in the sums)
         const float near = s_mean[g * a.cpg];   // a value of the group's size: differences from it are added up
-        float n = 0.0f, t = 0.0f;
-        for (int i = lane; i < items; i += 32) {
-            const int e = (i / a.cpg) * a.C + g * a.cpg + i % a.cpg;
+        float n = 0.0f, t = 0.0f, m2 = 0.0f;
+        each(g, [&](int e) {
             n += s_n[e];
             if (s_n[e] > 0.0f) t = fmaf(s_n[e], s_mean[e] - near, t);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            n += __shfl_xor_sync(~0u, n, o);
-            t += __shfl_xor_sync(~0u, t, o);
-        }
+        });
+        n = lanes_sum(n);
+        t = lanes_sum(t);
         const float mean = n > 0.0f ? near + t / n : 0.0f;
-        float m2 = 0.0f;
-        for (int i = lane; i < items; i += 32) {
-            const int e = (i / a.cpg) * a.C + g * a.cpg + i % a.cpg;
+        each(g, [&](int e) {
             if (s_n[e] > 0.0f) {
                 const float d = s_mean[e] - mean;
                 m2 += fmaf(s_n[e] * d, d, s_m2[e]);
             }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o);
-        if (lane == 0) {
-            float* out = a.part + (((int64_t)b * a.G + g) * a.chunks + chunk) * 2;
-            out[0] = mean;
-            out[1] = m2;
-        }
+        });
+        m2 = lanes_sum(m2);
+        if (lane == 0 && g0 + (int)threadIdx.x / lanes < a.G)
+            reinterpret_cast<float2*>(a.part)[((int64_t)b * a.G + g) * a.chunks + chunk] = make_float2(mean, m2);
     }
 }
 
 // values of one group in one chunk
 __device__ __forceinline__ float chunk_count(const Args& a, int chunk) {
-    const int64_t e0 = chunk * a.chunk_rows * a.L, e1 = min(a.elems, (chunk + 1) * a.chunk_rows * a.L);
-    return (float)((e1 - e0) / a.C * a.cpg);
+    const int n = tiles_of(a, chunk);
+    int64_t e = (int64_t)n * a.tile_rows * a.L;
+    if (chunk + (n - 1) * a.chunks == a.tiles - 1) e -= (int64_t)a.tiles * a.tile_rows * a.L - a.elems;   // the last tile
+    return (float)e * a.share;
 }
 
 // ---- forward, join: one CTA per (image, group) over the chunks ----------------------------------------------------
@@ -259,7 +391,7 @@ __global__ void __launch_bounds__(kJoinThreads) gn_stats_join_kernel(const Args 
     wait_for_previous();
     const int64_t bg = (int64_t)a.first * a.G + blockIdx.x;
     const float2* part = reinterpret_cast<const float2*>(a.part) + bg * a.chunks;
-    const float total = (float)(a.elems / a.C * a.cpg), near = part[0].x;
+    const float total = (float)a.elems * a.share, near = part[0].x;
     float2 mine[kMaxChunks / kJoinThreads];
     float t = 0.0f;
 #pragma unroll
@@ -283,17 +415,20 @@ __global__ void __launch_bounds__(kJoinThreads) gn_stats_join_kernel(const Args 
         }
     }
     m2 = cta_sum(m2, sh[1]);
-    if (threadIdx.x == 0) {
-        a.stats[bg * 2] = mean;
-        a.stats[bg * 2 + 1] = 1.0f / sqrtf(m2 / total + a.eps);
+    const float rstd = 1.0f / sqrtf(m2 / total + a.eps);
+    if (threadIdx.x == 0) reinterpret_cast<float2*>(a.stats)[bg] = make_float2(mean, rstd);
+    const int first = (int)(bg % a.G) * a.cpg;
+    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads) {
+        const float k = rstd * (a.weight ? load_param(a.weight, a.wdtype, first + i) : 1.0f);
+        reinterpret_cast<float2*>(a.coef)[bg * a.cpg + i] =
+            make_float2(k, fmaf(-mean, k, a.bias ? load_param(a.bias, a.wdtype, first + i) : 0.0f));
     }
 }
 
-// mean, rstd, weight and bias of channel `ch` of image b
-__device__ __forceinline__ float4 load_coef(const Args& a, int b, int ch) {
-    const float2 st = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + ch / a.cpg];
-    return make_float4(st.x, st.y, a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f,
-                       a.bias ? load_param(a.bias, a.wdtype, ch) : 0.0f);
+// channel of value j of a vector
+template <int V> __device__ __forceinline__ int channel(const Args& a, int vec, int j) {
+    const int e = vec * V + (V == 1 ? 0 : j);
+    return a.L == a.C ? e : e % a.C;
 }
 
 // ---- forward, pass 2 -----------------------------------------------------------------------------------------------
@@ -301,47 +436,47 @@ template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a) {
     let_next_start();
     wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = a.chunks - 1 - blockIdx.x;   // last read first: still in L2
-    const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
+    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     T* y = static_cast<T*>(a.y) + b * a.y_batch;
-    const int tiles = a.P <= kThreads ? 1 : (a.P + kThreads - 1) / kThreads;
-    for (int tile = 0; tile < tiles; ++tile) {
-        const Walk w = make_walk(a, tile);
+    for (int v0 = 0; v0 < a.P; v0 += kThreads) {
+        const Walk w = make_walk(a, v0);
         if (!w.on) continue;
-        const int vec = walk_vec(a, tile);
-        int tail;
-        const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        float k[V], q[V];   // u = k x + q; q is rounded at the size of mean rstd, as mean itself is
+        const int vec = v0 + (a.P <= kThreads ? (int)threadIdx.x % a.P : (int)threadIdx.x);
+        constexpr int H = (V + 1) / 2;
+        Two k[H], q[H];   // u = k x + q; q is rounded at the size of mean rstd, as mean itself is
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float4 c = load_coef(a, b, (vec * V + j) % a.C);
-            k[j] = c.y * c.z;
-            q[j] = fmaf(-c.x, k[j], c.w);
+        for (int i = 0; i < H; ++i) {
+            const float2* c = reinterpret_cast<const float2*>(a.coef) + (int64_t)b * a.C;
+            const float2 c0 = c[channel<V>(a, vec, 2 * i)], c1 = c[channel<V>(a, vec, 2 * i + 1)];
+            k[i] = two(c0.x, c1.x);
+            q[i] = two(c0.y, c1.y);
         }
-        auto value = [&](T v, int j) { return from_f<T>(act_value<ACT>(fmaf(to_f(v), k[j], q[j]))); };
-        int64_t r = r0 + w.lane_row;
-        const T* p = x + r * a.x_row + (int64_t)vec * V;
-        T* o = y + r * a.L + (int64_t)vec * V;
-        const int64_t step = w.rp * a.x_row, ostep = (int64_t)w.rp * a.L;
-        auto write = [&](T* to, const Vec<T, V>& v) {
+        auto value = [&](const Vec<T, V>& v) {
             Vec<T, V> res;
 #pragma unroll
-            for (int j = 0; j < V; ++j) res.v[j] = value(v.v[j], j);
-            *reinterpret_cast<Vec<T, V>*>(to) = res;
+            for (int i = 0; i < H; ++i) res.set(i, act_value<ACT>(fma2(v.pair(i), k[i], q[i])));
+            return res;
         };
-        for (; r + (kUnroll - 1) * w.rp < end; r += kUnroll * w.rp, p += kUnroll * step, o += kUnroll * ostep) {
-            Vec<T, V> v[kUnroll];
+        const int64_t step = w.rp * a.x_row, ostep = (int64_t)w.rp * a.L;
+        for (int tile = chunk + (tiles_of(a, chunk) - 1) * a.chunks; tile >= 0; tile -= a.chunks) {
+            const int64_t row = (int64_t)tile * a.tile_rows + w.lane_row;
+            const T* p = x + row * a.x_row + (int64_t)vec * V;
+            T* o = y + row * a.L + (int64_t)vec * V;
+            if (tile < a.whole_tiles) {
+                Vec<T, V> v[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
+                for (int u = 0; u < kUnroll; ++u) v[u] = load_last<T, V>(p + u * step);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) write(o + u * ostep, v[u]);
+                for (int u = 0; u < kUnroll; ++u) store_last<T, V>(o + u * ostep, value(v[u]));
+            } else {
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int has = valid<V>(a, row + u * w.rp, vec);
+                    if (has == V) store_last<T, V>(o + u * ostep, value(load_last<T, V>(p + u * step)));
+                    else store_some<T, V>(o + u * ostep, value(load_some<T, V>(p + u * step, has)), has);
+                }
+            }
         }
-        for (; r < end; r += w.rp, p += step, o += ostep) write(o, *reinterpret_cast<const Vec<T, V>*>(p));
-        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)   // r == end: the short row
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < tail) o[j] = value(p[j], j);
     }
 }
 
@@ -352,60 +487,69 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Ar
     let_next_start();
     wait_for_previous();
     const int b = a.first + blockIdx.y, chunk = blockIdx.x;
-    const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch;
     const int slots = (a.P <= kThreads ? kThreads / a.P : 1) * a.L;
     float *s_1 = sh, *s_2 = sh + slots;
-    const int tiles = a.P <= kThreads ? 1 : (a.P + kThreads - 1) / kThreads;
-    for (int tile = 0; tile < tiles; ++tile) {
-        const Walk w = make_walk(a, tile);
+    for (int v0 = 0; v0 < a.P; v0 += kThreads) {
+        const Walk w = make_walk(a, v0);
         if (!w.on) continue;
-        const int vec = walk_vec(a, tile);
-        int tail;
-        const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        float mean[V], k[V], q[V], s1[V], s2[V];   // u = k (x - mean) + q; s2 sums du (x - mean)
+        const int vec = v0 + (a.P <= kThreads ? (int)threadIdx.x % a.P : (int)threadIdx.x);
+        constexpr int H = (V + 1) / 2;
+        Two minus[H], k[H], q[H], s1[H], s2[H];   // u = k (x - mean) + q; s2 sums du (x - mean)
+        float rstd[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float4 c = load_coef(a, b, (vec * V + j) % a.C);
-            mean[j] = c.x;
-            k[j] = c.y * c.z;
-            q[j] = c.w;
-            s1[j] = s2[j] = 0.0f;
-        }
-        auto add = [&](T xv, T dv, int j) {
-            const float d = to_f(xv) - mean[j];
-            const float du = to_f(dv) * act_slope<ACT>(fmaf(d, k[j], q[j]));
-            s1[j] += du;
-            s2[j] = fmaf(du, d, s2[j]);
-        };
-        int64_t r = r0 + w.lane_row;
-        const T* p = x + r * a.x_row + (int64_t)vec * V;
-        const T* d = dy + r * a.dy_row + (int64_t)vec * V;
-        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row;
-        for (; r + (kUnroll2 - 1) * w.rp < end; r += kUnroll2 * w.rp, p += kUnroll2 * step, d += kUnroll2 * dstep) {
-            Vec<T, V> v[kUnroll2], g[kUnroll2];
+        for (int i = 0; i < H; ++i) {
+            float2 st[2];
+            float wt[2], bs[2];
 #pragma unroll
-            for (int u = 0; u < kUnroll2; ++u) {
-                v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
-                g[u] = *reinterpret_cast<const Vec<T, V>*>(d + u * dstep);
+            for (int j = 0; j < 2; ++j) {
+                const int ch = channel<V>(a, vec, 2 * i + j);
+                st[j] = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + (int)(((float)ch + 0.5f) * a.per_cpg)];
+                wt[j] = a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f;
+                bs[j] = a.bias ? load_param(a.bias, a.wdtype, ch) : 0.0f;
+                if (2 * i + j < V) rstd[2 * i + j] = st[j].y;
             }
-#pragma unroll
-            for (int u = 0; u < kUnroll2; ++u)
-#pragma unroll
-                for (int j = 0; j < V; ++j) add(v[u].v[j], g[u].v[j], j);
+            minus[i] = two(-st[0].x, -st[1].x);
+            k[i] = two(st[0].y * wt[0], st[1].y * wt[1]);
+            q[i] = two(bs[0], bs[1]);
+            s1[i] = s2[i] = both(0.0f);
         }
-        for (; r < end; r += w.rp, p += step, d += dstep) {
-            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p), g = *reinterpret_cast<const Vec<T, V>*>(d);
+        auto add = [&](const Vec<T, V>& x, const Vec<T, V>& dy) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) add(v.v[j], g.v[j], j);
+            for (int i = 0; i < H; ++i) {
+                const Two d = add2(x.pair(i), minus[i]);
+                const Two du = mul2(dy.pair(i), act_slope<ACT>(fma2(d, k[i], q[i])));
+                s1[i] = add2(s1[i], du);
+                s2[i] = fma2(du, d, s2[i]);
+            }
+        };
+        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row;
+        for (int i = tiles_of(a, chunk), tile = chunk; i > 0; --i, tile += a.chunks) {
+            const int64_t row = (int64_t)tile * a.tile_rows + w.lane_row;
+            const T* p = x + row * a.x_row + (int64_t)vec * V;
+            const T* d = dy + row * a.dy_row + (int64_t)vec * V;
+            if (tile < a.whole_tiles) {
+                Vec<T, V> v[kUnroll2], g[kUnroll2];
+#pragma unroll
+                for (int u = 0; u < kUnroll2; ++u) {
+                    v[u] = load<T, V>(p + u * step);
+                    g[u] = load<T, V>(d + u * dstep);
+                }
+#pragma unroll
+                for (int u = 0; u < kUnroll2; ++u) add(v[u], g[u]);
+            } else {
+                for (int u = 0; u < kUnroll2; ++u) {   // dy of zero behind the image's end
+                    const int has = valid<V>(a, row + u * w.rp, vec);
+                    if (has > 0) add(load_some<T, V>(p + u * step, has), load_some<T, V>(d + u * dstep, has));
+                }
+            }
         }
-        const bool mine = tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row;   // r == end: the short row
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (mine && j < tail) add(p[j], d[j], j);
-            s_1[w.lane_row * a.L + vec * V + j] = s1[j];
-            s_2[w.lane_row * a.L + vec * V + j] = s2[j] * load_coef(a, b, (vec * V + j) % a.C).y;
+            const float2 t1 = split(s1[j / 2]), t2 = split(s2[j / 2]);
+            s_1[w.lane_row * a.L + vec * V + j] = j & 1 ? t1.y : t1.x;
+            s_2[w.lane_row * a.L + vec * V + j] = (j & 1 ? t2.y : t2.x) * rstd[j];
         }
     }
     __syncthreads();
@@ -420,63 +564,69 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Ar
     }
 }
 
-// ---- backward, join: sums of every (image, channel) over the chunks; 16 channels x 64 lanes per CTA ---------------
-__global__ void __launch_bounds__(1024) gn_grad_join_kernel(const Args a) {
-    __shared__ float2 sh[64][16];
+// ---- backward, join: one CTA per (image, group): the sums of its channels over the chunks, the group's means, and the
+// coefficients of the second pass: u = k x + q, dx = k du + kx x + kc ------------------------------------------------
+__global__ void __launch_bounds__(kJoinThreads) gn_grad_join_kernel(const Args a) {
+    __shared__ float2 sh[kJoinThreads];
+    __shared__ float sw[2][kJoinThreads / 32];
     let_next_start();
     wait_for_previous();
-    const int in = threadIdx.x & 15, ch = blockIdx.x * 16 + in, part = threadIdx.x >> 4, b = a.first + blockIdx.y;
-    float2 t = make_float2(0.0f, 0.0f);
-    if (ch < a.C) {
-        const float2* p = reinterpret_cast<const float2*>(a.part) + (int64_t)b * a.chunks * a.C + ch;
+    const int g = blockIdx.x, b = a.first + blockIdx.y, first = g * a.cpg;
+    const int wide = min(a.cpg, kJoinThreads), parts = kJoinThreads / wide;   // channels at once, threads of each
+    const int in = threadIdx.x % wide, part = threadIdx.x / wide;
+    int top = 1;
+    while (top < parts) top <<= 1;
+    float2* sums = reinterpret_cast<float2*>(a.sums) + (int64_t)b * a.C + first;
+    float m1 = 0.0f, m2 = 0.0f;
+    for (int c0 = 0; c0 < a.cpg; c0 += wide) {
+        const int i = c0 + in;
+        float2 t = make_float2(0.0f, 0.0f);
+        if (i < a.cpg && part < parts) {
+            const float2* p = reinterpret_cast<const float2*>(a.part) + (int64_t)b * a.chunks * a.C + first + i;
 #pragma unroll 4
-        for (int k = part; k < a.chunks; k += 64) {
-            const float2 v = p[(int64_t)k * a.C];
-            t.x += v.x;
-            t.y += v.y;
+            for (int k = part; k < a.chunks; k += parts) {
+                const float2 v = p[(int64_t)k * a.C];
+                t.x += v.x;
+                t.y += v.y;
+            }
         }
-    }
-    sh[part][in] = t;
-    __syncthreads();
-#pragma unroll
-    for (int half = 32; half > 0; half >>= 1) {
-        if (part < half) {
-            sh[part][in].x += sh[part + half][in].x;
-            sh[part][in].y += sh[part + half][in].y;
+        sh[threadIdx.x] = t;
+        __syncthreads();
+        for (int half = top >> 1; half > 0; half >>= 1) {
+            if (part < half && part + half < parts) {
+                sh[threadIdx.x].x += sh[threadIdx.x + half * wide].x;
+                sh[threadIdx.x].y += sh[threadIdx.x + half * wide].y;
+            }
+            __syncthreads();
+        }
+        if (part == 0 && i < a.cpg) {
+            t = sh[threadIdx.x];
+            sums[i] = t;
+            const float w = a.weight ? load_param(a.weight, a.wdtype, first + i) : 1.0f;
+            m1 = fmaf(w, t.x, m1);
+            m2 = fmaf(w, t.y, m2);
         }
         __syncthreads();
     }
-    if (part == 0 && ch < a.C) reinterpret_cast<float2*>(a.sums)[(int64_t)b * a.C + ch] = sh[0][in];
+    const float inv = 1.0f / ((float)a.elems * a.share);
+    m1 = cta_sum(m1, sw[0]) * inv;
+    m2 = cta_sum(m2, sw[1]) * inv;
+    const float2 st = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + g];
+    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads) {
+        const float k = st.y * (a.weight ? load_param(a.weight, a.wdtype, first + i) : 1.0f);
+        const float kx = -st.y * st.y * m2;
+        reinterpret_cast<float4*>(a.coef)[(int64_t)b * a.C + first + i] =
+            make_float4(k, fmaf(-st.x, k, a.bias ? load_param(a.bias, a.wdtype, first + i) : 0.0f), kx, fmaf(-st.x, kx, -st.y * m1));
+    }
 }
 
 // ---- backward, pass 2: dx, and (last turn) the parameter gradients ------------------------------------------------
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const Args a, int params) {
-    extern __shared__ float sh[];   // [G][2] group means of w du and w du xhat
     let_next_start();
     wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = a.chunks - 1 - blockIdx.x;
+    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
     const float2* sums = reinterpret_cast<const float2*>(a.sums);
-    const float inv = 1.0f / (float)(a.elems / a.C * a.cpg);
-    for (int g = threadIdx.x >> 5; g < a.G; g += kThreads / 32) {
-        float m1 = 0.0f, m2 = 0.0f;
-        for (int i = threadIdx.x & 31; i < a.cpg; i += 32) {
-            const int ch = g * a.cpg + i;
-            const float2 s = sums[(int64_t)b * a.C + ch];
-            const float w = a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f;
-            m1 = fmaf(w, s.x, m1);
-            m2 = fmaf(w, s.y, m2);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            m1 += __shfl_xor_sync(~0u, m1, o);
-            m2 += __shfl_xor_sync(~0u, m2, o);
-        }
-        if ((threadIdx.x & 31) == 0) {
-            sh[g * 2] = m1 * inv;
-            sh[g * 2 + 1] = m2 * inv;
-        }
-    }
     if (params && blockIdx.y == 0)   // every CTA of one image takes a share of the channels
         for (int ch = blockIdx.x * kThreads + threadIdx.x; ch < a.C; ch += gridDim.x * kThreads) {
             float t1 = 0.0f, t2 = 0.0f;
@@ -488,61 +638,57 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const A
             if (a.dweight) store_param(a.dweight, a.wdtype, ch, t2);
             if (a.dbias) store_param(a.dbias, a.wdtype, ch, t1);
         }
-    __syncthreads();
     if (!a.y) return;
-    const int64_t r0 = chunk * a.chunk_rows, r1 = min(a.rows, r0 + a.chunk_rows);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch;
     T* dx = static_cast<T*>(a.y) + b * a.y_batch;
-    const int tiles = a.P <= kThreads ? 1 : (a.P + kThreads - 1) / kThreads;
-    for (int tile = 0; tile < tiles; ++tile) {
-        const Walk w = make_walk(a, tile);
+    for (int v0 = 0; v0 < a.P; v0 += kThreads) {
+        const Walk w = make_walk(a, v0);
         if (!w.on) continue;
-        const int vec = walk_vec(a, tile);
-        int tail;
-        const int64_t end = whole_rows<V>(a, r1, vec, tail);
-        float k[V], q[V], kx[V], kc[V];   // u = k x + q, dx = k du + kx x + kc
+        const int vec = v0 + (a.P <= kThreads ? (int)threadIdx.x % a.P : (int)threadIdx.x);
+        constexpr int H = (V + 1) / 2;
+        Two k[H], q[H], kx[H], kc[H];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int ch = (vec * V + j) % a.C;
-            const float4 c = load_coef(a, b, ch);
-            const float m1 = sh[ch / a.cpg * 2], m2 = sh[ch / a.cpg * 2 + 1];
-            k[j] = c.y * c.z;
-            q[j] = fmaf(-c.x, k[j], c.w);
-            kx[j] = -c.y * c.y * m2;
-            kc[j] = fmaf(-c.x, kx[j], -c.y * m1);
+        for (int i = 0; i < H; ++i) {
+            const float4* c = reinterpret_cast<const float4*>(a.coef) + (int64_t)b * a.C;
+            const float4 c0 = c[channel<V>(a, vec, 2 * i)], c1 = c[channel<V>(a, vec, 2 * i + 1)];
+            k[i] = two(c0.x, c1.x);
+            q[i] = two(c0.y, c1.y);
+            kx[i] = two(c0.z, c1.z);
+            kc[i] = two(c0.w, c1.w);
         }
-        auto value = [&](T xv, T dv, int j) {
-            const float x = to_f(xv), du = to_f(dv) * act_slope<ACT>(fmaf(x, k[j], q[j]));
-            return from_f<T>(fmaf(k[j], du, fmaf(kx[j], x, kc[j])));
-        };
-        int64_t r = r0 + w.lane_row;
-        const T* p = x + r * a.x_row + (int64_t)vec * V;
-        const T* d = dy + r * a.dy_row + (int64_t)vec * V;
-        T* o = dx + r * a.L + (int64_t)vec * V;
-        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row, ostep = (int64_t)w.rp * a.L;
-        auto write = [&](T* to, const Vec<T, V>& v, const Vec<T, V>& g) {
+        auto value = [&](const Vec<T, V>& x, const Vec<T, V>& dy) {
             Vec<T, V> res;
 #pragma unroll
-            for (int j = 0; j < V; ++j) res.v[j] = value(v.v[j], g.v[j], j);
-            *reinterpret_cast<Vec<T, V>*>(to) = res;
-        };
-        for (; r + (kUnroll2 - 1) * w.rp < end; r += kUnroll2 * w.rp, p += kUnroll2 * step, d += kUnroll2 * dstep, o += kUnroll2 * ostep) {
-            Vec<T, V> v[kUnroll2], g[kUnroll2];
-#pragma unroll
-            for (int u = 0; u < kUnroll2; ++u) {
-                v[u] = *reinterpret_cast<const Vec<T, V>*>(p + u * step);
-                g[u] = *reinterpret_cast<const Vec<T, V>*>(d + u * dstep);
+            for (int i = 0; i < H; ++i) {
+                const Two v = x.pair(i), du = mul2(dy.pair(i), act_slope<ACT>(fma2(v, k[i], q[i])));
+                res.set(i, fma2(k[i], du, fma2(kx[i], v, kc[i])));
             }
+            return res;
+        };
+        const int64_t step = w.rp * a.x_row, dstep = w.rp * a.dy_row, ostep = (int64_t)w.rp * a.L;
+        for (int tile = chunk + (tiles_of(a, chunk) - 1) * a.chunks; tile >= 0; tile -= a.chunks) {
+            const int64_t row = (int64_t)tile * a.tile_rows + w.lane_row;
+            const T* p = x + row * a.x_row + (int64_t)vec * V;
+            const T* d = dy + row * a.dy_row + (int64_t)vec * V;
+            T* o = dx + row * a.L + (int64_t)vec * V;
+            if (tile < a.whole_tiles) {
+                Vec<T, V> v[kUnroll2], g[kUnroll2];
 #pragma unroll
-            for (int u = 0; u < kUnroll2; ++u) write(o + u * ostep, v[u], g[u]);
+                for (int u = 0; u < kUnroll2; ++u) {
+                    v[u] = load_last<T, V>(p + u * step);
+                    g[u] = load_last<T, V>(d + u * dstep);
+                }
+#pragma unroll
+                for (int u = 0; u < kUnroll2; ++u) store_last<T, V>(o + u * ostep, value(v[u], g[u]));
+            } else {
+                for (int u = 0; u < kUnroll2; ++u) {
+                    const int has = valid<V>(a, row + u * w.rp, vec);
+                    if (has > 0)
+                        store_some<T, V>(o + u * ostep, value(load_some<T, V>(p + u * step, has), load_some<T, V>(d + u * dstep, has)), has);
+                }
+            }
         }
-        for (; r < end; r += w.rp, p += step, d += dstep, o += ostep)
-            write(o, *reinterpret_cast<const Vec<T, V>*>(p), *reinterpret_cast<const Vec<T, V>*>(d));
-        if (tail > 0 && end >= r0 && (end - r0) % w.rp == w.lane_row)   // r == end: the short row
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < tail) o[j] = value(p[j], d[j], j);
     }
 }
 
@@ -583,13 +729,10 @@ int images_per_turn(const D3gsGroupNorm& d, bool backward) {
     return (int)(n < 1 ? 1 : n);
 }
 
-// Chunks of one image: as many CTAs in a turn as run at once, none with less than two vectors a thread.
+// Chunks of one image: as many CTAs in a turn as run at once (a CTA without a tile is not launched).
 int chunks_of(const D3gsGroupNorm& d, bool backward) {
-    const int turn = images_per_turn(d, backward);
-    const int64_t want = div_up64((backward ? kCtas2 : kCtas) * 148, turn), values = d.pixels * d.channels;
-    const int64_t most = div_up64(values, (int64_t)kThreads * (16 / elem_size(d.dtype)) * 2);
-    int64_t n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > kMaxChunks ? kMaxChunks : n);
+    const int64_t n = div_up64((backward ? kCtas2 : kCtas) * 148, images_per_turn(d, backward));
+    return (int)(n > kMaxChunks ? kMaxChunks : n);
 }
 
 int32_t check(const D3gsGroupNorm* d, const char* what) {
@@ -599,7 +742,7 @@ int32_t check(const D3gsGroupNorm* d, const char* what) {
     D3GS_REQUIRE(d->channels >= 1 && d->channels <= kMaxChannels, "%s: %d channels (1 to %d)", what, d->channels, kMaxChannels);
     D3GS_REQUIRE(d->groups >= 1 && d->channels % d->groups == 0, "%s: %d groups do not divide %d channels", what, d->groups,
                  d->channels);
-    D3GS_REQUIRE(d->pixels <= (int64_t)1 << 40, "%s: image too large", what);
+    D3GS_REQUIRE(d->pixels < (int64_t)1 << 31, "%s: image too large", what);
     D3GS_REQUIRE(d->dtype >= 0 && d->dtype <= 2 && d->weight_dtype >= 0 && d->weight_dtype <= 2, "%s: dtype %d / %d", what,
                  d->dtype, d->weight_dtype);
     D3GS_REQUIRE(d->act >= 0 && d->act <= 2, "%s: act %d", what, d->act);
@@ -608,15 +751,15 @@ int32_t check(const D3gsGroupNorm* d, const char* what) {
 }
 
 struct Workspace {
-    size_t part, sums, bytes;   // offsets, total
+    size_t sums, coef, bytes;   // offsets (the partial sums come first), total
 };
 Workspace workspace_of(const D3gsGroupNorm& d, bool backward) {
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Workspace w;
-    const size_t chunks = chunks_of(d, backward);
-    w.part = 0;
-    const size_t n = (size_t)d.batch * chunks * (backward ? d.channels : d.groups) * 8;
-    w.sums = (n + 255) / 256 * 256;
-    w.bytes = w.sums + (backward ? (size_t)d.batch * d.channels * 8 : 0) + 256;
+    const size_t chunks = chunks_of(d, backward), channels = (size_t)d.batch * d.channels;
+    w.sums = up((size_t)d.batch * chunks * (backward ? d.channels : d.groups) * 8);
+    w.coef = w.sums + (backward ? up(channels * 8) : 0);
+    w.bytes = w.coef + up(channels * (backward ? 16 : 8)) + 256;
     return w;
 }
 
@@ -631,8 +774,10 @@ Args make_args(const D3gsGroupNorm& d, int v, bool backward, void* ws) {
     a.L = a.P * v;
     a.rows = div_up64(a.elems, a.L);
     a.chunks = chunks_of(d, backward);
-    a.chunk_rows = div_up64(a.rows, a.chunks);
-    a.chunks = (int)div_up64(a.rows, a.chunk_rows);    // no empty chunk
+    a.tile_rows = (a.P <= kThreads ? kThreads / a.P : 1) * (backward ? kUnroll2 : kUnroll);
+    a.tiles = (int)div_up64(a.rows, a.tile_rows);
+    a.whole_tiles = (int)(a.elems / ((int64_t)a.tile_rows * a.L));
+    if (a.chunks > a.tiles) a.chunks = a.tiles;        // no empty chunk
     a.x_batch = d.x_batch_stride;
     a.dy_batch = d.dy_batch_stride;
     a.x_row = a.L == a.C ? d.x_pixel_stride : a.L;
@@ -642,7 +787,10 @@ Args make_args(const D3gsGroupNorm& d, int v, bool backward, void* ws) {
     a.wdtype = d.weight_dtype;
     a.act = d.act;
     a.eps = d.eps;
-    a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);
+    a.share = 1.0f / d.groups;
+    a.per_cpg = 1.0f / a.cpg;
+    a.part = static_cast<float*>(ws);
+    a.coef = reinterpret_cast<float*>(static_cast<char*>(ws) + w.coef);
     a.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + w.sums);
     return a;
 }
@@ -689,9 +837,9 @@ int32_t run_backward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
         a.first = b;
         const dim3 grid(a.chunks, images);
         if (int32_t rc = launch(gn_grad_sums_kernel<T, V, ACT>, "gn_grad_sums_kernel", grid, kThreads, slots * 8, st, a)) return rc;
-        if (int32_t rc = launch(gn_grad_join_kernel, "gn_grad_join_kernel", dim3((a.C + 15) / 16, images), 1024, 0, st, a)) return rc;
+        if (int32_t rc = launch(gn_grad_join_kernel, "gn_grad_join_kernel", dim3(a.G, images), kJoinThreads, 0, st, a)) return rc;
         const int params = b + images == a.batch && (a.dweight || a.dbias);
-        if (int32_t rc = launch(gn_grad_apply_kernel<T, V, ACT>, "gn_grad_apply_kernel", grid, kThreads, (size_t)a.G * 8, st, a, params))
+        if (int32_t rc = launch(gn_grad_apply_kernel<T, V, ACT>, "gn_grad_apply_kernel", grid, kThreads, 0, st, a, params))
             return rc;
     }
     return D3GS_OK;

@@ -193,6 +193,18 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
     for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(s)[i];
 }
 
+// value i of the result: stored, or taken from the parameter
+__device__ __forceinline__ void write_result(const Table& t, const Matrix& m, int64_t i, float v) {
+    if (m.momentum) {
+        float* p = static_cast<float*>(m.dst) + i;
+        *p = fmaf(-m.rate, v, t.decay * *p);
+    } else if (t.bf16) {
+        static_cast<__nv_bfloat16*>(m.dst)[i] = __float2bfloat16_rn(v);
+    } else {
+        static_cast<float*>(m.dst)[i] = v;
+    }
+}
+
 // ---- last pass: result or parameter from the blocks of X; one CTA per block ---------------------------------------
 __global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constant__ Table t) {
     wait_for_previous();
@@ -213,14 +225,7 @@ __global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constan
             const int64_t j = tall ? xc * m.cols + xr : xr * m.cols + xc;
             float v = (k ? hi.y + lo.y : hi.x + lo.x) * t.out_scale;
             if (failed) v = __int_as_float(0x7fffffff);
-            if (m.momentum) {
-                float* p = static_cast<float*>(m.dst) + j;
-                *p = fmaf(-m.rate, v, t.decay * *p);
-            } else if (t.bf16) {
-                static_cast<__nv_bfloat16*>(m.dst)[j] = __float2bfloat16_rn(v);
-            } else {
-                static_cast<float*>(m.dst)[j] = v;
-            }
+            write_result(t, m, j, v);
         }
     }
 }
@@ -374,10 +379,10 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // One 16-byte piece of a result: eight columns of a row, from sums to planes; `diagonal`: which of them takes the shift.
-__device__ __forceinline__ void finish(const Table& t, const float* v, int diagonal, uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ void finish(const float* v, float scale, float shift, int diagonal, uint32_t* hi, uint32_t* lo) {
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = fmaf(v[i], t.out_scale, i == diagonal ? t.shift : 0.0f);
+    for (int i = 0; i < 8; ++i) f[i] = fmaf(v[i], scale, i == diagonal ? shift : 0.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) split2(f[2 * i], f[2 * i + 1], hi[i], lo[i]);
 }
@@ -400,6 +405,249 @@ template <bool TWO> __device__ __forceinline__ void write_mirrored(char* block, 
             const uint32_t l = __shfl_xor_sync(~0u, lo[i], 1);
             *reinterpret_cast<uint32_t*>(block + kPlane + o) = odd ? __byte_perm(l, lo[i], 0x7632) : __byte_perm(lo[i], l, 0x5410);
         }
+    }
+}
+
+// ---- tiny matrices: the whole chain in one CTA --------------------------------------------------------------------
+// A short side of one tile and a long side of four column blocks: X (128 KB at most) and A or B (64 KB) stay in shared
+// memory from the first step to the last, and a matrix costs one launch instead of seventeen.  What takes time is the way
+// from a product to its epilogue and back, three of each a step.  Sums of hi hi are taken out after every two blocks.
+// B = a I + b A + c A A here, A read back by the thread that wrote it.
+constexpr int kTinyThreads = 288, kTinyCols = 4 * kCols;   // eight warps for the sums, one that issues
+
+// the scalars of every step, in the products' scales (see scales_of)
+struct Steps {
+    float gram[D3GS_NS_MAX_STEPS], gram_shift[D3GS_NS_MAX_STEPS], square[D3GS_NS_MAX_STEPS], square_shift[D3GS_NS_MAX_STEPS],
+        linear[D3GS_NS_MAX_STEPS], apply[D3GS_NS_MAX_STEPS];
+    float first, last;    // scale of X at the start, one over that at the end
+    uint32_t cubic;       // a bit for each step with c = 0
+    int32_t count;
+};
+
+__global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_constant__ Table t, const __grid_constant__ Steps sp) {
+    constexpr uint32_t kBlock = 2 * kPlane;
+    extern __shared__ char raw[];
+    __shared__ uint64_t s_done, s_end;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    __shared__ double s_norm[kTinyThreads / 32];
+    char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Matrix& m = t.mat[blockIdx.x];
+    const int nk = m.nk, mk = m.mk;
+    char* const x = smem;                        // nk blocks
+    char* const ab = smem + nk * (int)kBlock;    // mk blocks: A, then B
+    const uint32_t columns = nk > 2 ? 512 : 256;
+    if (tid == 0) {
+        mbar_init(&s_done, 1);
+        mbar_init(&s_end, 1);
+        s_failed = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) tmem_alloc<1>(&s_tmem, columns);
+    for (int i = tid; i < nk * (int)kBlock / 16; i += kTinyThreads) reinterpret_cast<uint4*>(x)[i] = make_uint4(0, 0, 0, 0);
+    let_next_start();
+    wait_for_previous();
+
+    // ---- momentum, norm, X ----
+    const int count = m.rows * m.cols;
+    const bool tall = m.rows > m.cols;
+    double sum = 0.0;
+#pragma unroll 8
+    for (int i = tid; i < count; i += kTinyThreads) {
+        const int r = i / m.cols, c = i - r * m.cols;
+        float u = load_src(t, m, r, c);
+        if (m.momentum) {
+            const float buf = fmaf(t.mu, m.momentum[i], (1.0f - t.mu) * u);
+            m.momentum[i] = buf;
+            u = update_of(t, u, buf);
+        }
+        sum += (double)u * (double)u;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) s_norm[warp] = sum;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    sum = 0.0;
+    for (int k = 0; k < kTinyThreads / 32; ++k) sum += s_norm[k];
+    const double norm = sqrt(sum);
+    const float scale = (float)(1.0 / (norm < (double)t.eps ? (double)t.eps : norm)) * sp.first;   // a NaN stays one
+#pragma unroll 8
+    for (int i = tid; i < count; i += kTinyThreads) {   // (a thread reads the momentum that it wrote)
+        const int r = i / m.cols, c = i - r * m.cols;
+        float u = load_src(t, m, r, c);
+        if (m.momentum) u = update_of(t, u, m.momentum[i]);
+        u *= scale;
+        const int xr = tall ? c : r, xc = tall ? r : c;
+        char* const to = x + (xc / kCols) * (int)kBlock + block_offset(xr, xc % kCols);
+        const __half h = __float2half_rn(u);
+        *reinterpret_cast<__half*>(to) = h;
+        *reinterpret_cast<__half*>(to + kPlane) = __float2half_rn(u - __half2float(h));
+    }
+
+    // ---- products ----
+    const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
+    const int half = (warp >> 2) & 1, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const int tiles = (nk + 1) / 2;              // of B X: 128 columns each
+    const uint32_t rest = tmem + (nk > 2 ? 256 : 128);   // Gram: sums of hi lo + lo hi
+    bool ok = true;
+    uint32_t phase = 0;
+    auto next_phase = [&]() {   // what was written to shared memory is there for the products, TMEM is free
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    };
+    auto issue = [&](uint32_t sum_at, uint32_t rest_at, uint32_t a, uint32_t b, uint32_t step, uint32_t idesc, bool new_sum, bool new_rest) {
+#pragma unroll
+        for (int q = 0; q < kCols / 16; ++q) {
+            const uint64_t ah = operand(a + q * 2), al = operand(a + kPlane / 16 + q * 2);
+            const uint64_t bh = operand(b + q * step), bl = operand(b + kPlane / 16 + q * step);
+            tc_mma<1>(sum_at, ah, bh, idesc, !new_sum || q != 0);
+            tc_mma<1>(rest_at, ah, bl, idesc, !new_rest || q != 0);
+            tc_mma<1>(rest_at, al, bh, idesc, true);
+        }
+    };
+    auto wait_done = [&]() {
+        if (ok) ok = __all_sync(~0u, wait_for(&s_done, phase & 1, polls));
+        if (!ok) s_failed = 1;
+        tc_fence_after();
+    };
+    const uint32_t x0 = operand_low(smem_u32(x), 16), x0_across = operand_low(smem_u32(x), kBlock), ab0 = operand_low(smem_u32(ab), 16);
+    for (int step = 0; step < sp.count; ++step) {
+        const bool cubic = sp.cubic >> step & 1;
+        next_phase();   // A = X X^T
+        if (warp == 8) {
+            if (lane == 0 && !(t.hooks.hold == (int)blockIdx.x && phase == 0)) {   // (a test: these products never come)
+                for (int k = 0; k < nk; ++k) {
+                    const uint32_t b = x0 + k * (kBlock / 16);
+                    issue(tmem + (k >> 1) * 128, rest, b, b, 2, instruction(false, 128, 128), (k & 1) == 0, k == 0);
+                }
+                tc_commit<1>(&s_done);
+            }
+        } else {
+            wait_done();
+            if (half < mk) {
+                float v[64];
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    float w[32];
+                    tmem_load32(tmem + half * 64 + c + lanes, w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[c + i] = w[i];
+                    if (nk > 2) {
+                        tmem_load32(tmem + 128 + half * 64 + c + lanes, w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[c + i] += w[i];
+                    }
+                    tmem_load32(rest + half * 64 + c + lanes, w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[c + i] += w[i];
+                }
+                const int on = row < m.m && cubic ? row - half * 64 : -1;
+#pragma unroll
+                for (int c = 0; c < 64; c += 8) {
+                    uint32_t hi[4], lo[4];
+                    finish(v + c, sp.gram[step], sp.gram_shift[step], on - c, hi, lo);
+                    put<true>(ab + half * (int)kBlock + block_offset(row, c), hi, lo);
+                }
+            }
+        }
+        ++phase;
+        if (!cubic) {
+            next_phase();   // B = a I + b A + c A A
+            if (warp == 8) {
+                if (lane == 0) {
+                    for (int k = 0; k < mk; ++k) {
+                        const uint32_t b = ab0 + k * (kBlock / 16);
+                        issue(tmem, tmem + 128, b, b, 2, instruction(false, 128, 128), k == 0, k == 0);
+                    }
+                    tc_commit<1>(&s_done);
+                }
+            } else {
+                wait_done();
+                if (half < mk) {
+                    float v[64];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        float w[32];
+                        tmem_load32(tmem + half * 64 + c + lanes, w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[c + i] = w[i];
+                        tmem_load32(tmem + 128 + half * 64 + c + lanes, w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[c + i] += w[i];
+                    }
+                    const int on = row < m.m ? row - half * 64 : -1;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 8) {
+                        char* const at = ab + half * (int)kBlock + block_offset(row, c);
+                        const uint4 h = *reinterpret_cast<const uint4*>(at), l = *reinterpret_cast<const uint4*>(at + kPlane);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
+                            const float2 g = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
+                            v[c + 2 * i] = fmaf(v[c + 2 * i], sp.square[step], (f.x + g.x) * sp.linear[step]);
+                            v[c + 2 * i + 1] = fmaf(v[c + 2 * i + 1], sp.square[step], (f.y + g.y) * sp.linear[step]);
+                        }
+                        uint32_t hi[4], lo[4];
+                        finish(v + c, 1.0f, sp.square_shift[step], on - c, hi, lo);
+                        put<true>(at, hi, lo);
+                    }
+                }
+            }
+            ++phase;
+        }
+        next_phase();   // X <- B X, a tile of 128 columns for each half of the warps
+        if (warp == 8) {
+            if (lane == 0) {
+                for (int w = 0; w < tiles; ++w)
+                    for (int k = 0; k < mk; ++k)   // (columns behind X's last block take what lies there, and are not kept)
+                        issue(tmem + w * 256, tmem + w * 256 + 128, ab0 + k * (kBlock / 16),
+                              x0_across + (w * 2 * kBlock + k * (kPlane / 2)) / 16, 2048 / 16, instruction(true, 128, 128), k == 0, k == 0);
+                tc_commit<1>(&s_done);
+            }
+        } else {
+            wait_done();
+            if (half < tiles) {
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    if (2 * half + c / kCols >= nk) continue;
+                    float v[32], w[32];
+                    tmem_load32(tmem + half * 256 + c + lanes, v);
+                    tmem_load32(tmem + half * 256 + 128 + c + lanes, w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] += w[i];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t hi[4], lo[4];
+                        finish(v + i, sp.apply[step], 0.0f, -1, hi, lo);
+                        put<true>(x + (2 * half + c / kCols) * (int)kBlock + block_offset(row, (c + i) % kCols), hi, lo);
+                    }
+                }
+            }
+        }
+        ++phase;
+    }
+    if (warp == 8 && lane == 0) {   // whatever was issued has ended before TMEM is handed back
+        tc_commit<1>(&s_end);
+        wait_for(&s_end, 0);
+    }
+    next_phase();
+    if (warp == 8) tmem_free<1>(tmem, columns);
+
+    // ---- result ----
+    const bool failed = s_failed != 0;
+#pragma unroll 4
+    for (int i = tid; i < count; i += kTinyThreads) {
+        const int r = i / m.cols, c = i - r * m.cols, xr = tall ? c : r, xc = tall ? r : c;
+        const char* const at = x + (xc / kCols) * (int)kBlock + block_offset(xr, xc % kCols);
+        float v = (__half2float(*reinterpret_cast<const __half*>(at)) + __half2float(*reinterpret_cast<const __half*>(at + kPlane))) * sp.last;
+        if (failed) v = __int_as_float(0x7fffffff);
+        write_result(t, m, i, v);
     }
 }
 
@@ -569,11 +817,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             char* const to = out + ((int64_t)ti * wide + 2 * tj + c / kCols) * kBlock + block_offset(r, c % kCols);
             uint32_t hi[4], lo[4];
             const int on = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;   // diagonal
-            finish(t, w, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+            finish(w, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
             put<true>(to, hi, lo);
             if (MODE == kGram && same && !t.cubic) {
                 uint32_t vh[4], vl[4];
-                finish(t, w, on, vh, vl);
+                finish(w, t.out_scale, t.shift, on, vh, vl);
                 put<true>(m.v + (int64_t)(2 * ti + c / kCols) * kBlock + block_offset(r, c % kCols), vh, vl);
             }
             if (MODE != kApply && !same)   // the mirrored tile: this thread's row is a column
@@ -839,10 +1087,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 const uint32_t o = block_offset(r, c % kCols);
                 uint32_t hi[4], lo[4];
                 const int in = row * kRows + (int)r, on = in < m.m ? in - (col * kCols + c) : -1;   // diagonal
-                finish(t, v + c, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+                finish(v + c, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
                 put<P::kOut == 2>(space + (c / kCols) * kOutBytes + o, hi, lo);
                 if (MODE == kGram && keeps_v) {
-                    finish(t, v + c, on, hi, lo);
+                    finish(v + c, t.out_scale, t.shift, on, hi, lo);
                     put<P::kOut == 2>((N == 256 ? space + kMine : smem + (2 + half) * kMine) + (c / kCols) * kOutBytes + o, hi, lo);
                 }
                 if (MODE != kApply && mirrored) {
@@ -931,6 +1179,13 @@ bool large(const D3gsOrthoMatrix* mats, int32_t count) {
         if ((mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols) > kPairFrom && mats[i].rows > 0 && mats[i].cols > 0) return true;
     return false;
 }
+// One CTA a matrix when all of them are that small.  (A list with one larger matrix goes the other way as a whole: the
+// small ones run beside it there, and cost nothing.)
+bool tiny(const D3gsOrthoMatrix* mats, int32_t count) {
+    for (int32_t i = 0; i < count; ++i)
+        if (min(mats[i].rows, mats[i].cols) > kRows || max(mats[i].rows, mats[i].cols) > kTinyCols) return false;
+    return true;
+}
 // Planes of A and B.  Small matrices take two for 16-bit types too: with them it is not the products that take time, and
 // one plane would cost an 8 x 8 matrix up to twice the error of its own rounding.
 int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
@@ -1009,9 +1264,9 @@ int32_t check(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     return D3GS_OK;
 }
 
-template <typename K>
+template <typename K, typename... A>
 int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
-               const Table& t) {
+               const A&... args) {
     if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(grid);
@@ -1026,7 +1281,7 @@ int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     c.attrs = attr;
     c.numAttrs = 2;
-    D3GS_CUDA(cudaLaunchKernelEx(&c, kernel, t));
+    D3GS_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
     D3GS_LAUNCH_CHECK(name);
     return D3GS_OK;
 }
@@ -1068,47 +1323,76 @@ template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table
     else return pair_product<false, MODE, 1>(t, blocks, st);
 }
 
-template <bool F32, bool PAIR>
-int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg, bool muon, const Scales& sc, void* ws,
-            cudaStream_t st) {
-    char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
-    Table t{};
-    t.fail = reinterpret_cast<uint32_t*>(at);
-    at += 256;
-    t.bf16 = cfg.dtype == D3GS_DTYPE_BF16;
-    t.eps = cfg.eps;
-    t.mu = cfg.momentum;
-    t.nesterov = cfg.nesterov;
-    t.decay = cfg.decay;
-    t.hooks = test_hooks();
-    int32_t i = 0;
-    while (i < count) {
-        t.count = 0;
-        for (; i < count && t.count < kMaxMatrices; ++i) {
-            const D3gsOrthoMatrix& d = mats[i];
-            if (d.rows == 0 || d.cols == 0) continue;
-            const Parts p = parts_of(d, F32 ? 2 : 1);
-            Matrix& m = t.mat[t.count++];
-            m.src = d.src;
-            m.momentum = muon ? d.momentum : nullptr;
-            m.dst = d.dst;
-            m.src_stride = d.src_row_stride;
-            m.rows = (int32_t)d.rows;
-            m.cols = (int32_t)d.cols;
-            m.m = p.m;
-            m.n = p.n;
-            m.mb = p.mb;
-            m.mk = p.mk;
-            m.nk = p.nk;
-            m.rate = d.rate;
-            m.x[0] = at;
-            m.x[1] = at + p.x;
-            m.a = at + 2 * p.x;
-            m.b = at + 2 * p.x + p.a;
-            m.v = at + 2 * p.x + 2 * p.a;
-            m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a + p.v);
-            at += p.total;
+// Fills the table with as many matrices as it takes, from number i on, and gives them their workspace.
+void next_table(Table& t, const D3gsOrthoMatrix* mats, int32_t count, int32_t& i, bool muon, int planes, char*& at) {
+    t.count = 0;
+    for (; i < count && t.count < kMaxMatrices; ++i) {
+        const D3gsOrthoMatrix& d = mats[i];
+        if (d.rows == 0 || d.cols == 0) continue;
+        const Parts p = parts_of(d, planes);
+        Matrix& m = t.mat[t.count++];
+        m.src = d.src;
+        m.momentum = muon ? d.momentum : nullptr;
+        m.dst = d.dst;
+        m.src_stride = d.src_row_stride;
+        m.rows = (int32_t)d.rows;
+        m.cols = (int32_t)d.cols;
+        m.m = p.m;
+        m.n = p.n;
+        m.mb = p.mb;
+        m.mk = p.mk;
+        m.nk = p.nk;
+        m.rate = d.rate;
+        m.x[0] = at;
+        m.x[1] = at + p.x;
+        m.a = at + 2 * p.x;
+        m.b = at + 2 * p.x + p.a;
+        m.v = at + 2 * p.x + 2 * p.a;
+        m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a + p.v);
+        at += p.total;
+    }
+}
+
+Steps steps_of(const D3gsOrthoConfig& cfg, const Scales& sc) {
+    Steps sp{};
+    sp.count = cfg.steps;
+    sp.first = sc.x[0];
+    sp.last = 1.0f / sc.x[cfg.steps];
+    for (int s = 0; s < cfg.steps; ++s) {
+        const double a = cfg.coefficients[s][0], b = cfg.coefficients[s][1], c = cfg.coefficients[s][2];
+        const double sx = sc.x[s], sv = sc.v[s], sb = sc.b[s];
+        if (c == 0.0) {   // the Gram product gives B
+            sp.cubic |= 1u << s;
+            sp.gram[s] = (float)(b * (sb / (sx * sx)));
+            sp.gram_shift[s] = (float)(a * sb);
+        } else {
+            sp.gram[s] = (float)(sv / (sx * sx));
+            sp.gram_shift[s] = (float)(b / c * sv);
+            sp.square[s] = (float)(c * (sb / (sv * sv)));
+            sp.square_shift[s] = (float)(a * sb);
+            sp.linear[s] = (float)(b * (sb / sv));
         }
+        sp.apply[s] = sc.x[s + 1] / sc.b[s] / sc.x[s];
+    }
+    return sp;
+}
+
+// Matrices of one tile and four column blocks: one launch, a CTA each.
+int32_t run_tiny(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t count, bool muon, char* at, cudaStream_t st) {
+    for (int32_t i = 0; i < count;) {
+        next_table(t, mats, count, i, muon, 2, at);
+        if (t.count == 0) break;
+        int blocks = 0;
+        for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + t.mat[k].mk);
+        if (int32_t rc = launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st, t, sp)) return rc;
+    }
+    return D3GS_OK;
+}
+
+template <bool F32, bool PAIR>
+int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t count, bool muon, char* at, cudaStream_t st) {
+    for (int32_t i = 0; i < count;) {
+        next_table(t, mats, count, i, muon, F32 ? 2 : 1, at);
         if (t.count == 0) break;
         auto blocks = [&](auto per) {
             int64_t b = 0;
@@ -1123,27 +1407,25 @@ int32_t run(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& c
         t.from = 0;
         unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * m.cols, kNormChunk); });
         if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, t)) return rc;
-        t.out_scale = sc.x[0];
+        t.out_scale = sp.first;
         grid = blocks(every_block);
         if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, t)) return rc;
-        for (int s = 0; s < cfg.steps; ++s) {
-            const bool last = s == cfg.steps - 1;
-            const double a = cfg.coefficients[s][0], b = cfg.coefficients[s][1], c = cfg.coefficients[s][2];
-            const double sx = sc.x[s], sv = sc.v[s], sb = sc.b[s];
-            t.cubic = c == 0.0;
-            t.out_scale = (float)(t.cubic ? b * (sb / (sx * sx)) : sv / (sx * sx));
-            t.shift = (float)(t.cubic ? a * sb : b / c * sv);
+        for (int s = 0; s < sp.count; ++s) {
+            const bool last = s == sp.count - 1;
+            t.cubic = sp.cubic >> s & 1;
+            t.out_scale = sp.gram[s];
+            t.shift = sp.gram_shift[s];
             if (int32_t rc = product<F32, PAIR, kGram>(t, last, blocks, st)) return rc;
             if (!t.cubic) {
-                t.out_scale = (float)(c * (sb / (sv * sv)));
-                t.shift = (float)(a * sb);
+                t.out_scale = sp.square[s];
+                t.shift = sp.square_shift[s];
                 if (int32_t rc = product<F32, PAIR, kSquare>(t, last, blocks, st)) return rc;
             }
-            t.out_scale = sc.x[s + 1] / sc.b[s] / sc.x[s];
+            t.out_scale = sp.apply[s];
             if (int32_t rc = product<F32, PAIR, kApply>(t, last, blocks, st)) return rc;
             t.from ^= 1;
         }
-        t.out_scale = 1.0f / sc.x[cfg.steps];
+        t.out_scale = sp.last;
         grid = blocks(every_block);
         if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, t)) return rc;
     }
@@ -1160,9 +1442,21 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     D3GS_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= workspace_of(mats, count, *cfg),
                  "%s: workspace missing, unaligned or smaller than d3gs_orthogonalize_workspace_bytes", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!large(mats, count)) return run<true, false>(mats, count, *cfg, muon, sc, ws, st);
-    return cfg->dtype == D3GS_DTYPE_F32 ? run<true, true>(mats, count, *cfg, muon, sc, ws, st)
-                                        : run<false, true>(mats, count, *cfg, muon, sc, ws, st);
+    const Steps sp = steps_of(*cfg, sc);
+    char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
+    Table t{};
+    t.fail = reinterpret_cast<uint32_t*>(at);
+    at += 256;
+    t.bf16 = cfg->dtype == D3GS_DTYPE_BF16;
+    t.eps = cfg->eps;
+    t.mu = cfg->momentum;
+    t.nesterov = cfg->nesterov;
+    t.decay = cfg->decay;
+    t.hooks = test_hooks();
+    if (tiny(mats, count)) return run_tiny(t, sp, mats, count, muon, at, st);
+    if (!large(mats, count)) return run_products<true, false>(t, sp, mats, count, muon, at, st);
+    return cfg->dtype == D3GS_DTYPE_F32 ? run_products<true, true>(t, sp, mats, count, muon, at, st)
+                                        : run_products<false, true>(t, sp, mats, count, muon, at, st);
 }
 
 }  // namespace

@@ -73,7 +73,7 @@ def check(u, what="", **kw):
 
 SIZES = [(1, 1), (1, 7), (5, 1), (2, 2), (3, 64), (64, 64), (65, 63), (127, 129), (128, 128), (129, 1000), (128, 8), (257, 255),
          (300, 70), (512, 192), (200, 1111), (1111, 130), (64, 4000), (1, 5000), (640, 640), (1025, 515),
-         (385, 400), (500, 1300), (700, 2100)]
+         (385, 400), (500, 1300), (700, 2100), (20, 192), (128, 256), (256, 100), (77, 257), (129, 128)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -312,7 +312,7 @@ def test_refusals(cuda_device):
         orthogonalize(torch.empty(16385, 1, device="cuda").expand(16385, 16385))
 
 
-@pytest.mark.parametrize("m,n", [(200, 300), (500, 520)])
+@pytest.mark.parametrize("m,n", [(50, 200), (200, 300), (500, 520)])
 def test_a_wait_that_gives_up_spoils_the_result_and_no_more(cuda_device, m, n):
     """One CTA of every product never asks for its first tile (nothing is in flight when its waits run out): the call
     returns, its result is NaN, and the next call is right."""

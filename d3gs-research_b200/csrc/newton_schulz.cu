@@ -409,16 +409,16 @@ template <bool TWO> __device__ __forceinline__ void write_mirrored(char* block, 
 }
 
 // ---- tiny matrices: the whole chain in one CTA --------------------------------------------------------------------
-// A short side of one tile and a long side of four column blocks: X (128 KB at most) and A or B (64 KB) stay in shared
-// memory from the first step to the last, and a matrix costs one launch instead of seventeen.  What takes time is the way
-// from a product to its epilogue and back, three of each a step.  Sums of hi hi are taken out after every two blocks.
-// B = a I + b A + c A A here, A read back by the thread that wrote it.
-constexpr int kTinyThreads = 288, kTinyCols = 4 * kCols;   // eight warps for the sums, one that issues
+// Where X, A and V fit into shared memory together (sides of at most 128 and 256, seven blocks in all) they stay there from
+// the first step to the last, and a matrix costs one launch instead of seventeen.  What takes time is the way from a
+// product to its epilogue and back, three of each a step.  Sums of hi hi are taken out after every block (after every
+// second one the result of a 128 x 128 matrix was 2.4e-6 off instead of 1.6e-6).
+constexpr int kTinyThreads = 256, kTinyBlocks = 7, kTinyCols = 256;
 
 // the scalars of every step, in the products' scales (see scales_of)
 struct Steps {
     float gram[D3GS_NS_MAX_STEPS], gram_shift[D3GS_NS_MAX_STEPS], square[D3GS_NS_MAX_STEPS], square_shift[D3GS_NS_MAX_STEPS],
-        linear[D3GS_NS_MAX_STEPS], apply[D3GS_NS_MAX_STEPS];
+        apply[D3GS_NS_MAX_STEPS];
     float first, last;    // scale of X at the start, one over that at the end
     uint32_t cubic;       // a bit for each step with c = 0
     int32_t count;
@@ -436,15 +436,16 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     const Matrix& m = t.mat[blockIdx.x];
     const int nk = m.nk, mk = m.mk;
     char* const x = smem;                        // nk blocks
-    char* const ab = smem + nk * (int)kBlock;    // mk blocks: A, then B
-    const uint32_t columns = nk > 2 ? 512 : 256;
+    char* const ab = x + nk * (int)kBlock;       // mk blocks: A, then B
+    char* const v = ab + mk * (int)kBlock;       // mk blocks
+    constexpr uint32_t columns = 512;            // hi hi of two blocks, and the rest (and 128 that a power of two brings)
     if (tid == 0) {
         mbar_init(&s_done, 1);
         mbar_init(&s_end, 1);
         s_failed = 0;
         fence_mbar_init();
     }
-    if (warp == 8) tmem_alloc<1>(&s_tmem, columns);
+    if (warp == 0) tmem_alloc<1>(&s_tmem, columns);
     for (int i = tid; i < nk * (int)kBlock / 16; i += kTinyThreads) reinterpret_cast<uint4*>(x)[i] = make_uint4(0, 0, 0, 0);
     let_next_start();
     wait_for_previous();
@@ -489,10 +490,9 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
 
     // ---- products ----
     const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
-    const int half = (warp >> 2) & 1, row = tid & 127;
+    const int half = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const int tiles = (nk + 1) / 2;              // of B X: 128 columns each
-    const uint32_t rest = tmem + (nk > 2 ? 256 : 128);   // Gram: sums of hi lo + lo hi
     bool ok = true;
     uint32_t phase = 0;
     auto next_phase = [&]() {   // what was written to shared memory is there for the products, TMEM is free
@@ -501,143 +501,122 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
         __syncthreads();
         tc_fence_after();
     };
-    auto issue = [&](uint32_t sum_at, uint32_t rest_at, uint32_t a, uint32_t b, uint32_t step, uint32_t idesc, bool new_sum, bool new_rest) {
+    // one round of products: `blocks` (at most two) column blocks, hi hi of each to a sum of its own, the rest together
+    auto issue = [&](int blocks, uint32_t a, uint32_t a_next, uint32_t b, uint32_t b_next, uint32_t step, uint32_t idesc, bool new_rest) {
+        for (int k = 0; k < blocks; ++k, a += a_next, b += b_next)
 #pragma unroll
-        for (int q = 0; q < kCols / 16; ++q) {
-            const uint64_t ah = operand(a + q * 2), al = operand(a + kPlane / 16 + q * 2);
-            const uint64_t bh = operand(b + q * step), bl = operand(b + kPlane / 16 + q * step);
-            tc_mma<1>(sum_at, ah, bh, idesc, !new_sum || q != 0);
-            tc_mma<1>(rest_at, ah, bl, idesc, !new_rest || q != 0);
-            tc_mma<1>(rest_at, al, bh, idesc, true);
-        }
+            for (int q = 0; q < kCols / 16; ++q) {
+                const uint64_t ah = operand(a + q * 2), al = operand(a + kPlane / 16 + q * 2);
+                const uint64_t bh = operand(b + q * step), bl = operand(b + kPlane / 16 + q * step);
+                tc_mma<1>(tmem + k * 128, ah, bh, idesc, q != 0);
+                tc_mma<1>(tmem + 256, ah, bl, idesc, !new_rest || k != 0 || q != 0);
+                tc_mma<1>(tmem + 256, al, bh, idesc, true);
+            }
+        tc_commit<1>(&s_done);
     };
     auto wait_done = [&]() {
+        __syncwarp();
         if (ok) ok = __all_sync(~0u, wait_for(&s_done, phase & 1, polls));
         if (!ok) s_failed = 1;
         tc_fence_after();
     };
-    const uint32_t x0 = operand_low(smem_u32(x), 16), x0_across = operand_low(smem_u32(x), kBlock), ab0 = operand_low(smem_u32(ab), 16);
+    auto take = [&](float* to, uint32_t at) {   // adds 32 columns
+        float w[32];
+        tmem_load32(tmem + at + lanes, w);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) to[i] += w[i];
+    };
+    constexpr uint32_t kNext = kBlock / 16;
+    const uint32_t x0 = operand_low(smem_u32(x), 16), x0_across = operand_low(smem_u32(x), kBlock), ab0 = operand_low(smem_u32(ab), 16),
+                   v0 = operand_low(smem_u32(v), 16), square = instruction(false, 128, 128), across = instruction(true, 128, 128);
     for (int step = 0; step < sp.count; ++step) {
         const bool cubic = sp.cubic >> step & 1;
-        next_phase();   // A = X X^T
-        if (warp == 8) {
-            if (lane == 0 && !(t.hooks.hold == (int)blockIdx.x && phase == 0)) {   // (a test: these products never come)
-                for (int k = 0; k < nk; ++k) {
-                    const uint32_t b = x0 + k * (kBlock / 16);
-                    issue(tmem + (k >> 1) * 128, rest, b, b, 2, instruction(false, 128, 128), (k & 1) == 0, k == 0);
-                }
-                tc_commit<1>(&s_done);
-            }
-        } else {
+        float f[128];   // 64 of A or B, or 128 of X
+#pragma unroll
+        for (int c = 0; c < 64; ++c) f[c] = 0.0f;
+        for (int k = 0; k < nk; k += 2, ++phase) {   // A = X X^T, two blocks a round
+            next_phase();
+            const int blocks = min(2, nk - k);
+            if (tid == 0 && !(t.hooks.hold == (int)blockIdx.x && phase == 0))   // (a test: the first products never come)
+                issue(blocks, x0 + k * kNext, kNext, x0 + k * kNext, kNext, 2, square, k == 0);
             wait_done();
             if (half < mk) {
-                float v[64];
 #pragma unroll
                 for (int c = 0; c < 64; c += 32) {
-                    float w[32];
-                    tmem_load32(tmem + half * 64 + c + lanes, w);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c + i] = w[i];
-                    if (nk > 2) {
-                        tmem_load32(tmem + 128 + half * 64 + c + lanes, w);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[c + i] += w[i];
-                    }
-                    tmem_load32(rest + half * 64 + c + lanes, w);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c + i] += w[i];
-                }
-                const int on = row < m.m && cubic ? row - half * 64 : -1;
-#pragma unroll
-                for (int c = 0; c < 64; c += 8) {
-                    uint32_t hi[4], lo[4];
-                    finish(v + c, sp.gram[step], sp.gram_shift[step], on - c, hi, lo);
-                    put<true>(ab + half * (int)kBlock + block_offset(row, c), hi, lo);
+                    take(f + c, half * 64 + c);
+                    if (blocks > 1) take(f + c, 128 + half * 64 + c);
+                    if (k + 2 >= nk) take(f + c, 256 + half * 64 + c);
                 }
             }
         }
-        ++phase;
-        if (!cubic) {
-            next_phase();   // B = a I + b A + c A A
-            if (warp == 8) {
-                if (lane == 0) {
-                    for (int k = 0; k < mk; ++k) {
-                        const uint32_t b = ab0 + k * (kBlock / 16);
-                        issue(tmem, tmem + 128, b, b, 2, instruction(false, 128, 128), k == 0, k == 0);
-                    }
-                    tc_commit<1>(&s_done);
+        const int on = row < m.m ? row - half * 64 : -1;   // diagonal
+        if (half < mk) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 8) {
+                uint32_t hi[4], lo[4];
+                const uint32_t at = half * kBlock + block_offset(row, c);
+                finish(f + c, sp.gram[step], sp.gram_shift[step], cubic ? on - c : -1, hi, lo);
+                put<true>(ab + at, hi, lo);
+                if (!cubic) {
+                    finish(f + c, sp.gram[step], sp.gram_shift[step], on - c, hi, lo);
+                    put<true>(v + at, hi, lo);
                 }
-            } else {
-                wait_done();
-                if (half < mk) {
-                    float v[64];
+            }
+        }
+        if (!cubic) {
+            next_phase();   // B = a I + c A V
+            if (tid == 0) issue(mk, ab0, kNext, v0, kNext, 2, square, true);
+            wait_done();
+            if (half < mk) {
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
-                        float w[32];
-                        tmem_load32(tmem + half * 64 + c + lanes, w);
+                for (int c = 0; c < 64; ++c) f[c] = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[c + i] = w[i];
-                        tmem_load32(tmem + 128 + half * 64 + c + lanes, w);
+                for (int c = 0; c < 64; c += 32) {
+                    take(f + c, half * 64 + c);
+                    if (mk > 1) take(f + c, 128 + half * 64 + c);
+                    take(f + c, 256 + half * 64 + c);
+                }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[c + i] += w[i];
-                    }
-                    const int on = row < m.m ? row - half * 64 : -1;
-#pragma unroll
-                    for (int c = 0; c < 64; c += 8) {
-                        char* const at = ab + half * (int)kBlock + block_offset(row, c);
-                        const uint4 h = *reinterpret_cast<const uint4*>(at), l = *reinterpret_cast<const uint4*>(at + kPlane);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
-                            const float2 g = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
-                            v[c + 2 * i] = fmaf(v[c + 2 * i], sp.square[step], (f.x + g.x) * sp.linear[step]);
-                            v[c + 2 * i + 1] = fmaf(v[c + 2 * i + 1], sp.square[step], (f.y + g.y) * sp.linear[step]);
-                        }
-                        uint32_t hi[4], lo[4];
-                        finish(v + c, 1.0f, sp.square_shift[step], on - c, hi, lo);
-                        put<true>(at, hi, lo);
-                    }
+                for (int c = 0; c < 64; c += 8) {
+                    uint32_t hi[4], lo[4];
+                    finish(f + c, sp.square[step], sp.square_shift[step], on - c, hi, lo);
+                    put<true>(ab + half * (int)kBlock + block_offset(row, c), hi, lo);
                 }
             }
             ++phase;
         }
-        next_phase();   // X <- B X, a tile of 128 columns for each half of the warps
-        if (warp == 8) {
-            if (lane == 0) {
-                for (int w = 0; w < tiles; ++w)
-                    for (int k = 0; k < mk; ++k)   // (columns behind X's last block take what lies there, and are not kept)
-                        issue(tmem + w * 256, tmem + w * 256 + 128, ab0 + k * (kBlock / 16),
-                              x0_across + (w * 2 * kBlock + k * (kPlane / 2)) / 16, 2048 / 16, instruction(true, 128, 128), k == 0, k == 0);
-                tc_commit<1>(&s_done);
-            }
-        } else {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) f[c] = 0.0f;
+        for (int w = 0; w < tiles; ++w, ++phase) {   // X <- B X, a tile of 128 columns a round; each half of the warps takes one
+            next_phase();
+            if (tid == 0)   // (columns behind X's last block take what lies there, and are not kept)
+                issue(mk, ab0, kNext, x0_across + w * 2 * kNext, (kPlane / 2) / 16, 2048 / 16, across, true);
             wait_done();
-            if (half < tiles) {
+            if (half == w) {
 #pragma unroll
                 for (int c = 0; c < 128; c += 32) {
-                    if (2 * half + c / kCols >= nk) continue;
-                    float v[32], w[32];
-                    tmem_load32(tmem + half * 256 + c + lanes, v);
-                    tmem_load32(tmem + half * 256 + 128 + c + lanes, w);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] += w[i];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t hi[4], lo[4];
-                        finish(v + i, sp.apply[step], 0.0f, -1, hi, lo);
-                        put<true>(x + (2 * half + c / kCols) * (int)kBlock + block_offset(row, (c + i) % kCols), hi, lo);
-                    }
+                    take(f + c, c);
+                    if (mk > 1) take(f + c, 128 + c);
+                    take(f + c, 256 + c);
                 }
             }
         }
-        ++phase;
+        if (half < tiles) {   // every product has read X by now
+#pragma unroll
+            for (int c = 0; c < 128; c += 8) {
+                if (2 * half + c / kCols >= nk) continue;
+                uint32_t hi[4], lo[4];
+                finish(f + c, sp.apply[step], 0.0f, -1, hi, lo);
+                put<true>(x + (2 * half + c / kCols) * (int)kBlock + block_offset(row, c % kCols), hi, lo);
+            }
+        }
     }
-    if (warp == 8 && lane == 0) {   // whatever was issued has ended before TMEM is handed back
+    if (tid == 0) {   // whatever was issued has ended before TMEM is handed back
         tc_commit<1>(&s_end);
         wait_for(&s_end, 0);
     }
     next_phase();
-    if (warp == 8) tmem_free<1>(tmem, columns);
+    if (warp == 0) tmem_free<1>(tmem, columns);
 
     // ---- result ----
     const bool failed = s_failed != 0;
@@ -1182,8 +1161,10 @@ bool large(const D3gsOrthoMatrix* mats, int32_t count) {
 // One CTA a matrix when all of them are that small.  (A list with one larger matrix goes the other way as a whole: the
 // small ones run beside it there, and cost nothing.)
 bool tiny(const D3gsOrthoMatrix* mats, int32_t count) {
-    for (int32_t i = 0; i < count; ++i)
-        if (min(mats[i].rows, mats[i].cols) > kRows || max(mats[i].rows, mats[i].cols) > kTinyCols) return false;
+    for (int32_t i = 0; i < count; ++i) {
+        const int64_t m = min(mats[i].rows, mats[i].cols), n = max(mats[i].rows, mats[i].cols);
+        if (m > kRows || n > kTinyCols || div_up64(n, kCols) + 2 * div_up64(m, kCols) > kTinyBlocks) return false;
+    }
     return true;
 }
 // Planes of A and B.  Small matrices take two for 16-bit types too: with them it is not the products that take time, and
@@ -1370,20 +1351,19 @@ Steps steps_of(const D3gsOrthoConfig& cfg, const Scales& sc) {
             sp.gram_shift[s] = (float)(b / c * sv);
             sp.square[s] = (float)(c * (sb / (sv * sv)));
             sp.square_shift[s] = (float)(a * sb);
-            sp.linear[s] = (float)(b * (sb / sv));
         }
         sp.apply[s] = sc.x[s + 1] / sc.b[s] / sc.x[s];
     }
     return sp;
 }
 
-// Matrices of one tile and four column blocks: one launch, a CTA each.
+// Tiny matrices: one launch, a CTA each.
 int32_t run_tiny(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t count, bool muon, char* at, cudaStream_t st) {
     for (int32_t i = 0; i < count;) {
         next_table(t, mats, count, i, muon, 2, at);
         if (t.count == 0) break;
         int blocks = 0;
-        for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + t.mat[k].mk);
+        for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + 2 * t.mat[k].mk);
         if (int32_t rc = launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st, t, sp)) return rc;
     }
     return D3GS_OK;

@@ -73,7 +73,7 @@ def check(u, what="", **kw):
 
 SIZES = [(1, 1), (1, 7), (5, 1), (2, 2), (3, 64), (64, 64), (65, 63), (127, 129), (128, 128), (129, 1000), (128, 8), (257, 255),
          (300, 70), (512, 192), (200, 1111), (1111, 130), (64, 4000), (1, 5000), (640, 640), (1025, 515),
-         (385, 400), (500, 1300), (700, 2100), (20, 192), (128, 256), (256, 100), (77, 257), (129, 128)]
+         (385, 400), (500, 1300), (700, 2100), (20, 192), (128, 256), (256, 100), (77, 257), (129, 128), (100, 192), (192, 128), (100, 193)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

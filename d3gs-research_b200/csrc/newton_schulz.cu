@@ -316,18 +316,18 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ float load_shared_of(uint32_t at, uint32_t rank) {
-    float v;
+// four floats at the same place in CTA `rank` of the cluster
+__device__ __forceinline__ float4 load_shared_of(uint32_t at, uint32_t rank) {
+    float4 v;
     asm volatile(
         "{\n\t.reg .b32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %1, %2;\n\t"
-        "ld.shared::cluster.f32 %0, [a];\n\t}"
-        : "=f"(v)
+        "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
         : "r"(at), "r"(rank)
         : "memory");
     return v;
 }
-
 // mbar_wait_bounded without its sleep: a wait here is a link of the chain that every column block goes through.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint32_t limit = 0) {
     const uint32_t polls = limit != 0 ? limit : (1u << 24);
@@ -782,42 +782,67 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         const uint32_t r = threadIdx.x;
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
         char* const out = MODE == kGram && !t.cubic ? m.a : MODE != kApply ? m.b : m.x[t.from ^ 1];
-            float* const sums = reinterpret_cast<float*>(smem);
+        float4* const sums = reinterpret_cast<float4*>(smem) + r;   // four columns of 128 rows after one another
         if (parts > 1) {
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) sums[c * 128 + r] = v[c];
+            for (int c = 0; c < kTile; c += 4) sums[c * 32] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
         }
         if (!ok) *t.fail = 1;
         if (parts > 1) cluster_sync();
-        const int share = kTile / parts, from = part * share;   // columns this CTA finishes
-        // eight columns at a time; with one CTA they are in registers, where only constants can index
-        auto piece = [&](int c, const float* w) {
-            if (2 * tj + c / kCols >= wide) return;
-            char* const to = out + ((int64_t)ti * wide + 2 * tj + c / kCols) * kBlock + block_offset(r, c % kCols);
+        // Eight columns of the result.  `direct`: this tile's blocks, `mirror`: the mirrored tile's, where this thread's row
+        // is a column, `diagonal`: V's, of tiles on the diagonal; each two neighbouring blocks.
+        auto piece = [&](int c, const float* w, char* direct, char* mirror, char* diagonal) {
+            const uint32_t o = (c / kCols) * kBlock + block_offset(r, c % kCols);
             uint32_t hi[4], lo[4];
-            const int on = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;   // diagonal
+            const int on = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;
             finish(w, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
-            put<true>(to, hi, lo);
+            put<true>(direct + o, hi, lo);
+            if (MODE != kApply && !same) write_mirrored<true>(mirror + (r / kCols) * kBlock, c, r % kCols, hi, lo);
             if (MODE == kGram && same && !t.cubic) {
-                uint32_t vh[4], vl[4];
-                finish(w, t.out_scale, t.shift, on, vh, vl);
-                put<true>(m.v + (int64_t)(2 * ti + c / kCols) * kBlock + block_offset(r, c % kCols), vh, vl);
+                finish(w, t.out_scale, t.shift, on, hi, lo);
+                put<true>(diagonal + o, hi, lo);
             }
-            if (MODE != kApply && !same)   // the mirrored tile: this thread's row is a column
-                write_mirrored<true>(out + ((int64_t)tj * wide + 2 * ti + r / kCols) * kBlock, c, r % kCols, hi, lo);
         };
+        char* const direct = out + ((int64_t)ti * wide + 2 * tj) * kBlock;
+        char* const mirror = out + ((int64_t)tj * wide + 2 * ti) * kBlock;
+        char* const diagonal = m.v + (int64_t)2 * ti * kBlock;
+        const int valid = min(2, wide - 2 * tj);         // of the two blocks
         if (parts == 1) {
+            // by way of shared memory, from where whole blocks leave: stores from here would touch 32 lines each
 #pragma unroll
-            for (int c = 0; c < kTile; c += 8) piece(c, v + c);
+            for (int c = 0; c < kTile; c += 8)
+                if (c / kCols < valid) piece(c, v + c, smem, smem + 2 * kBlock, smem + 2 * kBlock);
+            fence_proxy_async_smem();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 0 && ok) {
+                bulk_copy_s2g(direct, smem, valid * kBlock);
+                if (MODE != kApply && !same) bulk_copy_s2g(mirror, smem + 2 * kBlock, 2 * kBlock);
+                if (MODE == kGram && same && !t.cubic) bulk_copy_s2g(diagonal, smem + 2 * kBlock, valid * kBlock);
+                bulk_commit_group();
+                bulk_wait_group_read0();   // (what leaves is in memory when the grid has ended)
+            }
         } else {
+            const int share = kTile / parts, from = part * share;   // columns this CTA finishes
             for (int c = from; c < from + share; c += 8) {
+                if (c / kCols >= valid) continue;
+                // all parts on their way before the first is added
+                float4 a[8], b[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < parts) {
+                        a[q] = load_shared_of(smem_u32(sums + c * 32), q);
+                        b[q] = load_shared_of(smem_u32(sums + (c + 4) * 32), q);
+                    }
                 float w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) w[i] = 0.0f;
-                for (int q = 0; q < parts; ++q)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] += load_shared_of(smem_u32(sums + (c + i) * 128 + r), q);
-                piece(c, w);
+                for (int q = 0; q < 8; ++q)
+                    if (q < parts) {
+                        w[0] += a[q].x, w[1] += a[q].y, w[2] += a[q].z, w[3] += a[q].w;
+                        w[4] += b[q].x, w[5] += b[q].y, w[6] += b[q].z, w[7] += b[q].w;
+                    }
+                piece(c, w, direct, mirror, diagonal);
             }
             cluster_sync();   // no CTA leaves while another reads its sums
         }

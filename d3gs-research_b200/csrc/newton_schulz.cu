@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kMaxMatrices = 32;   // per launch, a table of less than 4 KB; longer lists are cut
 constexpr int kThreads = 256;
-constexpr int kNormChunk = 8192;   // values per CTA of the norm pass
+constexpr int kPieces = 1024;       // pieces of eight neighbouring columns per CTA of the norm pass
 constexpr int kMaxShort = 16384, kMaxLong = 1 << 24;
 constexpr int kRows = 128, kCols = 64;                 // one block
 constexpr uint32_t kPlane = kRows * kCols * 2;         // bytes of one fp16 plane of a block
@@ -98,24 +98,85 @@ __device__ __forceinline__ float update_of(const Table& t, float g, float buf) {
     return t.nesterov ? fmaf(t.mu, buf, (1.0f - t.mu) * g) : buf;
 }
 
+// Eight neighbouring columns of a row of U, of which `n` exist; where rows are so aligned, as vectors.
+struct Access {
+    bool src, state;   // gradient or update; momentum and parameter
+};
+__device__ __forceinline__ Access access_of(const Table& t, const Matrix& m) {
+    Access a;
+    a.src = ((uintptr_t)m.src & 15) == 0 && m.src_stride % (t.bf16 ? 8 : 4) == 0;
+    a.state = (((uintptr_t)m.momentum | (uintptr_t)m.dst) & 15) == 0 && m.cols % (t.bf16 ? 8 : 4) == 0;
+    return a;
+}
+__device__ __forceinline__ void load8(const float* p, bool vector, int n, float (&v)[8]) {
+    if (vector && n == 8) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store8(float* p, bool vector, int n, const float (&v)[8]) {
+    if (vector && n == 8) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = v[i];
+    }
+}
+__device__ __forceinline__ void load_src8(const Table& t, const Matrix& m, int64_t at, bool vector, int n, float (&v)[8]) {
+    if (!t.bf16) return load8(static_cast<const float*>(m.src) + at, vector, n, v);
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(m.src) + at;
+    if (vector && n == 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(q[i] << 16);
+            v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
+    }
+}
+
 // ---- new momentum, and the sum of squares of the update (in 64 bits: no value of a float overflows it) -----------
 __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant__ Table t) {
     __shared__ double s[kThreads / 32];
+    int block;
+    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
+    const unsigned per_row = (m.cols + 7) / 8, pieces = m.rows * per_row;
+    const Access access = access_of(t, m);
     let_next_start();
     wait_for_previous();
     if (blockIdx.x == 0 && threadIdx.x == 0) *t.fail = 0;
-    int block;
-    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
-    const int64_t count = (int64_t)m.rows * m.cols, i0 = (int64_t)block * kNormChunk, i1 = min(count, i0 + kNormChunk);
     double sum = 0.0;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) {
-        float u = load_src(t, m, i / m.cols, i % m.cols);
+    float u[kPieces / kThreads][8], buf[kPieces / kThreads][8];
+#pragma unroll
+    for (int k = 0; k < kPieces / kThreads; ++k) {
+        const unsigned i = (unsigned)block * kPieces + k * kThreads + threadIdx.x;
+        const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
+        load_src8(t, m, n ? r * m.src_stride + c : 0, access.src, n, u[k]);
+        if (m.momentum) load8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces / kThreads; ++k) {
         if (m.momentum) {
-            const float buf = fmaf(t.mu, m.momentum[i], (1.0f - t.mu) * u);
-            m.momentum[i] = buf;
-            u = update_of(t, u, buf);
+            const unsigned i = (unsigned)block * kPieces + k * kThreads + threadIdx.x;
+            const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                buf[k][j] = fmaf(t.mu, buf[k][j], (1.0f - t.mu) * u[k][j]);
+                u[k][j] = update_of(t, u[k][j], buf[k][j]);
+            }
+            store8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
         }
-        sum += (double)u * (double)u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += (double)u[k][j] * (double)u[k][j];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -130,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
 // every CTA adds the sums up itself, in the same order
 __device__ __forceinline__ float inverse_norm(const Table& t, const Matrix& m) {
     __shared__ double s[kThreads / 32];
-    const int n = (int)(((int64_t)m.rows * m.cols + kNormChunk - 1) / kNormChunk);
+    const int n = (int)(((int64_t)m.rows * ((m.cols + 7) / 8) + kPieces - 1) / kPieces);
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += kThreads) sum += m.norms[i];
 #pragma unroll
@@ -147,50 +208,60 @@ __device__ __forceinline__ float inverse_norm(const Table& t, const Matrix& m) {
 __device__ __forceinline__ uint32_t block_offset(uint32_t r, uint32_t c) {
     return r * 128u + (((c >> 3) ^ (r & 7u)) << 4) + (c & 7u) * 2u;
 }
-// v = hi + lo with 22 bits; lo takes what hi's rounding left
-__device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
-    hi = __float2half_rn(v);
-    lo = __float2half_rn(v - __half2float(hi));
-}
-__device__ __forceinline__ uint32_t pack(__half a, __half b) {
-    return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16);
+// A pair of values v = hi + lo with 22 bits each, as pairs of fp16: hi, and what its rounding left.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // ---- first pass: blocks of X = U / norm, transposed when the matrix is tall; one CTA per block --------------------
+// Pieces of eight columns of U.  As rows of X they go straight to their block, eight threads to a 128-byte line; as
+// columns by way of shared memory.
 __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant__ Table t) {
-    __shared__ __align__(16) uint32_t s[2 * kPlane / 4];
-    let_next_start();
-    wait_for_previous();
+    __shared__ __align__(16) char s[2 * kPlane];
     int block;
     const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
-    const float inv = inverse_norm(t, m);
     const bool tall = m.rows > m.cols;
     const int r0 = block / m.nk * kRows, c0 = block % m.nk * kCols;
-    // two neighbouring columns of X a thread; neighbouring threads along the rows of U
-    for (int i = threadIdx.x; i < kRows * kCols / 2; i += kThreads) {
-        const int r = tall ? i % kRows : i / (kCols / 2), c = (tall ? i / kRows : i % (kCols / 2)) * 2;
-        float v[2];
+    const Access access = access_of(t, m);
+    char* const out = m.x[0] + (int64_t)block * 2 * kPlane;
+    let_next_start();
+    wait_for_previous();
+    const float scale = inverse_norm(t, m) * t.out_scale;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < kRows * kCols / 8; i += kThreads) {
+        // row and column within the block's part of U
+        const int r = tall ? i % kCols : i / (kCols / 8), c = (tall ? i / kCols : i % (kCols / 8)) * 8;
+        const int ur = (tall ? c0 : r0) + r, uc = (tall ? r0 : c0) + c, n = ur < m.rows ? max(0, min(8, m.cols - uc)) : 0;
+        float u[8], buf[8];
+        load_src8(t, m, n ? ur * m.src_stride + uc : 0, access.src, n, u);
+        if (m.momentum) {
+            load8(m.momentum + (n ? (int64_t)ur * m.cols + uc : 0), access.state, n, buf);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int64_t xr = r0 + r, xc = c0 + c + k;
-            v[k] = 0.0f;
-            if (xr < m.m && xc < m.n) {
-                const int64_t ur = tall ? xc : xr, uc = tall ? xr : xc;
-                float u = load_src(t, m, ur, uc);
-                if (m.momentum) u = update_of(t, u, m.momentum[ur * m.cols + uc]);
-                v[k] = u * inv * t.out_scale;
+            for (int j = 0; j < 8; ++j) u[j] = update_of(t, u[j], buf[j]);
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2(u[2 * j] * scale, u[2 * j + 1] * scale, hi[j], lo[j]);
+        if (!tall) {
+            const uint32_t o = block_offset(r, c);
+            *reinterpret_cast<uint4*>(out + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(out + kPlane + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t o = block_offset(c + j, r);
+                *reinterpret_cast<uint16_t*>(s + o) = (uint16_t)(hi[j / 2] >> (16 * (j & 1)));
+                *reinterpret_cast<uint16_t*>(s + kPlane + o) = (uint16_t)(lo[j / 2] >> (16 * (j & 1)));
             }
         }
-        __half h[2], l[2];
-        split(v[0], h[0], l[0]);
-        split(v[1], h[1], l[1]);
-        const uint32_t o = block_offset(r, c) / 4;
-        s[o] = pack(h[0], h[1]);
-        s[kPlane / 4 + o] = pack(l[0], l[1]);
     }
+    if (!tall) return;
     __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(m.x[0] + (int64_t)block * 2 * kPlane);
-    for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(s)[i];
+    for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s)[i];
 }
 
 // value i of the result: stored, or taken from the parameter
@@ -207,25 +278,57 @@ __device__ __forceinline__ void write_result(const Table& t, const Matrix& m, in
 
 // ---- last pass: result or parameter from the blocks of X; one CTA per block ---------------------------------------
 __global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constant__ Table t) {
-    wait_for_previous();
     int block;
     const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
-    const bool tall = m.rows > m.cols, failed = *t.fail != 0;
+    const bool tall = m.rows > m.cols;
     const int r0 = block / m.nk * kRows, c0 = block % m.nk * kCols;
-    const char* x = m.x[t.from] + (int64_t)block * 2 * kPlane;
-    for (int i = threadIdx.x; i < kRows * kCols / 2; i += kThreads) {
-        const int r = tall ? i % kRows : i / (kCols / 2), c = (tall ? i / kRows : i % (kCols / 2)) * 2;
-        const uint32_t o = block_offset(r, c);
-        const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(x + o));
-        const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(x + kPlane + o));
+    const Access access = access_of(t, m);
+    const char* const x = m.x[t.from] + (int64_t)block * 2 * kPlane;
+    wait_for_previous();
+    const bool failed = *t.fail != 0;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < kRows * kCols / 8; i += kThreads) {
+        const int r = tall ? i % kCols : i / (kCols / 8), c = (tall ? i / kCols : i % (kCols / 8)) * 8;
+        const int ur = (tall ? c0 : r0) + r, uc = (tall ? r0 : c0) + c, n = ur < m.rows ? max(0, min(8, m.cols - uc)) : 0;
+        if (n == 0) continue;
+        float v[8];
+        if (!tall) {
+            const uint32_t o = block_offset(r, c);
+            const uint4 h = *reinterpret_cast<const uint4*>(x + o), l = *reinterpret_cast<const uint4*>(x + kPlane + o);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int64_t xr = r0 + r, xc = c0 + c + k;
-            if (xr >= m.m || xc >= m.n) continue;
-            const int64_t j = tall ? xc * m.cols + xr : xr * m.cols + xc;
-            float v = (k ? hi.y + lo.y : hi.x + lo.x) * t.out_scale;
-            if (failed) v = __int_as_float(0x7fffffff);
-            write_result(t, m, j, v);
+            for (int j = 0; j < 4; ++j) {
+                const float2 a = __half22float2(reinterpret_cast<const __half2*>(&h)[j]), b = __half22float2(reinterpret_cast<const __half2*>(&l)[j]);
+                v[2 * j] = a.x + b.x;
+                v[2 * j + 1] = a.y + b.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {   // (neighbouring threads read neighbouring columns of X)
+                const uint32_t o = block_offset(c + j, r);
+                v[j] = __half2float(*reinterpret_cast<const __half*>(x + o)) + __half2float(*reinterpret_cast<const __half*>(x + kPlane + o));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = failed ? __int_as_float(0x7fffffff) : v[j] * t.out_scale;
+        const int64_t at = (int64_t)ur * m.cols + uc;
+        if (m.momentum) {
+            float p[8];
+            load8(static_cast<const float*>(m.dst) + at, access.state, n, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = fmaf(-m.rate, v[j], t.decay * p[j]);
+            store8(static_cast<float*>(m.dst) + at, access.state, n, p);
+        } else if (!t.bf16) {
+            store8(static_cast<float*>(m.dst) + at, access.state, n, v);
+        } else if (access.state && n == 8) {
+            uint4 w;
+            __nv_bfloat162* const q = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m.dst) + at) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) static_cast<__nv_bfloat16*>(m.dst)[at + j] = __float2bfloat16_rn(v[j]);
         }
     }
 }
@@ -370,14 +473,6 @@ template <bool F32, int MODE, int RIGHT> struct Planes {
     static constexpr uint32_t kAB = (F32 ? 2 : 1) * kPlane, kX = 2 * kPlane;   // bytes of one block
 };
 
-// A pair of values as pairs of fp16: hi and what hi's rounding left.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 // One 16-byte piece of a result: eight columns of a row, from sums to planes; `diagonal`: which of them takes the shift.
 __device__ __forceinline__ void finish(const float* v, float scale, float shift, int diagonal, uint32_t* hi, uint32_t* lo) {
     float f[8];
@@ -1171,7 +1266,7 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.nk = (p.n + kCols - 1) / kCols;
     p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
-    p.norms = up256((size_t)div_up64(d.rows * d.cols, kNormChunk) * 8);
+    p.norms = up256((size_t)div_up64(d.rows * ((d.cols + 7) / 8), kPieces) * 8);
     p.v = (size_t)p.mb * 2 * planes * kPlane;
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
@@ -1410,7 +1505,7 @@ int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int
         };
         auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
         t.from = 0;
-        unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * m.cols, kNormChunk); });
+        unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
         if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, t)) return rc;
         t.out_scale = sp.first;
         grid = blocks(every_block);

@@ -877,58 +877,37 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         const uint32_t r = threadIdx.x;
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
         char* const out = MODE == kGram && !t.cubic ? m.a : MODE != kApply ? m.b : m.x[t.from ^ 1];
-        float4* const sums = reinterpret_cast<float4*>(smem) + r;   // four columns of 128 rows after one another
-        if (parts > 1) {
+        // The sums go through shared memory, four columns of 128 rows after one another, so that what follows is a loop: code
+        // that every CTA runs once is bound by fetching it, and unrolled over the registers it took twice the time.
+        float4* const sums = reinterpret_cast<float4*>(smem) + r;
 #pragma unroll
-            for (int c = 0; c < kTile; c += 4) sums[c * 32] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-        }
+        for (int c = 0; c < kTile; c += 4) sums[c * 32] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
         if (!ok) *t.fail = 1;
         if (parts > 1) cluster_sync();
-        // Eight columns of the result.  `direct`: this tile's blocks, `mirror`: the mirrored tile's, where this thread's row
-        // is a column, `diagonal`: V's, of tiles on the diagonal; each two neighbouring blocks.
-        auto piece = [&](int c, const float* w, char* direct, char* mirror, char* diagonal) {
-            const uint32_t o = (c / kCols) * kBlock + block_offset(r, c % kCols);
-            uint32_t hi[4], lo[4];
-            const int on = same && ti * kRows + (int)r < m.m ? (int)r - c : -1;
-            finish(w, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
-            put<true>(direct + o, hi, lo);
-            if (MODE != kApply && !same) write_mirrored<true>(mirror + (r / kCols) * kBlock, c, r % kCols, hi, lo);
-            if (MODE == kGram && same && !t.cubic) {
-                finish(w, t.out_scale, t.shift, on, hi, lo);
-                put<true>(diagonal + o, hi, lo);
-            }
-        };
-        char* const direct = out + ((int64_t)ti * wide + 2 * tj) * kBlock;
-        char* const mirror = out + ((int64_t)tj * wide + 2 * ti) * kBlock;
-        char* const diagonal = m.v + (int64_t)2 * ti * kBlock;
-        const int valid = min(2, wide - 2 * tj);         // of the two blocks
-        if (parts == 1) {
-            // by way of shared memory, from where whole blocks leave: stores from here would touch 32 lines each
-#pragma unroll
-            for (int c = 0; c < kTile; c += 8)
-                if (c / kCols < valid) piece(c, v + c, smem, smem + 2 * kBlock, smem + 2 * kBlock);
-            fence_proxy_async_smem();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (threadIdx.x == 0 && ok) {
-                bulk_copy_s2g(direct, smem, valid * kBlock);
-                if (MODE != kApply && !same) bulk_copy_s2g(mirror, smem + 2 * kBlock, 2 * kBlock);
-                if (MODE == kGram && same && !t.cubic) bulk_copy_s2g(diagonal, smem + 2 * kBlock, valid * kBlock);
-                bulk_commit_group();
-                bulk_wait_group_read0();   // (what leaves is in memory when the grid has ended)
-            }
-        } else {
-            const int share = kTile / parts, from = part * share;   // columns this CTA finishes
-            for (int c = from; c < from + share; c += 8) {
-                if (c / kCols >= valid) continue;
-                // all parts on their way before the first is added
-                float4 a[8], b[8];
+        const int valid = min(2, wide - 2 * tj);         // of the tile's two blocks across
+        const bool mirrored = MODE != kApply && !same, keeps_v = MODE == kGram && same && !t.cubic;
+        // This tile's blocks; the mirrored tile's, where this thread's row is a column, or V's, of tiles on the diagonal.
+        // With one CTA they are put together in shared memory and leave as whole blocks.
+        char* const to_direct = out + ((int64_t)ti * wide + 2 * tj) * kBlock;
+        char* const to_other = mirrored ? out + ((int64_t)tj * wide + 2 * ti) * kBlock : m.v + (int64_t)2 * ti * kBlock;
+        char* const direct = parts == 1 ? smem + 2 * kBlock : to_direct;
+        char* const other = parts == 1 ? smem + 4 * kBlock : to_other;
+        const int share = kTile / parts, end = min((part + 1) * share, valid * kCols);   // columns this CTA finishes
+        const int diagonal = same && ti * kRows + (int)r < m.m ? (int)r : -256;
+#pragma unroll 1
+        for (int c = part * share; c < end; c += 8) {
+            float w[8];
+            if (parts == 1) {
+                const float4 a = sums[c * 32], b = sums[(c + 4) * 32];
+                w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+            } else {
+                float4 a[8], b[8];   // all parts on their way before the first is added
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                     if (q < parts) {
                         a[q] = load_shared_of(smem_u32(sums + c * 32), q);
                         b[q] = load_shared_of(smem_u32(sums + (c + 4) * 32), q);
                     }
-                float w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) w[i] = 0.0f;
 #pragma unroll
@@ -937,8 +916,27 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                         w[0] += a[q].x, w[1] += a[q].y, w[2] += a[q].z, w[3] += a[q].w;
                         w[4] += b[q].x, w[5] += b[q].y, w[6] += b[q].z, w[7] += b[q].w;
                     }
-                piece(c, w, direct, mirror, diagonal);
             }
+            const uint32_t o = (c / kCols) * kBlock + block_offset(r, c % kCols);
+            uint32_t hi[4], lo[4];
+            finish(w, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? diagonal - c : -1, hi, lo);
+            put<true>(direct + o, hi, lo);
+            if (mirrored) write_mirrored<true>(other + (r / kCols) * kBlock, c, r % kCols, hi, lo);
+            if (keeps_v) {
+                finish(w, t.out_scale, t.shift, diagonal - c, hi, lo);
+                put<true>(other + o, hi, lo);
+            }
+        }
+        if (parts == 1) {
+            fence_proxy_async_smem();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 0 && ok) {
+                bulk_copy_s2g(to_direct, direct, valid * kBlock);
+                if (mirrored || keeps_v) bulk_copy_s2g(to_other, other, (mirrored ? 2 : valid) * kBlock);
+                bulk_commit_group();
+                bulk_wait_group_read0();   // (what leaves is in memory when the grid has ended)
+            }
+        } else {
             cluster_sync();   // no CTA leaves while another reads its sums
         }
     }

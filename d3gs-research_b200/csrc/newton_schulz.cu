@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
 // ---- small matrices: one 128 x 128 tile a cluster, its CTAs share the summed axis ---------------------------------
 // With few tiles the summed axis is what takes time: the CTAs of a cluster (1, 2, 4 or 8) each sum a part of it, put
 // their sums into shared memory and each finish a part of the columns, adding the parts in the order of their ranks.
-constexpr int kSmallThreads = 192, kTile = 128;
+constexpr int kSmallThreads = 320, kTile = 128;
 struct SmallStages {
     static constexpr uint32_t kLeft = 2 * kPlane, kRight = 2 * kPlane, kStage = kLeft + kRight;
     static constexpr int kCount = 3;
@@ -753,12 +753,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_sum[i], 1);
-            mbar_init(&s_taken[i], 128);
+            mbar_init(&s_taken[i], 256);
         }
         mbar_init(&s_last, 1);
         fence_mbar_init();
     }
-    if (warp == 5) tmem_alloc<1>(&s_tmem, kTmem);
+    if (warp == 9) tmem_alloc<1>(&s_tmem, kTmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     let_next_start();
     wait_for_previous();
 
-    if (warp == 4) {
+    if (warp == 8) {
         if (lane == 0) {
             int k = 0;
             for (; k < blocks; ++k) {
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
                     wait_for(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         if (lane == 0) {
             const uint32_t idesc = instruction(MODE == kApply, 128, kTile);
             constexpr uint32_t kStep = (MODE == kApply ? 2048 : 32) / 16, kNext = MODE == kApply ? kPlane / 2 : 16;
@@ -850,14 +850,16 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             if (!ok) wait_for(&s_last, 0);
         }
     } else {
-        float v[kTile];
+        constexpr int kPart = kTile / 2;                 // columns of a thread; the warps' upper half takes the right ones
+        const int half = warp >> 2;
+        float v[kPart];
 #pragma unroll
-        for (int c = 0; c < kTile; ++c) v[c] = 0.0f;
+        for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
         auto take = [&](uint32_t from) {
 #pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
+            for (int c = 0; c < kPart; c += 32) {
                 float w[32];
-                tmem_load32(tmem + from + c + ((uint32_t)warp << 21), w);
+                tmem_load32(tmem + from + half * kPart + c + ((uint32_t)(warp & 3) << 21), w);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[c + i] += w[i];
             }
@@ -874,14 +876,14 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         tc_fence_after();
         if (ok && blocks > 0) take(2 * kTile);
         // every product has read its operands by now: their shared memory is free
-        const uint32_t r = threadIdx.x;
+        const uint32_t r = threadIdx.x & 127;
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
         char* const out = MODE == kGram && !t.cubic ? m.a : MODE != kApply ? m.b : m.x[t.from ^ 1];
         // The sums go through shared memory, four columns of 128 rows after one another, so that what follows is a loop: code
         // that every CTA runs once is bound by fetching it, and unrolled over the registers it took twice the time.
         float4* const sums = reinterpret_cast<float4*>(smem) + r;
 #pragma unroll
-        for (int c = 0; c < kTile; c += 4) sums[c * 32] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+        for (int c = 0; c < kPart; c += 4) sums[(half * kPart + c) * 32] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
         if (!ok) *t.fail = 1;
         if (parts > 1) cluster_sync();
         const int valid = min(2, wide - 2 * tj);         // of the tile's two blocks across
@@ -892,10 +894,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         char* const to_other = mirrored ? out + ((int64_t)tj * wide + 2 * ti) * kBlock : m.v + (int64_t)2 * ti * kBlock;
         char* const direct = parts == 1 ? smem + 2 * kBlock : to_direct;
         char* const other = parts == 1 ? smem + 4 * kBlock : to_other;
-        const int share = kTile / parts, end = min((part + 1) * share, valid * kCols);   // columns this CTA finishes
+        const int share = kPart / parts, begin = (2 * part + half) * share;   // columns this CTA finishes, half of them here
+        const int end = min(begin + share, valid * kCols);
         const int diagonal = same && ti * kRows + (int)r < m.m ? (int)r : -256;
 #pragma unroll 1
-        for (int c = part * share; c < end; c += 8) {
+        for (int c = begin; c < end; c += 8) {
             float w[8];
             if (parts == 1) {
                 const float4 a = sums[c * 32], b = sums[(c + 4) * 32];
@@ -929,7 +932,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         }
         if (parts == 1) {
             fence_proxy_async_smem();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             if (threadIdx.x == 0 && ok) {
                 bulk_copy_s2g(to_direct, direct, valid * kBlock);
                 if (mirrored || keeps_v) bulk_copy_s2g(to_other, other, (mirrored ? 2 : valid) * kBlock);
@@ -940,7 +943,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             cluster_sync();   // no CTA leaves while another reads its sums
         }
     }
-    if (warp >= 4) {
+    if (warp >= 8) {
         if (!ok) *t.fail = 1;
         __syncwarp();
         if (parts > 1) {
@@ -951,7 +954,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_free<1>(tmem, kTmem);
+    if (warp == 9) tmem_free<1>(tmem, kTmem);
 }
 
 // ---- large matrices: one 256 x N tile a pair of CTAs --------------------------------------------------------------

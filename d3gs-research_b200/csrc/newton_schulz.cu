@@ -89,10 +89,6 @@ __device__ __forceinline__ int find_matrix(const Table& t, int id, int& block) {
     return lo;
 }
 
-__device__ __forceinline__ float load_src(const Table& t, const Matrix& m, int64_t r, int64_t c) {
-    const int64_t i = r * m.src_stride + c;
-    return t.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(m.src)[i]) : static_cast<const float*>(m.src)[i];
-}
 // the update from gradient and NEW momentum
 __device__ __forceinline__ float update_of(const Table& t, float g, float buf) {
     return t.nesterov ? fmaf(t.mu, buf, (1.0f - t.mu) * g) : buf;
@@ -264,15 +260,29 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
     for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s)[i];
 }
 
-// value i of the result: stored, or taken from the parameter
-__device__ __forceinline__ void write_result(const Table& t, const Matrix& m, int64_t i, float v) {
+// Eight neighbouring values of the result: stored, or taken from the parameter.
+__device__ __forceinline__ void write_result8(const Table& t, const Matrix& m, int64_t at, bool vector, int n, float (&v)[8], float scale,
+                                              bool failed) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = failed ? __int_as_float(0x7fffffff) : v[j] * scale;
     if (m.momentum) {
-        float* p = static_cast<float*>(m.dst) + i;
-        *p = fmaf(-m.rate, v, t.decay * *p);
-    } else if (t.bf16) {
-        static_cast<__nv_bfloat16*>(m.dst)[i] = __float2bfloat16_rn(v);
+        float p[8];
+        load8(static_cast<const float*>(m.dst) + at, vector, n, p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = fmaf(-m.rate, v[j], t.decay * p[j]);
+        store8(static_cast<float*>(m.dst) + at, vector, n, p);
+    } else if (!t.bf16) {
+        store8(static_cast<float*>(m.dst) + at, vector, n, v);
+    } else if (vector && n == 8) {
+        uint4 w;
+        __nv_bfloat162* const q = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m.dst) + at) = w;
     } else {
-        static_cast<float*>(m.dst)[i] = v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) static_cast<__nv_bfloat16*>(m.dst)[at + j] = __float2bfloat16_rn(v[j]);
     }
 }
 
@@ -308,28 +318,7 @@ __global__ void __launch_bounds__(kThreads) ns_store_kernel(const __grid_constan
                 v[j] = __half2float(*reinterpret_cast<const __half*>(x + o)) + __half2float(*reinterpret_cast<const __half*>(x + kPlane + o));
             }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = failed ? __int_as_float(0x7fffffff) : v[j] * t.out_scale;
-        const int64_t at = (int64_t)ur * m.cols + uc;
-        if (m.momentum) {
-            float p[8];
-            load8(static_cast<const float*>(m.dst) + at, access.state, n, p);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = fmaf(-m.rate, v[j], t.decay * p[j]);
-            store8(static_cast<float*>(m.dst) + at, access.state, n, p);
-        } else if (!t.bf16) {
-            store8(static_cast<float*>(m.dst) + at, access.state, n, v);
-        } else if (access.state && n == 8) {
-            uint4 w;
-            __nv_bfloat162* const q = reinterpret_cast<__nv_bfloat162*>(&w);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m.dst) + at) = w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < n) static_cast<__nv_bfloat16*>(m.dst)[at + j] = __float2bfloat16_rn(v[j]);
-        }
+        write_result8(t, m, (int64_t)ur * m.cols + uc, access.state, n, v, t.out_scale, failed);
     }
 }
 
@@ -545,20 +534,34 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     let_next_start();
     wait_for_previous();
 
-    // ---- momentum, norm, X ----
-    const int count = m.rows * m.cols;
+    // ---- momentum, norm, X: pieces of eight columns of U ----
     const bool tall = m.rows > m.cols;
-    double sum = 0.0;
-#pragma unroll 8
-    for (int i = tid; i < count; i += kTinyThreads) {
-        const int r = i / m.cols, c = i - r * m.cols;
-        float u = load_src(t, m, r, c);
+    const int per_row = (m.cols + 7) / 8, pieces = m.rows * per_row;
+    const Access access = access_of(t, m);
+    auto load_piece = [&](int i, int& r, int& c, float (&u)[8], bool update) {
+        r = i / per_row;
+        c = (i - r * per_row) * 8;
+        const int n = min(8, m.cols - c);
+        load_src8(t, m, r * m.src_stride + c, access.src, n, u);
         if (m.momentum) {
-            const float buf = fmaf(t.mu, m.momentum[i], (1.0f - t.mu) * u);
-            m.momentum[i] = buf;
-            u = update_of(t, u, buf);
+            float buf[8];
+            load8(m.momentum + r * m.cols + c, access.state, n, buf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (update) buf[e] = fmaf(t.mu, buf[e], (1.0f - t.mu) * u[e]);
+                u[e] = update_of(t, u[e], buf[e]);
+            }
+            if (update) store8(m.momentum + r * m.cols + c, access.state, n, buf);
         }
-        sum += (double)u * (double)u;
+    };
+    double sum = 0.0;
+#pragma unroll 2
+    for (int i = tid; i < pieces; i += kTinyThreads) {
+        int r, c;
+        float u[8];
+        load_piece(i, r, c, u, true);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += (double)u[e] * (double)u[e];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -570,17 +573,24 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     for (int k = 0; k < kTinyThreads / 32; ++k) sum += s_norm[k];
     const double norm = sqrt(sum);
     const float scale = (float)(1.0 / (norm < (double)t.eps ? (double)t.eps : norm)) * sp.first;   // a NaN stays one
-#pragma unroll 8
-    for (int i = tid; i < count; i += kTinyThreads) {   // (a thread reads the momentum that it wrote)
-        const int r = i / m.cols, c = i - r * m.cols;
-        float u = load_src(t, m, r, c);
-        if (m.momentum) u = update_of(t, u, m.momentum[i]);
-        u *= scale;
-        const int xr = tall ? c : r, xc = tall ? r : c;
-        char* const to = x + (xc / kCols) * (int)kBlock + block_offset(xr, xc % kCols);
-        const __half h = __float2half_rn(u);
-        *reinterpret_cast<__half*>(to) = h;
-        *reinterpret_cast<__half*>(to + kPlane) = __float2half_rn(u - __half2float(h));
+#pragma unroll 2
+    for (int i = tid; i < pieces; i += kTinyThreads) {   // (a thread reads the momentum that it wrote)
+        int r, c;
+        float u[8];
+        load_piece(i, r, c, u, false);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split2(u[2 * e] * scale, u[2 * e + 1] * scale, hi[e], lo[e]);
+        if (!tall) {   // (a piece's columns behind the matrix' end are zeros, as all that is not written)
+            put<true>(x + (c / kCols) * (int)kBlock + block_offset(r, c % kCols), hi, lo);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                char* const to = x + (r / kCols) * (int)kBlock + block_offset(c + e, r % kCols);
+                *reinterpret_cast<uint16_t*>(to) = (uint16_t)(hi[e / 2] >> (16 * (e & 1)));
+                *reinterpret_cast<uint16_t*>(to + kPlane) = (uint16_t)(lo[e / 2] >> (16 * (e & 1)));
+            }
+        }
     }
 
     // ---- products ----
@@ -623,10 +633,13 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     };
     constexpr uint32_t kNext = kBlock / 16;
     const uint32_t x0 = operand_low(smem_u32(x), 16), x0_across = operand_low(smem_u32(x), kBlock), ab0 = operand_low(smem_u32(ab), 16),
-                   v0 = operand_low(smem_u32(v), 16), square = instruction(false, 128, 128), across = instruction(true, 128, 128);
+                   v0 = operand_low(smem_u32(v), 16), square = instruction(false, 128, mk * kCols);
+    const int share = mk * 32, col = half * share;       // columns of A and B that each half of the warps finishes
+    char* const at_ab = ab + (col / kCols) * (int)kBlock;
+    const int on = row < m.m ? row - col : -256;         // the diagonal among them
     for (int step = 0; step < sp.count; ++step) {
         const bool cubic = sp.cubic >> step & 1;
-        float f[128];   // 64 of A or B, or 128 of X
+        float f[128];   // of A or B, or of X
 #pragma unroll
         for (int c = 0; c < 64; ++c) f[c] = 0.0f;
         for (int k = 0; k < nk; k += 2, ++phase) {   // A = X X^T, two blocks a round
@@ -635,75 +648,73 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
             if (tid == 0 && !(t.hooks.hold == (int)blockIdx.x && phase == 0))   // (a test: the first products never come)
                 issue(blocks, x0 + k * kNext, kNext, x0 + k * kNext, kNext, 2, square, k == 0);
             wait_done();
-            if (half < mk) {
 #pragma unroll
-                for (int c = 0; c < 64; c += 32) {
-                    take(f + c, half * 64 + c);
-                    if (blocks > 1) take(f + c, 128 + half * 64 + c);
-                    if (k + 2 >= nk) take(f + c, 256 + half * 64 + c);
-                }
+            for (int c = 0; c < 64; c += 32) {
+                if (c >= share) continue;
+                take(f + c, col + c);
+                if (blocks > 1) take(f + c, 128 + col + c);
+                if (k + 2 >= nk) take(f + c, 256 + col + c);
             }
         }
-        const int on = row < m.m ? row - half * 64 : -1;   // diagonal
-        if (half < mk) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 8) {
-                uint32_t hi[4], lo[4];
-                const uint32_t at = half * kBlock + block_offset(row, c);
-                finish(f + c, sp.gram[step], sp.gram_shift[step], cubic ? on - c : -1, hi, lo);
-                put<true>(ab + at, hi, lo);
-                if (!cubic) {
-                    finish(f + c, sp.gram[step], sp.gram_shift[step], on - c, hi, lo);
-                    put<true>(v + at, hi, lo);
-                }
-            }
+        for (int c = 0; c < 64; c += 8) {
+            if (c >= share) continue;
+            uint32_t hi[4], lo[4];
+            const uint32_t at = block_offset(row, col % kCols + c);
+            finish(f + c, sp.gram[step], sp.gram_shift[step], cubic ? on - c : -1, hi, lo);
+            put<true>(at_ab + at, hi, lo);
+            if (cubic) continue;
+            if ((unsigned)(on - c) < 8u) finish(f + c, sp.gram[step], sp.gram_shift[step], on - c, hi, lo);
+            put<true>(at_ab + mk * (int)kBlock + at, hi, lo);   // V
         }
         if (!cubic) {
             next_phase();   // B = a I + c A V
             if (tid == 0) issue(mk, ab0, kNext, v0, kNext, 2, square, true);
             wait_done();
-            if (half < mk) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) f[c] = 0.0f;
+            for (int c = 0; c < 64; ++c) f[c] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 64; c += 32) {
-                    take(f + c, half * 64 + c);
-                    if (mk > 1) take(f + c, 128 + half * 64 + c);
-                    take(f + c, 256 + half * 64 + c);
-                }
+            for (int c = 0; c < 64; c += 32) {
+                if (c >= share) continue;
+                take(f + c, col + c);
+                if (mk > 1) take(f + c, 128 + col + c);
+                take(f + c, 256 + col + c);
+            }
 #pragma unroll
-                for (int c = 0; c < 64; c += 8) {
-                    uint32_t hi[4], lo[4];
-                    finish(f + c, sp.square[step], sp.square_shift[step], on - c, hi, lo);
-                    put<true>(ab + half * (int)kBlock + block_offset(row, c), hi, lo);
-                }
+            for (int c = 0; c < 64; c += 8) {
+                if (c >= share) continue;
+                uint32_t hi[4], lo[4];
+                finish(f + c, sp.square[step], sp.square_shift[step], on - c, hi, lo);
+                put<true>(at_ab + block_offset(row, col % kCols + c), hi, lo);
             }
             ++phase;
         }
 #pragma unroll
         for (int c = 0; c < 128; ++c) f[c] = 0.0f;
-        for (int w = 0; w < tiles; ++w, ++phase) {   // X <- B X, a tile of 128 columns a round; each half of the warps takes one
-            next_phase();
-            if (tid == 0)   // (columns behind X's last block take what lies there, and are not kept)
-                issue(mk, ab0, kNext, x0_across + w * 2 * kNext, (kPlane / 2) / 16, 2048 / 16, across, true);
-            wait_done();
-            if (half == w) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    take(f + c, c);
-                    if (mk > 1) take(f + c, 128 + c);
-                    take(f + c, 256 + c);
+        for (int w = 0; w < 2; ++w) {   // X <- B X, two blocks a round, one for each half of the warps
+            if (w >= tiles) continue;
+            next_phase();
+            if (tid == 0)
+                issue(mk, ab0, kNext, x0_across + w * 2 * kNext, (kPlane / 2) / 16, 2048 / 16, instruction(true, 128, min(2, nk - 2 * w) * kCols), true);
+            wait_done();
+            if (2 * w + half < nk) {
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    take(f + w * 64 + c, half * 64 + c);
+                    if (mk > 1) take(f + w * 64 + c, 128 + half * 64 + c);
+                    take(f + w * 64 + c, 256 + half * 64 + c);
                 }
             }
+            ++phase;
         }
-        if (half < tiles) {   // every product has read X by now
 #pragma unroll
-            for (int c = 0; c < 128; c += 8) {
-                if (2 * half + c / kCols >= nk) continue;
-                uint32_t hi[4], lo[4];
-                finish(f + c, sp.apply[step], 0.0f, -1, hi, lo);
-                put<true>(x + (2 * half + c / kCols) * (int)kBlock + block_offset(row, c % kCols), hi, lo);
-            }
+        for (int c = 0; c < 128; c += 8) {   // every product has read X by now
+            const int block = c / 64 * 2 + half;
+            if (block >= nk) continue;
+            uint32_t hi[4], lo[4];
+            finish(f + c, sp.apply[step], 0.0f, -1, hi, lo);
+            put<true>(x + block * (int)kBlock + block_offset(row, c % kCols), hi, lo);
         }
     }
     if (tid == 0) {   // whatever was issued has ended before TMEM is handed back
@@ -715,13 +726,16 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
 
     // ---- result ----
     const bool failed = s_failed != 0;
-#pragma unroll 4
-    for (int i = tid; i < count; i += kTinyThreads) {
-        const int r = i / m.cols, c = i - r * m.cols, xr = tall ? c : r, xc = tall ? r : c;
-        const char* const at = x + (xc / kCols) * (int)kBlock + block_offset(xr, xc % kCols);
-        float v = (__half2float(*reinterpret_cast<const __half*>(at)) + __half2float(*reinterpret_cast<const __half*>(at + kPlane))) * sp.last;
-        if (failed) v = __int_as_float(0x7fffffff);
-        write_result(t, m, i, v);
+    for (int i = tid; i < pieces; i += kTinyThreads) {
+        const int r = i / per_row, c = (i - r * per_row) * 8, n = min(8, m.cols - c);
+        float u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int xr = tall ? c + e : r, xc = tall ? r : c + e;
+            const char* const at = x + (xc / kCols) * (int)kBlock + block_offset(xr, xc % kCols);   // (in X, up to its last block's end)
+            u[e] = __half2float(*reinterpret_cast<const __half*>(at)) + __half2float(*reinterpret_cast<const __half*>(at + kPlane));
+        }
+        write_result8(t, m, r * m.cols + c, access.state, n, u, sp.last, failed);
     }
 }
 

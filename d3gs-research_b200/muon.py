@@ -32,8 +32,7 @@ def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib
         raise ValueError(f"{what}: eps must be finite and positive, got {eps}")
     cfg = _lib.OrthoConfig()
     cfg.dtype, cfg.steps, cfg.eps = dtype, steps, eps
-    for k, c in enumerate(coefficients):
-        cfg.coefficients[k][:] = c
+    C.memmove(cfg.coefficients, (C.c_float * (3 * steps))(*[v for c in coefficients for v in c]), 12 * steps)
     return cfg
 
 

@@ -26,5 +26,6 @@ def __getattr__(name):
         "create_origin_3dgs_optimizers": "tools", "SplatTrainer": "trainer",
     }
     if name in table:
-        return getattr(importlib.import_module(f"{__name__}.{table[name]}"), name)
+        value = globals()[name] = getattr(importlib.import_module(f"{__name__}.{table[name]}"), name)
+        return value
     raise AttributeError(name)

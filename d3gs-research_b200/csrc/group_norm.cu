@@ -31,6 +31,7 @@ constexpr int kUnroll = 8, kUnroll2 = 4;
 constexpr int kCtas = 2, kCtas2 = 2;
 constexpr int kMaxChannels = 16384;       // per-channel sums of one CTA stay in shared memory
 constexpr int64_t kTurnBytes = 72 << 20;  // inputs of one turn, to be found in L2 (126 MB) by the second pass
+constexpr int64_t kSmallBytes = 128 << 10;
 constexpr int kJoinThreads = 256, kMaxChunks = 1024;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2 };
@@ -228,12 +229,8 @@ template <typename T, int V> __device__ __forceinline__ void store_some(T* p, co
 // Squares are taken around the mean k of the thread's first rows: when k is far from the mean of the rest, the rows
 // that k came from are themselves far from it and the variance is at least kUnroll/n of that distance squared, so
 // the cancellation in q - s^2/n costs at most n/kUnroll units of the last place, whatever the mean.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a) {
-    extern __shared__ float sh[];
-    let_next_start();
-    wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
+// out(group, mean, m2) takes the result; sh: three floats for every entry.
+template <typename T, int V, typename Out> __device__ __forceinline__ void chunk_stats(const Args& a, int b, int chunk, float* sh, Out out) {
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const int slots = (a.P <= kThreads ? kThreads / a.P : 1) * a.L;   // entries of the CTA: [row][value of the row]
     float *s_n = sh, *s_mean = sh + slots, *s_m2 = sh + 2 * slots;
@@ -361,9 +358,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a)
             }
         });
         m2 = lanes_sum(m2);
-        if (lane == 0 && g0 + (int)threadIdx.x / lanes < a.G)
-            reinterpret_cast<float2*>(a.part)[((int64_t)b * a.G + g) * a.chunks + chunk] = make_float2(mean, m2);
+        if (lane == 0 && g0 + (int)threadIdx.x / lanes < a.G) out(g, mean, m2);
     }
+}
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, kCtas) gn_stats_kernel(const Args a) {
+    extern __shared__ float sh[];
+    let_next_start();
+    wait_for_previous();
+    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
+    chunk_stats<T, V>(a, b, chunk, sh, [&](int g, float mean, float m2) {
+        reinterpret_cast<float2*>(a.part)[((int64_t)b * a.G + g) * a.chunks + chunk] = make_float2(mean, m2);
+    });
 }
 
 // values of one group in one chunk
@@ -372,6 +378,18 @@ __device__ __forceinline__ float chunk_count(const Args& a, int chunk) {
     int64_t e = (int64_t)n * a.tile_rows * a.L;
     if (chunk + (n - 1) * a.chunks == a.tiles - 1) e -= (int64_t)a.tiles * a.tile_rows * a.L - a.elems;   // the last tile
     return (float)e * a.share;
+}
+
+// u = k x + q of a channel; q is rounded at the size of mean rstd, as mean itself is
+__device__ __forceinline__ float2 forward_coef(const Args& a, int ch, float2 st) {
+    const float k = st.y * (a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f);
+    return make_float2(k, fmaf(-st.x, k, a.bias ? load_param(a.bias, a.wdtype, ch) : 0.0f));
+}
+// and dx = k du + kx x + kc, with the group's means of w du and of w du xhat
+__device__ __forceinline__ float4 backward_coef(const Args& a, int ch, float2 st, float m1, float m2) {
+    const float2 f = forward_coef(a, ch, st);
+    const float kx = -st.y * st.y * m2;
+    return make_float4(f.x, f.y, kx, fmaf(-st.x, kx, -st.y * m1));
 }
 
 // ---- forward, join: one CTA per (image, group) over the chunks ----------------------------------------------------
@@ -418,11 +436,8 @@ __global__ void __launch_bounds__(kJoinThreads) gn_stats_join_kernel(const Args 
     const float rstd = 1.0f / sqrtf(m2 / total + a.eps);
     if (threadIdx.x == 0) reinterpret_cast<float2*>(a.stats)[bg] = make_float2(mean, rstd);
     const int first = (int)(bg % a.G) * a.cpg;
-    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads) {
-        const float k = rstd * (a.weight ? load_param(a.weight, a.wdtype, first + i) : 1.0f);
-        reinterpret_cast<float2*>(a.coef)[bg * a.cpg + i] =
-            make_float2(k, fmaf(-mean, k, a.bias ? load_param(a.bias, a.wdtype, first + i) : 0.0f));
-    }
+    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads)
+        reinterpret_cast<float2*>(a.coef)[bg * a.cpg + i] = forward_coef(a, first + i, make_float2(mean, rstd));
 }
 
 // channel of value j of a vector
@@ -432,11 +447,8 @@ template <int V> __device__ __forceinline__ int channel(const Args& a, int vec, 
 }
 
 // ---- forward, pass 2 -----------------------------------------------------------------------------------------------
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a) {
-    let_next_start();
-    wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
+// c: k and q of the image's channels
+template <typename T, int V, int ACT> __device__ __forceinline__ void chunk_apply(const Args& a, int b, int chunk, const float2* c) {
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     T* y = static_cast<T*>(a.y) + b * a.y_batch;
     for (int v0 = 0; v0 < a.P; v0 += kThreads) {
@@ -444,10 +456,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a)
         if (!w.on) continue;
         const int vec = v0 + (a.P <= kThreads ? (int)threadIdx.x % a.P : (int)threadIdx.x);
         constexpr int H = (V + 1) / 2;
-        Two k[H], q[H];   // u = k x + q; q is rounded at the size of mean rstd, as mean itself is
+        Two k[H], q[H];
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            const float2* c = reinterpret_cast<const float2*>(a.coef) + (int64_t)b * a.C;
             const float2 c0 = c[channel<V>(a, vec, 2 * i)], c1 = c[channel<V>(a, vec, 2 * i + 1)];
             k[i] = two(c0.x, c1.x);
             q[i] = two(c0.y, c1.y);
@@ -480,13 +491,39 @@ __global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a)
     }
 }
 
-// ---- backward, pass 1: sum of du and of du xhat per channel over one chunk ----------------------------------------
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Args a) {
-    extern __shared__ float sh[];
+__global__ void __launch_bounds__(kThreads, kCtas) gn_apply_kernel(const Args a) {
     let_next_start();
     wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
+    const int b = a.first + blockIdx.y;
+    chunk_apply<T, V, ACT>(a, b, blockIdx.x, reinterpret_cast<const float2*>(a.coef) + (int64_t)b * a.C);
+}
+
+// ---- forward of a small image: both passes in one CTA ---------------------------------------------------------------
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, kCtas) gn_small_kernel(const Args a) {
+    extern __shared__ float sh[];   // k and q of every channel, mean and rstd of every group, entries
+    let_next_start();
+    wait_for_previous();
+    const int b = blockIdx.x;
+    float2* const coef = reinterpret_cast<float2*>(sh);
+    float2* const stats = coef + a.C;
+    const float total = (float)a.elems * a.share;
+    chunk_stats<T, V>(a, b, 0, sh + 2 * (a.C + a.G), [&](int g, float mean, float m2) {
+        const float2 st = make_float2(mean, 1.0f / sqrtf(m2 / total + a.eps));
+        stats[g] = st;
+        reinterpret_cast<float2*>(a.stats)[(int64_t)b * a.G + g] = st;
+    });
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < a.C; ch += kThreads) coef[ch] = forward_coef(a, ch, stats[ch / a.cpg]);
+    __syncthreads();
+    chunk_apply<T, V, ACT>(a, b, 0, coef);
+}
+
+// ---- backward, pass 1: sum of du and of du xhat per channel over one chunk ----------------------------------------
+// out(channel, sums) takes the result; sh: two floats for every entry.
+template <typename T, int V, int ACT, typename Out>
+__device__ __forceinline__ void chunk_grad_sums(const Args& a, int b, int chunk, float* sh, Out out) {
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch;
     const int slots = (a.P <= kThreads ? kThreads / a.P : 1) * a.L;
@@ -553,19 +590,27 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Ar
         }
     }
     __syncthreads();
-    float2* out = reinterpret_cast<float2*>(a.part) + ((int64_t)b * a.chunks + chunk) * a.C;
     for (int ch = threadIdx.x; ch < a.C; ch += kThreads) {
         float t1 = 0.0f, t2 = 0.0f;
         for (int e = ch; e < slots; e += a.C) {
             t1 += s_1[e];
             t2 += s_2[e];
         }
-        out[ch] = make_float2(t1, t2);
+        out(ch, make_float2(t1, t2));
     }
+}
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_sums_kernel(const Args a) {
+    extern __shared__ float sh[];
+    let_next_start();
+    wait_for_previous();
+    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
+    float2* const part = reinterpret_cast<float2*>(a.part) + ((int64_t)b * a.chunks + chunk) * a.C;
+    chunk_grad_sums<T, V, ACT>(a, b, chunk, sh, [&](int ch, float2 t) { part[ch] = t; });
 }
 
 // ---- backward, join: one CTA per (image, group): the sums of its channels over the chunks, the group's means, and the
-// coefficients of the second pass: u = k x + q, dx = k du + kx x + kc ------------------------------------------------
+// coefficients of the second pass ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(kJoinThreads) gn_grad_join_kernel(const Args a) {
     __shared__ float2 sh[kJoinThreads];
     __shared__ float sw[2][kJoinThreads / 32];
@@ -612,33 +657,24 @@ __global__ void __launch_bounds__(kJoinThreads) gn_grad_join_kernel(const Args a
     m1 = cta_sum(m1, sw[0]) * inv;
     m2 = cta_sum(m2, sw[1]) * inv;
     const float2 st = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + g];
-    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads) {
-        const float k = st.y * (a.weight ? load_param(a.weight, a.wdtype, first + i) : 1.0f);
-        const float kx = -st.y * st.y * m2;
-        reinterpret_cast<float4*>(a.coef)[(int64_t)b * a.C + first + i] =
-            make_float4(k, fmaf(-st.x, k, a.bias ? load_param(a.bias, a.wdtype, first + i) : 0.0f), kx, fmaf(-st.x, kx, -st.y * m1));
-    }
+    for (int i = threadIdx.x; i < a.cpg; i += kJoinThreads)
+        reinterpret_cast<float4*>(a.coef)[(int64_t)b * a.C + first + i] = backward_coef(a, first + i, st, m1, m2);
 }
 
 // ---- backward, pass 2: dx, and (last turn) the parameter gradients ------------------------------------------------
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const Args a, int params) {
-    let_next_start();
-    wait_for_previous();
-    const int b = a.first + blockIdx.y, chunk = blockIdx.x;
-    const float2* sums = reinterpret_cast<const float2*>(a.sums);
-    if (params && blockIdx.y == 0)   // every CTA of one image takes a share of the channels
-        for (int ch = blockIdx.x * kThreads + threadIdx.x; ch < a.C; ch += gridDim.x * kThreads) {
-            float t1 = 0.0f, t2 = 0.0f;
-            for (int k = 0; k < a.batch; ++k) {
-                const float2 s = sums[(int64_t)k * a.C + ch];
-                t1 += s.x;
-                t2 += s.y;
-            }
-            if (a.dweight) store_param(a.dweight, a.wdtype, ch, t2);
-            if (a.dbias) store_param(a.dbias, a.wdtype, ch, t1);
-        }
-    if (!a.y) return;
+// the parameter gradients of channel ch: over all images
+__device__ __forceinline__ void param_grads(const Args& a, int ch) {
+    const float2* sums = reinterpret_cast<const float2*>(a.sums) + ch;
+    float t1 = 0.0f, t2 = 0.0f;
+    for (int k = 0; k < a.batch; ++k) {
+        const float2 s = sums[(int64_t)k * a.C];
+        t1 += s.x;
+        t2 += s.y;
+    }
+    if (a.dweight) store_param(a.dweight, a.wdtype, ch, t2);
+    if (a.dbias) store_param(a.dbias, a.wdtype, ch, t1);
+}
+template <typename T, int V, int ACT> __device__ __forceinline__ void chunk_grad_apply(const Args& a, int b, int chunk, const float4* c) {
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch;
     const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch;
     T* dx = static_cast<T*>(a.y) + b * a.y_batch;
@@ -650,7 +686,6 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const A
         Two k[H], q[H], kx[H], kc[H];
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            const float4* c = reinterpret_cast<const float4*>(a.coef) + (int64_t)b * a.C;
             const float4 c0 = c[channel<V>(a, vec, 2 * i)], c1 = c[channel<V>(a, vec, 2 * i + 1)];
             k[i] = two(c0.x, c1.x);
             q[i] = two(c0.y, c1.y);
@@ -692,6 +727,67 @@ __global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const A
     }
 }
 
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, kCtas2) gn_grad_apply_kernel(const Args a, int params) {
+    let_next_start();
+    wait_for_previous();
+    const int b = a.first + blockIdx.y;
+    if (params && blockIdx.y == 0)   // every CTA of one image takes a share of the channels
+        for (int ch = blockIdx.x * kThreads + threadIdx.x; ch < a.C; ch += gridDim.x * kThreads) param_grads(a, ch);
+    if (a.y) chunk_grad_apply<T, V, ACT>(a, b, blockIdx.x, reinterpret_cast<const float4*>(a.coef) + (int64_t)b * a.C);
+}
+
+// ---- backward of a small image: both passes in one CTA; the parameter gradients of several images in another launch ---
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads, kCtas2) gn_small_grad_kernel(const Args a) {
+    extern __shared__ float4 sh4[];   // coefficients of every channel, its sums, means of every group, entries
+    let_next_start();
+    wait_for_previous();
+    const int b = blockIdx.x;
+    float4* const coef = sh4;
+    float2* const sums = reinterpret_cast<float2*>(coef + a.C);
+    float2* const means = sums + a.C;
+    chunk_grad_sums<T, V, ACT>(a, b, 0, reinterpret_cast<float*>(means + a.G), [&](int ch, float2 t) {
+        sums[ch] = t;
+        reinterpret_cast<float2*>(a.sums)[(int64_t)b * a.C + ch] = t;
+        if (a.batch == 1) {
+            if (a.dweight) store_param(a.dweight, a.wdtype, ch, t.y);
+            if (a.dbias) store_param(a.dbias, a.wdtype, ch, t.x);
+        }
+    });
+    if (!a.y) return;
+    __syncthreads();
+    const float inv = 1.0f / ((float)a.elems * a.share);
+    for (int g = threadIdx.x >> 5; g < a.G; g += kThreads / 32) {
+        float m1 = 0.0f, m2 = 0.0f;
+        for (int i = threadIdx.x & 31; i < a.cpg; i += 32) {
+            const int ch = g * a.cpg + i;
+            const float w = a.weight ? load_param(a.weight, a.wdtype, ch) : 1.0f;
+            m1 = fmaf(w, sums[ch].x, m1);
+            m2 = fmaf(w, sums[ch].y, m2);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            m1 += __shfl_xor_sync(~0u, m1, o);
+            m2 += __shfl_xor_sync(~0u, m2, o);
+        }
+        if ((threadIdx.x & 31) == 0) means[g] = make_float2(m1 * inv, m2 * inv);
+    }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < a.C; ch += kThreads) {
+        const int g = ch / a.cpg;
+        coef[ch] = backward_coef(a, ch, reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.G + g], means[g].x, means[g].y);
+    }
+    __syncthreads();
+    chunk_grad_apply<T, V, ACT>(a, b, 0, coef);
+}
+__global__ void __launch_bounds__(kThreads) gn_params_kernel(const Args a) {
+    let_next_start();
+    wait_for_previous();
+    const int ch = blockIdx.x * kThreads + threadIdx.x;
+    if (ch < a.C) param_grads(a, ch);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------
 int gcd(int64_t a, int64_t b) {
     while (b) {
@@ -727,6 +823,12 @@ int images_per_turn(const D3gsGroupNorm& d, bool backward) {
     int64_t n = kTurnBytes / (image > 0 ? image : 1);
     if (n > d.batch) n = d.batch;
     return (int)(n < 1 ? 1 : n);
+}
+
+// One CTA per image and one launch (two in the backward of a batch): an image of this size takes a CTA about a microsecond a
+// pass, a launch more takes longer.  (Many channels would not leave its shared memory room.)
+bool small_image(const D3gsGroupNorm& d) {
+    return d.pixels * d.channels * elem_size(d.dtype) <= kSmallBytes && d.channels <= 2048;
 }
 
 // Chunks of one image: as many CTAs in a turn as run at once (a CTA without a tile is not launched).
@@ -817,6 +919,10 @@ template <typename T, int V, int ACT>
 int32_t run_forward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, false);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
+    if (small_image(d)) {
+        a.chunks = 1;
+        return launch(gn_small_kernel<T, V, ACT>, "gn_small_kernel", dim3(a.batch), kThreads, slots * 12 + (a.C + a.G) * 8, st, a);
+    }
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;
@@ -832,6 +938,14 @@ template <typename T, int V, int ACT>
 int32_t run_backward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, true);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
+    if (small_image(d)) {
+        a.chunks = 1;
+        if (int32_t rc = launch(gn_small_grad_kernel<T, V, ACT>, "gn_small_grad_kernel", dim3(a.batch), kThreads,
+                                slots * 8 + (size_t)a.C * 24 + a.G * 8, st, a))
+            return rc;
+        if (a.batch == 1 || !(a.dweight || a.dbias)) return D3GS_OK;
+        return launch(gn_params_kernel, "gn_params_kernel", dim3((a.C + kThreads - 1) / kThreads), kThreads, 0, st, a);
+    }
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;

@@ -8,7 +8,7 @@
 // Both directions are bound by memory: the statistics of a group need all of an image before its first output, so
 // x (and dy) is read twice and the result written once.  Images are handled in turns small enough for the second
 // read to come from L2 (see images_per_turn).  Three launches per turn: partial sums per chunk of an image, their
-// join, and the pass that writes.  Sums are joined in a fixed order, so results do not change from run to run.
+// join, and the pass that writes; one launch for small images, a CTA each (see one_cta).  Sums are joined in a fixed order, so results do not change from run to run.
 //
 // Layout of the work: a thread owns V neighbouring values (16 bytes where alignment allows) of a "row" and walks
 // down the rows, so that its V channels never change.  A row is one pixel when V divides C; where it does not and
@@ -31,7 +31,7 @@ constexpr int kUnroll = 8, kUnroll2 = 4;
 constexpr int kCtas = 2, kCtas2 = 2;
 constexpr int kMaxChannels = 16384;       // per-channel sums of one CTA stay in shared memory
 constexpr int64_t kTurnBytes = 72 << 20;  // inputs of one turn, to be found in L2 (126 MB) by the second pass
-constexpr int64_t kSmallBytes = 128 << 10;
+constexpr int kSmall = 4096, kSmallGrad = 2048, kSmallMany = 32768;   // vectors of an image, see one_cta()
 constexpr int kJoinThreads = 256, kMaxChunks = 1024;
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2 };
@@ -817,18 +817,24 @@ int pick_vector(const D3gsGroupNorm& d, const void* x, const void* dy, const voi
     return 1;
 }
 
-// Images per turn: as many as keep the turn's inputs within kTurnBytes, at least one.
+// Images per turn: as many as keep the turn's inputs within kTurnBytes, at least one, and the turns about equal.
 int images_per_turn(const D3gsGroupNorm& d, bool backward) {
     const int64_t image = d.pixels * d.channels * elem_size(d.dtype) * (backward ? 2 : 1);
     int64_t n = kTurnBytes / (image > 0 ? image : 1);
-    if (n > d.batch) n = d.batch;
-    return (int)(n < 1 ? 1 : n);
+    if (n < 1) n = 1;
+    return d.batch ? (int)div_up64(d.batch, div_up64(d.batch, n)) : 1;
 }
 
-// One CTA per image and one launch (two in the backward of a batch): an image of this size takes a CTA about a microsecond a
-// pass, a launch more takes longer.  (Many channels would not leave its shared memory room.)
-bool small_image(const D3gsGroupNorm& d) {
-    return d.pixels * d.channels * elem_size(d.dtype) <= kSmallBytes && d.channels <= 2048;
+// An image by one CTA, both passes in one launch (the backward of a batch takes one more), or every image by many CTAs
+// with a join between the passes: one CTA is slower with the image, a launch is not.  Measured with 64 channels, many
+// CTAs -> one, us: forward of a float32 image of 16 KB 15 -> 12, 64 KB 15 -> 12, 128 KB 15 -> 15 (bf16 17 -> 18), 256 KB
+// 16 -> 19; backward 16 KB 13 -> 10, 32 KB 13 -> 10 (16 images of bf16 17 -> 17), 64 KB 13 -> 12 (bf16 17 -> 18, 16
+// images 17 -> 22), 128 KB 13 -> 17.  Where there is an image for every SM one CTA also finds its image in L2 again:
+// 200 images of 16 KB 22 -> 14 and 24 -> 22, of 512 KB 80 -> 59 and 130 -> 110.  (Many channels would leave a CTA no
+// shared memory for their coefficients.)
+bool one_cta(const D3gsGroupNorm& d, const Args& a, bool backward) {
+    const int64_t vectors = a.elems / (a.L / a.P);   // what a thread loads at a time, 16 bytes in the figures above
+    return d.channels <= 2048 && vectors <= (d.batch >= 148 ? kSmallMany : backward ? kSmallGrad : kSmall);
 }
 
 // Chunks of one image: as many CTAs in a turn as run at once (a CTA without a tile is not launched).
@@ -919,7 +925,7 @@ template <typename T, int V, int ACT>
 int32_t run_forward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, false);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
-    if (small_image(d)) {
+    if (one_cta(d, a, false)) {
         a.chunks = 1;
         return launch(gn_small_kernel<T, V, ACT>, "gn_small_kernel", dim3(a.batch), kThreads, slots * 12 + (a.C + a.G) * 8, st, a);
     }
@@ -938,7 +944,7 @@ template <typename T, int V, int ACT>
 int32_t run_backward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, true);
     const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
-    if (small_image(d)) {
+    if (one_cta(d, a, true)) {
         a.chunks = 1;
         if (int32_t rc = launch(gn_small_grad_kernel<T, V, ACT>, "gn_small_grad_kernel", dim3(a.batch), kThreads,
                                 slots * 8 + (size_t)a.C * 24 + a.G * 8, st, a))

@@ -106,9 +106,16 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return (*_backward(ctx.desc, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
+        # the wrapper that refuses a second derivative takes the host 14 us, as long as the kernels of a small image
+        return (_differentiable_once if torch.is_grad_enabled() else _gradients)(ctx, dy)
+
+
+def _gradients(ctx, dy):
+    return (*_backward(ctx.desc, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
+
+
+_differentiable_once = torch.autograd.function.once_differentiable(_gradients)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,

@@ -119,6 +119,12 @@ CASES = [
     ((2, 200, 301, 32), 8, BF16, F32, "silu"),       # many chunks, a ragged last one
     ((2, 201, 301, 3), 3, F32, F32, "gelu"),         # colour images: instance normalisation
     ((5, 401, 399, 32), 1, F16, F32, "silu"),        # several turns of images
+    ((2, 25, 30, 64), 8, F32, F32, "silu"),          # a forward in one launch, a backward in three
+    ((3, 20, 40, 80), 5, BF16, BF16, "gelu"),        # one launch for either, parameter gradients in another
+    ((1, 3, 2, 2048), 32, BF16, F32, "silu"),        # the most channels that a CTA takes alone
+    ((1, 3, 2, 2056), 257, BF16, F32, "silu"),       # and one vector more
+    ((150, 31, 33, 64), 8, BF16, F32, "silu"),       # an image for every SM
+    ((150, 9, 11, 7), 7, F16, F32, "gelu"),          # the same, odd
 ]
 
 
@@ -291,6 +297,24 @@ def test_captured_and_replayed(cuda_device):
         torch.cuda.synchronize()
         for graph, leaves, dy, out, step in made:
             assert all(torch.equal(p, q) for p, q in zip(out, step()))
+
+
+@pytest.mark.parametrize("size", [4, 64])
+def test_first_gradients_of_a_graph_that_is_kept(cuda_device, size):
+    """create_graph gives the same gradients; a second derivative is refused, not wrong."""
+    x, dy, w, b = make((2, size, size, 8), 2, F32, F32)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = group_norm_act(leaves[0], 2, leaves[1], leaves[2])
+    plain = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    kept = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    assert all(torch.equal(p, k) for p, k in zip(plain, kept))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(kept[0].sum(), leaves[0])
+
+
+def test_most_images(cuda_device):
+    x, dy, w, b = make((65535, 2, 3), 3, F32, F32)
+    check(x, dy, w, b, 3, "silu")
 
 
 def test_refusals_on_the_device(cuda_device):

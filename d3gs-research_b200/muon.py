@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from bisect import bisect_left
 from typing import Sequence
 
 import torch
@@ -112,12 +113,13 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
 
     A parameter of more than two axes (a convolution's filters) is taken as ``[size(0), the rest]``.  ``ratio`` is
     ``sqrt(max(1, rows / columns))``, or with ``adjust_lr_fn="match_rms_adamw"`` ``0.2 sqrt(max(rows, columns))``.
-    Parameters and buffers must be dense (contiguous or channels last) and must not overlap one another."""
+    Parameters and buffers must be dense (contiguous or channels last) and must not overlap one another or a gradient."""
     params, grads, momentum_buffers = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} params, {len(grads)} grads, {len(momentum_buffers)} momentum_buffers")
     if adjust_lr_fn not in _ADJUST:
         raise ValueError(f"muon_step: adjust_lr_fn must be one of {_ADJUST}, got {adjust_lr_fn!r}")
+    lr, weight_decay, momentum = float(lr), float(weight_decay), float(momentum)
     for name, v in (("lr", lr), ("weight_decay", weight_decay)):
         if not 0.0 <= v < float("inf"):
             raise ValueError(f"muon_step: {name} must be finite and not negative, got {v}")
@@ -126,7 +128,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     cfg = _config("muon_step", 0, ns_coefficients, eps, ns_steps)
     cfg.momentum, cfg.decay, cfg.nesterov = momentum, 1.0 - lr * weight_decay, int(nesterov)
     mats = (_lib.OrthoMatrix * max(len(params), 1))()
-    keep, spans, count, device = [], [], 0, None
+    keep, spans, read, count, device = [], [], [], 0, None
     for p, g, buf in zip(params, grads, momentum_buffers):
         if not (p.is_cuda and p.dtype == g.dtype == buf.dtype == torch.float32 and p.dim() >= 2 and g.device == p.device
                 and buf.device == p.device and g.shape == p.shape == buf.shape and g.layout == torch.strided):
@@ -154,12 +156,19 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         at, state, size = p.data_ptr(), buf.data_ptr(), rows * cols * 4
         mats[count] = (g.data_ptr(), state, at, rows, cols, row_stride, _adjusted_lr(lr, rows, cols, adjust_lr_fn), 0)
         spans += [(state, state + size), (at, at + size)]
+        first = g.data_ptr()
+        read.append((first, first + ((rows - 1) * row_stride + cols) * 4))
         count += 1
     if count == 0:
         return
     spans.sort()
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("muon_step: parameters or buffers overlap (is one given twice?)")
+    ends = [end for _, end in spans]
+    for first, last in read:
+        k = bisect_left(ends, first + 1)   # the first span that ends behind the gradient's start
+        if k < len(spans) and spans[k][0] < last:
+            raise ValueError("muon_step: a gradient overlaps a parameter or a buffer")
     _run("d3gs_muon_step", mats, count, cfg, device)
     torch.autograd.graph.increment_version([*params, *momentum_buffers])
 

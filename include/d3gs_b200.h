@@ -556,7 +556,7 @@ int32_t d3gs_group_norm_backward(const D3gsGroupNorm* desc, const void* x, const
  *   d3gs_muon_step: momentum = mu momentum + (1 - mu) src;  U = nesterov ? mu momentum + (1 - mu) src : momentum;
  *                   dst = decay dst - rate X   (src the gradient, dst the parameter, all 32 bits)
  * A list of matrices of any sizes shares the launches.  src: rows lie src_row_stride values apart, columns are dense;
- * dst and momentum are dense.  No matrix's dst or momentum may overlap another's.  Short side at most 16384, long side
+ * dst and momentum are dense.  No matrix's dst or momentum may overlap another's, nor another's src.  Short side at most 16384, long side
  * at most 2^24, below 2^31 values.  An empty matrix is left alone; one of zeros gives zeros.  Refused are coefficients
  * with which singular values in [0, 1] grow past 1024, or with 0 < 1024 |c| < |b|. */
 #define D3GS_NS_MAX_STEPS 32

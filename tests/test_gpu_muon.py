@@ -304,6 +304,14 @@ def test_refusals(cuda_device):
                      (([a[:, :3]], [b[:, :3]], [c[:, :3]]), {}), (([a], [b.T], [c]), {})):
         with pytest.raises(ValueError, match="muon_step"):
             muon_step(*args, **{"lr": 0.1, **kw})
+    # a gradient that shares memory with a parameter or a buffer, its own or another's, by one value or as a whole
+    flat = torch.zeros(100, device="cuda")
+    p, q, s, r = (flat[24 * k:24 * k + 24].view(4, 6) for k in range(4))
+    for args in (([p], [p], [q]), ([p], [q], [q]), ([p, s], [a, s], [b, c]), ([p, a], [b, flat[23:47].view(4, 6)], [r, c]),
+                 ([q], [flat[1:25].view(4, 6)], [s]), ([p], [flat[18:].as_strided((4, 6), (20, 1))], [s])):
+        with pytest.raises(ValueError, match="gradient overlaps"):
+            muon_step(*args, lr=0.1)
+    muon_step([p, r], [q, q], [s, a], lr=0.1)          # neighbours, and one gradient for two parameters
     with pytest.raises(ValueError, match="GaussianMuon"):
         GaussianMuon([torch.nn.Parameter(torch.zeros(3, device="cuda"))])
     with pytest.raises(RuntimeError, match="singular values grow"):

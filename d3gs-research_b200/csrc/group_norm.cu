@@ -854,6 +854,8 @@ int32_t check(const D3gsGroupNorm* d, const char* what) {
     D3GS_REQUIRE(d->dtype >= 0 && d->dtype <= 2 && d->weight_dtype >= 0 && d->weight_dtype <= 2, "%s: dtype %d / %d", what,
                  d->dtype, d->weight_dtype);
     D3GS_REQUIRE(d->act >= 0 && d->act <= 2, "%s: act %d", what, d->act);
+    D3GS_REQUIRE(d->x_batch_stride >= 0 && d->x_pixel_stride >= 0 && d->dy_batch_stride >= 0 && d->dy_pixel_stride >= 0,
+                 "%s: strides must not be negative", what);
     D3GS_REQUIRE(d->eps >= 0.0f, "%s: eps must not be negative", what);
     return D3GS_OK;
 }

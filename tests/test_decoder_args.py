@@ -19,6 +19,7 @@ def gn_desc(**kw):
 @pytest.mark.parametrize("field,value,word", [("groups", 3, "divide"), ("groups", 0, "divide"), ("channels", 0, "channels"),
                                               ("channels", 16385, "channels"), ("batch", 65536, "batch"), ("batch", -1, "batch"),
                                               ("dtype", 3, "dtype"), ("weight_dtype", -1, "dtype"), ("act", 3, "act"),
+                                              ("x_pixel_stride", -8, "strides"), ("dy_batch_stride", -1, "strides"),
                                               ("eps", -1.0, "eps"), ("eps", float("nan"), "eps")])
 def test_group_norm_descriptor(field, value, word):
     lib = _lib.load()

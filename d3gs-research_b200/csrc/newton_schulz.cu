@@ -16,7 +16,7 @@
 // hold every entry that matters.  One fp16 value keeps 11 bits, two of them, v = hi + lo, keep 22.
 //  * 32-bit matrices: all operands hi + lo, three products hi hi + hi lo + lo hi; the dropped lo lo is of the size of
 //    the last bit.  (Two bf16 values would hold 16 bits only, and three of them need six products.)
-//  * 16-bit matrices: A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
+//  * 16-bit matrices (large ones, see planes_of): A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
 //    and B lose turns X's singular directions by that much and no more.  What X loses is noise in all directions alike,
 //    and the next steps amplify it where X is small: with one value the result is 4e-3 off at 512 x 512 and 6e-3 at
 //    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.
@@ -53,7 +53,7 @@ struct Matrix {
     char* v;              // V's blocks on the diagonal: two for each block of rows
     double* norms;        // sums of squares of the norm pass
     int32_t rows, cols;
-    int32_t m, n;         // short and long side
+    int32_t m;            // short side
     int32_t mb, mk, nk;   // blocks: rows of all three, columns of A and B, columns of X
     float rate;
 };
@@ -453,8 +453,8 @@ __device__ __forceinline__ uint32_t instruction(bool across, uint32_t rows, uint
 // column block of A and B hold anything: nothing sums over them, and no valid row or column reads them.
 enum { kGram = 0, kSquare = 1, kApply = 2 };
 
-// What the products of a mode of large matrices read: planes of the left and the right factor and of the result, and how many planes lie
-// between blocks of A and B.  RIGHT is 1 in the last step of 16-bit matrices.
+// What the products of a mode of large matrices read: planes of the left and the right factor and of the result, and how
+// many planes lie between blocks of A and B.  RIGHT is 1 in the last step of 16-bit matrices.
 template <bool F32, int MODE, int RIGHT> struct Planes {
     static constexpr int kLeft = F32 ? 2 : 1;
     static constexpr int kRight = RIGHT;
@@ -494,7 +494,7 @@ template <bool TWO> __device__ __forceinline__ void write_mirrored(char* block, 
 
 // ---- tiny matrices: the whole chain in one CTA --------------------------------------------------------------------
 // Where X, A and V fit into shared memory together (sides of at most 128 and 256, seven blocks in all) they stay there from
-// the first step to the last, and a matrix costs one launch instead of seventeen.  What takes time is the way from a
+// the first step to the last, and a matrix costs one launch instead of eighteen.  What takes time is the way from a
 // product to its epilogue and back, three of each a step.  Sums of hi hi are taken out after every block (after every
 // second one the result of a 128 x 128 matrix was 2.4e-6 off instead of 1.6e-6).
 constexpr int kTinyThreads = 256, kTinyBlocks = 7, kTinyCols = 256;
@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     }
     if (warp == 0) tmem_alloc<1>(&s_tmem, columns);
     for (int i = tid; i < nk * (int)kBlock / 16; i += kTinyThreads) reinterpret_cast<uint4*>(x)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();   // no CTA of the next kernel takes an SM before this one has its TMEM
     let_next_start();
     wait_for_previous();
 
@@ -1454,7 +1455,6 @@ void next_table(Table& t, const D3gsOrthoMatrix* mats, int32_t count, int32_t& i
         m.rows = (int32_t)d.rows;
         m.cols = (int32_t)d.cols;
         m.m = p.m;
-        m.n = p.n;
         m.mb = p.mb;
         m.mk = p.mk;
         m.nk = p.nk;

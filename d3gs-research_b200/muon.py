@@ -8,7 +8,9 @@ parameters in a handful of launches, ``GaussianMuon`` the optimizer around it.  
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
+import struct
 from bisect import bisect_left
 from typing import Sequence
 
@@ -19,21 +21,27 @@ from . import _lib
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib.OrthoConfig:
+@functools.lru_cache(maxsize=64)
+def _coefficients(what: str, coefficients: tuple, steps: int):
+    """a, b, c of every step as the library takes them."""
     if not 1 <= steps <= _lib.NS_MAX_STEPS:
         raise ValueError(f"{what}: ns_steps must be 1 to {_lib.NS_MAX_STEPS}, got {steps}")
-    coefficients = list(coefficients)
-    if len(coefficients) == 3 and not isinstance(coefficients[0], (tuple, list)):
-        coefficients = [coefficients] * steps
+    if len(coefficients) == 3 and not isinstance(coefficients[0], tuple):
+        coefficients = (coefficients,) * steps
     if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
         raise ValueError(f"{what}: ns_coefficients must be (a, b, c), or one such triple for each of {steps} steps")
     if not all(math.isfinite(v) for c in coefficients for v in c):
         raise ValueError(f"{what}: ns_coefficients must be finite")
+    return (C.c_float * (3 * steps))(*[v for c in coefficients for v in c])
+
+
+def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib.OrthoConfig:
+    values = _coefficients(what, tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), int(steps))
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"{what}: eps must be finite and positive, got {eps}")
     cfg = _lib.OrthoConfig()
     cfg.dtype, cfg.steps, cfg.eps = dtype, steps, eps
-    C.memmove(cfg.coefficients, (C.c_float * (3 * steps))(*[v for c in coefficients for v in c]), 12 * steps)
+    C.memmove(cfg.coefficients, values, C.sizeof(values))
     return cfg
 
 
@@ -97,6 +105,8 @@ def _adjusted_lr(lr: float, rows: int, cols: int, adjust_lr_fn: str | None) -> f
     return lr * math.sqrt(max(1.0, rows / cols))
 
 
+_MATRIX = struct.Struct("PPPqqqfi")   # OrthoMatrix; a struct filled through ctypes takes three times as long
+assert _MATRIX.size == C.sizeof(_lib.OrthoMatrix)
 _ADJUST = (None, "original", "match_rms_adamw")
 
 
@@ -127,37 +137,41 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         raise ValueError(f"muon_step: momentum must be in [0, 1), got {momentum}")
     cfg = _config("muon_step", 0, ns_coefficients, eps, ns_steps)
     cfg.momentum, cfg.decay, cfg.nesterov = momentum, 1.0 - lr * weight_decay, int(nesterov)
-    mats = (_lib.OrthoMatrix * max(len(params), 1))()
-    keep, spans, read, count, device = [], [], [], 0, None
+    table = bytearray(C.sizeof(_lib.OrthoMatrix) * len(params))
+    keep, spans, read, count, device, f32 = [], [], [], 0, None, torch.float32
     for p, g, buf in zip(params, grads, momentum_buffers):
-        if not (p.is_cuda and p.dtype == g.dtype == buf.dtype == torch.float32 and p.dim() >= 2 and g.device == p.device
-                and buf.device == p.device and g.shape == p.shape == buf.shape and g.layout == torch.strided):
+        at_device, shape = p.device, p.shape
+        if not (p.is_cuda and p.dtype is f32 and g.dtype is f32 and buf.dtype is f32 and len(shape) >= 2
+                and g.device == at_device and buf.device == at_device and g.shape == shape and buf.shape == shape
+                and g.layout is torch.strided):
             raise ValueError("muon_step: params, grads and momentum_buffers must be float32 CUDA tensors of two or more axes "
                              f"with equal shapes and devices, got {tuple(p.shape)} {p.dtype} {p.device}, {tuple(g.shape)} "
                              f"{g.dtype} {g.device}, {tuple(buf.shape)} {buf.dtype} {buf.device}")
         if device is None:
-            device = p.device
-        if p.device != device:
+            device = at_device
+        if at_device != device:
             raise ValueError(f"muon_step: parameters on {device} and {p.device} in one call")
-        if p.numel() == 0:
+        size = p.numel()
+        if size == 0:
             continue
         plain = p.is_contiguous()
         if not (plain and buf.is_contiguous()) and (not _dense_rows(p) or not _same_order(p, buf)):
             raise ValueError(f"muon_step: a parameter of strides {p.stride()} or its buffer of strides {buf.stride()} is not "
                              "dense (contiguous or channels last, the two alike)")
-        rows, cols = p.shape[0], p.numel() // p.shape[0]
-        row_stride = cols
+        rows = shape[0]
+        row_stride = cols = size // rows
         if not (plain and g.is_contiguous()) and not _same_order(p, g):
-            if g.dim() == 2 and (cols == 1 or g.stride(1) == 1) and p.is_contiguous():
+            if g.dim() == 2 and (cols == 1 or g.stride(1) == 1) and plain:
                 row_stride = g.stride(0)
             else:
                 g = torch.empty_like(p).copy_(g)
                 keep.append(g)
-        at, state, size = p.data_ptr(), buf.data_ptr(), rows * cols * 4
-        mats[count] = (g.data_ptr(), state, at, rows, cols, row_stride, _adjusted_lr(lr, rows, cols, adjust_lr_fn), 0)
-        spans += [(state, state + size), (at, at + size)]
-        first = g.data_ptr()
-        read.append((first, first + ((rows - 1) * row_stride + cols) * 4))
+        src, state, at, size = g.data_ptr(), buf.data_ptr(), p.data_ptr(), 4 * size
+        _MATRIX.pack_into(table, count * _MATRIX.size, src, state, at, rows, cols, row_stride,
+                          _adjusted_lr(lr, rows, cols, adjust_lr_fn), 0)
+        spans.append((state, state + size))
+        spans.append((at, at + size))
+        read.append((src, src + ((rows - 1) * row_stride + cols) * 4))
         count += 1
     if count == 0:
         return
@@ -169,7 +183,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         k = bisect_left(ends, first + 1)   # the first span that ends behind the gradient's start
         if k < len(spans) and spans[k][0] < last:
             raise ValueError("muon_step: a gradient overlaps a parameter or a buffer")
-    _run("d3gs_muon_step", mats, count, cfg, device)
+    _run("d3gs_muon_step", (_lib.OrthoMatrix * len(params)).from_buffer(table), count, cfg, device)
     torch.autograd.graph.increment_version([*params, *momentum_buffers])
 
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -15,6 +16,8 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"none": 0, "silu": 1, "gelu": 2}
+_DESC = struct.Struct("6q5if")   # GroupNorm; filled through ctypes it takes the host twice as long
+assert _DESC.size == C.sizeof(_lib.GroupNorm)
 
 
 def _pixel_strides(t: torch.Tensor):
@@ -49,40 +52,45 @@ def _prepared(t: torch.Tensor):
     return t, strides
 
 
-def _workspace(lib, d: _lib.GroupNorm, backward: int, device):
+def _workspace_bytes(lib, d, backward: int) -> int:
     n = lib.d3gs_group_norm_workspace_bytes(C.byref(d), backward)
     if n == 0:
         raise RuntimeError(f"d3gs_group_norm_workspace_bytes: {_lib.last_error()}")
-    return torch.empty(n, dtype=torch.uint8, device=device), n
+    return n
 
 
-def _forward(x, groups, weight, bias, eps, act):
+def _forward(x, groups, weight, bias, eps, act, keep: bool):
+    """The input as it was read, the result, and for the backward (``keep``) the statistics and the arguments."""
     device = x.device
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _forward(x, groups, weight, bias, eps, act)
+            return _forward(x, groups, weight, bias, eps, act, keep)
     lib = _lib.load()
     x, (image, pixel) = _prepared(x)
     shape = x.shape
+    batch = shape[0]
     wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    d = _lib.GroupNorm(shape[0], math.prod(shape[1:-1]), image, pixel, 0, 0, shape[-1], groups, _DTYPES[x.dtype],
-                       _DTYPES[wdtype], act, eps)
+    args = bytearray(_DESC.pack(batch, math.prod(shape[1:-1]), image, pixel, 0, 0, shape[-1], groups, _DTYPES[x.dtype],
+                                _DTYPES[wdtype], act, eps))
+    d = _lib.GroupNorm.from_buffer(args)
     y = torch.empty(shape, dtype=x.dtype, device=device)
-    stats = torch.empty((shape[0], groups, 2), dtype=torch.float32, device=device)
-    ws, n = _workspace(lib, d, 0, device)
+    n = _workspace_bytes(lib, d, 0)
+    ws = torch.empty(n if keep else n + batch * groups * 8, dtype=torch.uint8, device=device)
+    at = ws.data_ptr()
+    stats = torch.empty((batch, groups, 2), dtype=torch.float32, device=device) if keep else None
     _lib.check(lib.d3gs_group_norm_forward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), y.data_ptr(),
-                                           stats.data_ptr(), ws.data_ptr(), n, _lib.raw_stream(device.index)),
+                                           stats.data_ptr() if keep else at + n, at, n, _lib.raw_stream(device.index)),
                "d3gs_group_norm_forward")
-    return x, y, stats, d
+    return x, y, stats, args
 
 
-def _backward(d, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b: bool):
+def _backward(args, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b: bool):
     device = x.device
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _backward(d, x, weight, bias, stats, dy, need_x, need_w, need_b)
+            return _backward(args, x, weight, bias, stats, dy, need_x, need_w, need_b)
     lib = _lib.load()
-    d = _lib.GroupNorm.from_buffer_copy(d)
+    d = _lib.GroupNorm.from_buffer_copy(args)
     dy, (d.dy_batch_stride, d.dy_pixel_stride) = _prepared(dy)
     empty = x.numel() == 0
     dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
@@ -90,7 +98,8 @@ def _backward(d, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b:
     dw = make(weight) if need_w else None
     db = make(bias) if need_b else None
     if not empty and (need_x or need_w or need_b):
-        ws, n = _workspace(lib, d, 1, device)
+        n = _workspace_bytes(lib, d, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
         _lib.check(lib.d3gs_group_norm_backward(C.byref(d), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias),
                                                 stats.data_ptr(), dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
                                                 _lib.ptr(db), ws.data_ptr(), n, _lib.raw_stream(device.index)),
@@ -101,7 +110,7 @@ def _backward(d, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b:
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups: int, eps: float, act: int):
-        x, y, stats, ctx.desc = _forward(x.detach(), groups, weight, bias, eps, act)
+        x, y, stats, ctx.args = _forward(x.detach(), groups, weight, bias, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
         return y
 
@@ -112,7 +121,7 @@ class _GroupNormAct(torch.autograd.Function):
 
 
 def _gradients(ctx, dy):
-    return (*_backward(ctx.desc, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
+    return (*_backward(ctx.args, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
 
 
 _differentiable_once = torch.autograd.function.once_differentiable(_gradients)
@@ -138,8 +147,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     num_groups = int(num_groups)
     if num_groups < 1 or c < 1 or c % num_groups:
         raise ValueError(f"group_norm_act: {num_groups} groups do not divide {c} channels")
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"group_norm_act: eps must be finite and not negative, got {eps}")
+    if not 0.0 <= eps <= 1e30:
+        raise ValueError(f"group_norm_act: eps must be in [0, 1e30], got {eps}")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.dim() != 1 or t.shape[0] != c or t.device != x.device or t.dtype not in _DTYPES):
             raise ValueError(f"group_norm_act: {name} must be [{c}] on {x.device} in float32, bfloat16 or float16, got "
@@ -151,4 +160,4 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNormAct.apply(x, weight, bias, num_groups, float(eps), _ACTS[act])
-    return _forward(x, num_groups, weight, bias, float(eps), _ACTS[act])[1]
+    return _forward(x, num_groups, weight, bias, float(eps), _ACTS[act], False)[1]

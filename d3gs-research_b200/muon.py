@@ -131,8 +131,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         raise ValueError(f"muon_step: adjust_lr_fn must be one of {_ADJUST}, got {adjust_lr_fn!r}")
     lr, weight_decay, momentum = float(lr), float(weight_decay), float(momentum)
     for name, v in (("lr", lr), ("weight_decay", weight_decay)):
-        if not 0.0 <= v < float("inf"):
-            raise ValueError(f"muon_step: {name} must be finite and not negative, got {v}")
+        if not 0.0 <= v <= 1e30:
+            raise ValueError(f"muon_step: {name} must be in [0, 1e30], got {v}")
     if not 0.0 <= momentum < 1.0:
         raise ValueError(f"muon_step: momentum must be in [0, 1), got {momentum}")
     cfg = _config("muon_step", 0, ns_coefficients, eps, ns_steps)

@@ -323,7 +323,7 @@ def test_refusals_on_the_device(cuda_device):
     for bad in (lambda: group_norm_act(x, 3, w), lambda: group_norm_act(x, 0, w), lambda: group_norm_act(x, 2, w[:4]),
                 lambda: group_norm_act(x, 2, w.double()), lambda: group_norm_act(x.double(), 2, w),
                 lambda: group_norm_act(x, 2, w.cpu()), lambda: group_norm_act(x, 2, w, w.half()),
-                lambda: group_norm_act(x, 2, w, act="relu"), lambda: group_norm_act(x, 2, w, eps=-1.0),
+                lambda: group_norm_act(x, 2, w, act="relu"), lambda: group_norm_act(x, 2, w, eps=-1.0), lambda: group_norm_act(x, 2, w, eps=1e300),
                 lambda: group_norm_act(x, 2, w, eps=float("nan")), lambda: group_norm_act(x[0, 0, 0], 2, w)):
         with pytest.raises(ValueError, match="group_norm_act"):
             bad()

@@ -297,7 +297,7 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError, match="orthogonalize"):
             bad()
     a, b, c = (torch.zeros(4, 6, device="cuda") for _ in range(3))
-    for args, kw in ((([a], [b], []), {}), (([a], [b], [c]), {"momentum": 1.0}), (([a], [b], [c]), {"lr": -1.0}),
+    for args, kw in ((([a], [b], []), {}), (([a], [b], [c]), {"momentum": 1.0}), (([a], [b], [c]), {"lr": -1.0}), (([a], [b], [c]), {"lr": 1e300}),
                      (([a], [b], [c]), {"adjust_lr_fn": "x"}), (([a, a], [b, b], [c, c.clone()]), {}),
                      (([a, b], [b, b], [c, c]), {}), (([a], [b], [a]), {}), (([a[0]], [b[0]], [c[0]]), {}),
                      (([a.T], [b.T], [c.T]), {}), (([a], [b.half()], [c]), {}), (([a], [b.cpu()], [c]), {}),

@@ -8,7 +8,12 @@
 // Both directions are bound by memory: the statistics of a group need all of an image before its first output, so
 // x (and dy) is read twice and the result written once.  Images are handled in turns small enough for the second
 // read to come from L2 (see images_per_turn).  Three launches per turn: partial sums per chunk of an image, their
-// join, and the pass that writes; one launch for small images, a CTA each (see one_cta).  Sums are joined in a fixed order, so results do not change from run to run.
+// join, and the pass that writes; one launch for small images, a CTA each (see one_cta).  Sums are joined in a fixed
+// order, so results do not change from run to run.
+//
+// Measured: 1080p x 32 channels in fp16, forward 88 us (133 MB read twice, the second time partly from L2, and written; a
+// copy of that size takes 44 us, a plain read 30).  Forward and backward of 4 x 1080p x 32 in bf16 867 us, 4.9 TB/s with
+// the second reads, which miss L2 there; of 8 x 135 x 240 x 256 in fp16 263 us, the second reads from L2.
 //
 // Layout of the work: a thread owns V neighbouring values (16 bytes where alignment allows) of a "row" and walks
 // down the rows, so that its V channels never change.  A row is one pixel when V divides C; where it does not and

@@ -495,7 +495,8 @@ template <bool TWO> __device__ __forceinline__ void write_mirrored(char* block, 
 // ---- tiny matrices: the whole chain in one CTA --------------------------------------------------------------------
 // Where X, A and V fit into shared memory together (sides of at most 128 and 256, seven blocks in all) they stay there from
 // the first step to the last, and a matrix costs one launch instead of eighteen.  What takes time is the way from a
-// product to its epilogue and back, three of each a step.  Sums of hi hi are taken out after every block (after every
+// product to its epilogue and back, three of each a step: 64 x 64 takes 25 us, 1.6 us a product (the launches of larger
+// matrices 82 us); 128 x 128 48 us (110), thirty of 128 x 192 64 us (121).  Sums of hi hi are taken out after every block (after every
 // second one the result of a 128 x 128 matrix was 2.4e-6 off instead of 1.6e-6).
 constexpr int kTinyThreads = 256, kTinyBlocks = 7, kTinyCols = 256;
 
@@ -741,8 +742,12 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
 }
 
 // ---- small matrices: one 128 x 128 tile a cluster, its CTAs share the summed axis ---------------------------------
-// With few tiles the summed axis is what takes time: the CTAs of a cluster (1, 2, 4 or 8) each sum a part of it, put
-// their sums into shared memory and each finish a part of the columns, adding the parts in the order of their ranks.
+// With few tiles the summed axis is what takes time, the long one of X X^T: there the CTAs of a cluster (1, 2, 4 or 8)
+// each sum a part of it, put their sums into shared memory and each finish a part of the columns, adding the parts in the
+// order of their ranks.  The other products sum over at most kPairFrom / 64 = 6 blocks, in one CTA.
+// Nine convolution layers of 3 to 256 rows take 165 us, eighteen launches of 9 us with the tensor cores busy for 5 to 7 %:
+// what bounds them is one launch after another, each a wait for the last one's memory, a fill of the stages, the way out
+// through TMEM and shared memory.
 constexpr int kSmallThreads = 320, kTile = 128;
 struct SmallStages {
     static constexpr uint32_t kLeft = 2 * kPlane, kRight = 2 * kPlane, kStage = kLeft + kRight;
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     __shared__ uint32_t s_tmem;
     char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int parts = (int)cluster_size(), part = (int)cluster_rank();
+    const int parts = MODE == kGram ? (int)cluster_size() : 1, part = MODE == kGram ? (int)cluster_rank() : 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kCount; ++i) {
             mbar_init(&s_full[i], 1);
@@ -977,11 +982,16 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
 // than its 128 bytes a cycle.  In a pair each CTA holds 128 rows of the left and N / 2 columns of the right factor, and
 // both are read by the products of both: at N = 256, 8 KB in 128 cycles.  CTA 0 issues; CTA 1's second warp passes on
 // that its tiles have arrived.
+//
+// Measured: 4096 x 4096 in 16 bits 1.5 to 1.8 ms a call of five steps, 0.90 to 0.77 PFLOP/s, with X's second plane counted
+// 1.26 to 1.07, near what the power limit leaves a plain product; tensor cores busy for 69 % of B X, 56 % of the others
+// (1.84 rounds of tiles on 74 pairs).  2048 x 2048 in 32 bits 0.52 to 0.58 ms: busy for 58 % of B X in 256-wide tiles, 38 %
+// of the others in 128-wide ones, which an SM takes 48 KB in for every 768 cycles of products.
 constexpr int kPairThreads = 320;
 template <int L, int R, int N> struct PairStages {
     static constexpr uint32_t kLeft = L * kPlane, kRight = R * (uint32_t)N / 2 * 128, kStage = kLeft + kRight;
     // A commit takes the issuing thread about 400 cycles.  Where a column block is 256 or 512 cycles of products one
-    // commit hands back two stages.
+    // commit hands back two stages (one -> two: 2048 x 2048 305 -> 300 us, 4096 x 4096 1715 -> 1698).
     static constexpr int kGroup = L == 1 && R == 1 ? 2 : 1;
     static constexpr int kCount = (int)(196608u / kStage) / kGroup * kGroup;
     static constexpr uint32_t kBytes = kCount * kStage + 1024;
@@ -1287,7 +1297,8 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
 }
-// How the products of a list of matrices are cut: pairs of CTAs when the largest short side is above kPairFrom.
+// How the products of a list of matrices are cut: pairs of CTAs when the largest short side is above kPairFrom.  (Pairs
+// from 257 on instead: 320 x 320 155 us either way, 384 x 384 171 instead of 167, 384 x 3456 335 instead of 176.)
 constexpr int kPairFrom = 384;
 bool large(const D3gsOrthoMatrix* mats, int32_t count) {
     for (int32_t i = 0; i < count; ++i)
@@ -1407,16 +1418,21 @@ template <int MODE, typename B> int32_t small_product(const Table& t, B& blocks,
     const unsigned tiles = blocks([](const Matrix& m) {
         return MODE == kApply ? (int64_t)m.mb * ((m.nk + 1) / 2) : (int64_t)m.mb * (m.mb + 1) / 2;
     });
-    // as many CTAs a tile as the machine has room for, none without four blocks to sum
-    int longest = 0;
-    for (int k = 0; k < t.count; ++k) longest = max(longest, MODE == kGram ? t.mat[k].nk : t.mat[k].mk);
+    // X X^T: as many CTAs a tile as the machine has room for, none without four blocks to sum (one CTA a tile -> this:
+    // 256 x 2304 250 -> 146 us, 64 x 1152 143 -> 104, 384 x 512 170 -> 156)
     unsigned parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
+    if (MODE == kGram) {
+        int longest = 0;
+        for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);
+        while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
+    }
     return launch(ns_small_kernel<MODE>, "ns_small_kernel", tiles * parts, kSmallThreads, SmallStages::kBytes, parts, st, t);
 }
 template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const Table& t, B& blocks, cudaStream_t st) {
     constexpr int L = Planes<F32, MODE, RIGHT>::kLeft;
-    // 256 x 256 tiles move the least; 256 x 128 ones when those would leave SMs idle
+    // 256 x 256 tiles move the least; 256 x 128 ones when those would leave SMs idle.  (256-wide from 40 CTAs on -> 100:
+    // 2048 x 2048 719 -> 522 us, 8 x 2048 x 512 in 16 bits 314 -> 275; from 160 on -> 100: 2560 x 2560 1188 -> 1063 us,
+    // 2048 x 2048 600 -> 522.)
     const unsigned tiles = blocks([](const Matrix& m) {
         const int64_t pairs = (m.mb + 1) / 2;
         return MODE == kApply ? pairs * ((m.nk + 3) / 4) : pairs * (pairs + 1) / 2;

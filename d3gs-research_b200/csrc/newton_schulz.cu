@@ -42,6 +42,8 @@ constexpr int kPieces = 1024;       // pieces of eight neighbouring columns per 
 constexpr int kMaxShort = 16384, kMaxLong = 1 << 24;
 constexpr int kRows = 128, kCols = 64;                 // one block
 constexpr uint32_t kPlane = kRows * kCols * 2;         // bytes of one fp16 plane of a block
+constexpr int kTickets = 148;                          // of shared tiles: one for every CTA at most
+constexpr size_t kSumBytes = 128 * 256 * 4;            // of a CTA of a shared tile
 constexpr float kMaxSpectrum = 1024.0f;                // largest singular value the scales leave room for
 
 struct Matrix {
@@ -69,6 +71,9 @@ struct Table {
     float shift;          // added on the diagonal of V or B
     int32_t cubic;        // c = 0: the first product gives B
     uint32_t* fail;       // set when a bounded wait ran out: the last pass then writes NaN
+    int32_t parts;        // how many pairs of CTAs share the sum of a tile
+    uint32_t* tickets;    // how many of them have put their sums down: for both halves of every tile, zero between products
+    float4* sums;         // those sums
     TestHooks hooks;
 };
 
@@ -150,6 +155,7 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
     let_next_start();
     wait_for_previous();
     if (blockIdx.x == 0 && threadIdx.x == 0) *t.fail = 0;
+    if (blockIdx.x == 0 && threadIdx.x < kTickets) t.tickets[threadIdx.x] = 0;
     double sum = 0.0;
     float u[kPieces / kThreads][8], buf[kPieces / kThreads][8];
 #pragma unroll
@@ -997,7 +1003,8 @@ template <int L, int R, int N> struct PairStages {
     static constexpr uint32_t kBytes = kCount * kStage + 1024;
 };
 
-template <bool F32, int MODE, int RIGHT, int N>
+// SHARED: several pairs share the sum of a tile.
+template <bool F32, int MODE, int RIGHT, int N, bool SHARED = false>
 __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_constant__ Table t) {
     using P = Planes<F32, MODE, RIGHT>;
     constexpr int L = P::kLeft, R = P::kRight, kWide = N / kCols;   // column blocks of the tile
@@ -1030,7 +1037,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = s_tmem, polls = t.hooks.poll_limit;
     int block;
-    const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x / 2, block)];
+    const int parts = SHARED ? t.parts : 1, tile = (int)blockIdx.x / 2 / parts, part = (int)blockIdx.x / 2 - tile * parts;
+    const Matrix& m = t.mat[find_matrix(t, tile, block)];
     const int pairs = (m.mb + 1) / 2;                   // 256-row tiles
     int ti, tj;
     if (MODE == kApply) {
@@ -1054,7 +1062,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     const char* const left = MODE == kGram ? m.x[t.from] : MODE == kSquare ? m.a : m.b;
     const char* const right = MODE == kSquare ? m.a : m.x[t.from];
     constexpr uint32_t kLeftBlock = MODE == kGram ? P::kX : P::kAB, kRightBlock = MODE == kSquare ? P::kAB : P::kX;
-    const int blocks = MODE == kGram ? m.nk : m.mk;
+    const int all = MODE == kGram ? m.nk : m.mk;         // column blocks summed over, this pair's share of them
+    const int first = all * part / parts, blocks = all * (part + 1) / parts - first;
     bool ok = true;
     let_next_start();
     wait_for_previous();
@@ -1078,26 +1087,27 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
                 if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
-                const bool shared = same && !(MODE == kSquare && k >> 2 == tj);
+                const int kb = first + k;
+                const bool shared = same && !(MODE == kSquare && kb >> 2 == tj);
                 mbar_arrive_expect_tx(&s_full[st], shared ? S::kLeft : S::kStage);
-                bulk_copy_g2s(a, left + ((int64_t)lrow * blocks + k) * kLeftBlock, S::kLeft, &s_full[st]);
+                bulk_copy_g2s(a, left + ((int64_t)lrow * all + kb) * kLeftBlock, S::kLeft, &s_full[st]);
                 if (MODE == kApply) {
                     for (int p = 0; p < R; ++p)
                         for (int w = 0; w < kWide / 2; ++w)                // 64 rows of a block: one half of a plane
                             bulk_copy_g2s(b + (p * (kWide / 2) + w) * (kPlane / 2),
-                                          right + ((int64_t)(k >> 1) * m.nk + min(kWide * tj + kWide / 2 * rank + w, m.nk - 1)) * kRightBlock +
-                                              p * kPlane + (k & 1) * (kPlane / 2),
+                                          right + ((int64_t)(kb >> 1) * m.nk + min(kWide * tj + kWide / 2 * rank + w, m.nk - 1)) * kRightBlock +
+                                              p * kPlane + (kb & 1) * (kPlane / 2),
                                           kPlane / 2, &s_full[st]);
                 } else if (N == 256) {
                     const int j = min(2 * tj + rank, m.mb - 1);
-                    const bool v = MODE == kSquare && k >> 1 == j;
+                    const bool v = MODE == kSquare && kb >> 1 == j;
                     if (!shared)
-                        bulk_copy_g2s(b, v ? m.v + (int64_t)k * kRightBlock : right + ((int64_t)j * blocks + k) * kRightBlock, S::kRight,
+                        bulk_copy_g2s(b, v ? m.v + (int64_t)kb * kRightBlock : right + ((int64_t)j * all + kb) * kRightBlock, S::kRight,
                                       &s_full[st]);
                 } else {
                     const int j = min(tj, m.mb - 1);
-                    const bool v = MODE == kSquare && k >> 1 == j;
-                    const char* from = v ? m.v + (int64_t)k * kRightBlock : right + ((int64_t)j * blocks + k) * kRightBlock;
+                    const bool v = MODE == kSquare && kb >> 1 == j;
+                    const char* from = v ? m.v + (int64_t)kb * kRightBlock : right + ((int64_t)j * all + kb) * kRightBlock;
                     for (int p = 0; p < R; ++p)
                         bulk_copy_g2s(b + p * (kPlane / 2), from + p * kPlane + rank * (kPlane / 2), kPlane / 2, &s_full[st]);
                 }
@@ -1119,7 +1129,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             const uint32_t a0 = operand_low(smem_u32(smem), 16), b0 = operand_low(smem_u32(smem) + S::kLeft, kNext);
             auto left_of = [&](int st) { return a0 + st * (S::kStage / 16); };
             auto right_of = [&](int k, int st) {
-                const bool shared = same && !(MODE == kSquare && k >> 2 == tj);
+                const bool shared = same && !(MODE == kSquare && (first + k) >> 2 == tj);
                 return shared ? left_of(st) : b0 + st * (S::kStage / 16);
             };
             auto rest = [&](int k, int st) {   // hi lo + lo hi
@@ -1190,8 +1200,40 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             }
         if (ok) ok = __all_sync(~0u, wait_for(&s_last, 0, polls));
         tc_fence_after();
-        if (ok) take(F32 ? kSums * N : 0);
+        if (ok && (!SHARED || blocks > 0)) take(F32 ? kSums * N : 0);
         if (!ok) *t.fail = 1;
+        // A tile that several pairs share: everyone puts its sums down, four columns of 128 rows after one another, the last
+        // one to do so adds them up in the order of the parts and goes on.
+        bool finishes = true;
+        if constexpr (SHARED) {
+            __shared__ uint32_t s_ticket;
+            float4* const sums = t.sums + (int64_t)(tile * 2 + rank) * parts * (kSumBytes / 16) + half * kPart * 32 + r;
+#pragma unroll
+            for (int c = 0; c < kPart; c += 4)
+                __stcg(sums + part * (int)(kSumBytes / 16) + c * 32, make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]));
+            __threadfence();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (threadIdx.x == 0) {
+                uint32_t* const ticket = t.tickets + tile * 2 + rank;
+                s_ticket = atomicAdd(ticket, 1u);
+                if (s_ticket == (uint32_t)parts - 1) *ticket = 0;   // for the next product
+                __threadfence();
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            finishes = s_ticket == (uint32_t)parts - 1;
+            if (finishes) {
+#pragma unroll
+                for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
+#pragma unroll 1
+                for (int q = 0; q < parts; ++q) {
+#pragma unroll
+                    for (int c = 0; c < kPart; c += 4) {
+                        const float4 w = __ldcg(sums + q * (int)(kSumBytes / 16) + c * 32);
+                        v[c] += w.x, v[c + 1] += w.y, v[c + 2] += w.z, v[c + 3] += w.w;
+                    }
+                }
+            }
+        }
         // Every product has read its operands by now: their shared memory takes the finished blocks, from where they
         // leave as whole blocks.
         const int wide = MODE == kApply ? m.nk : m.mk;   // blocks across the result
@@ -1252,7 +1294,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         };
         auto all_warps = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         const bool sender = ok && (threadIdx.x & 127) == 0 && row < m.mb;
-        if (kTurns) {
+        if (SHARED && !finishes) {
+        } else if (kTurns) {
             for (int turn = 0; turn < 2; ++turn) {
                 if (half == turn) write();
                 all_warps();
@@ -1319,8 +1362,10 @@ bool tiny(const D3gsOrthoMatrix* mats, int32_t count) {
 int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
     return cfg.dtype == D3GS_DTYPE_F32 || !large(mats, count) ? 2 : 1;
 }
+constexpr size_t kHead = 256 + 1024;   // the failure word, the tickets
+size_t shared_bytes(const D3gsOrthoMatrix* mats, int32_t count) { return large(mats, count) ? kTickets * kSumBytes : 0; }
 size_t workspace_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
-    size_t need = 512;   // alignment, the failure word
+    size_t need = 256 + kHead + shared_bytes(mats, count);   // (alignment)
     const int planes = planes_of(mats, count, cfg);
     for (int32_t i = 0; i < count; ++i) need += parts_of(mats[i], planes).total;
     return need;
@@ -1437,6 +1482,20 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
         const int64_t pairs = (m.mb + 1) / 2;
         return MODE == kApply ? pairs * ((m.nk + 3) / 4) : pairs * (pairs + 1) / 2;
     });
+    if constexpr (MODE == kGram) {
+        // Few tiles and a long axis: four or eight pairs a tile, with enough of the axis for each.  Two do not make up for
+        // the way of the sums through memory (10 us).  One pair a tile -> this: 512 x 4608 412 -> 361 us, 512 x 8192 625 ->
+        // 413, 512 x 32768 2154 -> 955, 1024 x 8192 826 -> 667; 512 x 8192 in 16 bits 317 -> 257.  (With two: 2048 x 4096
+        // 891 -> 939, 640 x 2304 313 -> 357.  With 16 blocks each in 16 bits: 1024 x 4096 267 -> 277.)
+        Table u = t;
+        int longest = 0;
+        for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);
+        u.parts = 8;
+        while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? 16 : 32))) u.parts /= 2;
+        if (u.parts >= 4)
+            return launch(ns_pair_kernel<F32, MODE, RIGHT, 256, true>, "ns_pair_kernel", tiles * u.parts * 2, kPairThreads,
+                          PairStages<L, RIGHT, 256>::kBytes, 2, st, u);
+    }
     if (tiles * 2 > 100)
         return launch(ns_pair_kernel<F32, MODE, RIGHT, 256>, "ns_pair_kernel", tiles * 2, kPairThreads,
                       PairStages<L, RIGHT, 256>::kBytes, 2, st, t);
@@ -1577,7 +1636,9 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
     Table t{};
     t.fail = reinterpret_cast<uint32_t*>(at);
-    at += 256;
+    t.tickets = reinterpret_cast<uint32_t*>(at + 256);
+    t.sums = reinterpret_cast<float4*>(at + kHead);
+    at += kHead + shared_bytes(mats, count);
     t.bf16 = cfg->dtype == D3GS_DTYPE_BF16;
     t.eps = cfg->eps;
     t.mu = cfg->momentum;

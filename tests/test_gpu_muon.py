@@ -82,7 +82,8 @@ def test_sizes(cuda_device, m, n, dtype):
     check(make(m, n, seed=m * 7 + n).to(dtype))
 
 
-@pytest.mark.parametrize("m,n,dtype", [(2048, 1500, F32), (1500, 2048, BF16), (96, 16384, F32), (4096, 256, BF16)])
+@pytest.mark.parametrize("m,n,dtype", [(2048, 1500, F32), (1500, 2048, BF16), (96, 16384, F32), (4096, 256, BF16),
+                                       (500, 8200, F32), (8200, 500, BF16), (1000, 4200, F32), (450, 20000, BF16)])
 def test_large_sizes(cuda_device, m, n, dtype):
     check(make(m, n).to(dtype))
 
@@ -209,6 +210,17 @@ def test_step_of_more_matrices_than_a_launch_takes(cuda_device):
     check_step(*tensors([(8 + k % 5, 16 + k) for k in range(70)]))
 
 
+def test_step_of_long_and_short_matrices(cuda_device):
+    """The long ones' sums over the long axis are shared among CTAs; the short ones in the same launch leave most of
+    those without a column block.  The same bits every time."""
+    shapes = [(512, 8192), (400, 30), (8200, 390), (3, 500)]
+    runs = [tensors(shapes) for _ in range(3)]
+    check_step(*runs[0])
+    for run in runs[1:]:
+        muon_step(*run, lr=0.02)
+        assert all(torch.equal(a, b) for a, b in zip(run[0], runs[0][0]))
+
+
 def test_step_layouts(cuda_device):
     """Channels-last filters, gradients of other strides than their parameter's."""
     params, grads, buffers = tensors([(32, 8, 3, 3), (40, 30), (40, 30), (16, 8, 1, 1)])
@@ -320,7 +332,7 @@ def test_refusals(cuda_device):
         orthogonalize(torch.empty(16385, 1, device="cuda").expand(16385, 16385))
 
 
-@pytest.mark.parametrize("m,n", [(50, 200), (200, 300), (500, 520)])
+@pytest.mark.parametrize("m,n", [(50, 200), (200, 300), (500, 520), (500, 8200)])
 def test_a_wait_that_gives_up_spoils_the_result_and_no_more(cuda_device, m, n):
     """One CTA of every product never asks for its first tile (nothing is in flight when its waits run out): the call
     returns, its result is NaN, and the next call is right."""

@@ -1484,14 +1484,15 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
     });
     if constexpr (MODE == kGram) {
         // Few tiles and a long axis: four or eight pairs a tile, with enough of the axis for each.  Two do not make up for
-        // the way of the sums through memory (10 us).  One pair a tile -> this: 512 x 4608 412 -> 361 us, 512 x 8192 625 ->
-        // 413, 512 x 32768 2154 -> 955, 1024 x 8192 826 -> 667; 512 x 8192 in 16 bits 317 -> 257.  (With two: 2048 x 4096
-        // 891 -> 939, 640 x 2304 313 -> 357.  With 16 blocks each in 16 bits: 1024 x 4096 267 -> 277.)
+        // the way of the sums through memory (10 us).  One pair a tile -> this: 512 x 3400 352 -> 332 us, 512 x 8192 628 ->
+        // 404, 512 x 32768 2162 -> 946, 1024 x 8192 829 -> 667; 512 x 6400 in 16 bits 294 -> 259.  (With two pairs: 2048 x
+        // 4096 891 -> 939.  With eight blocks each: 512 x 2048 278 -> 317, 1024 x 2304 357 -> 391; with 16 in 16 bits: 1024 x
+        // 4096 268 -> 275.)
         Table u = t;
         int longest = 0;
         for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);
         u.parts = 8;
-        while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? 16 : 32))) u.parts /= 2;
+        while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? 12 : 24))) u.parts /= 2;
         if (u.parts >= 4)
             return launch(ns_pair_kernel<F32, MODE, RIGHT, 256, true>, "ns_pair_kernel", tiles * u.parts * 2, kPairThreads,
                           PairStages<L, RIGHT, 256>::kBytes, 2, st, u);

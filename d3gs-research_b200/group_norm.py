@@ -7,7 +7,6 @@ reference has no counterpart.
 from __future__ import annotations
 
 import ctypes as C
-import math
 import struct
 
 import torch
@@ -68,10 +67,10 @@ def _forward(x, groups, weight, bias, eps, act, keep: bool):
     lib = _lib.load()
     x, (image, pixel) = _prepared(x)
     shape = x.shape
-    batch = shape[0]
+    batch, channels, values = shape[0], shape[-1], x.numel()
     wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    args = bytearray(_DESC.pack(batch, math.prod(shape[1:-1]), image, pixel, 0, 0, shape[-1], groups, _DTYPES[x.dtype],
-                                _DTYPES[wdtype], act, eps))
+    args = bytearray(_DESC.pack(batch, values // (batch * channels) if values else 0, image, pixel, 0, 0, channels, groups,
+                                _DTYPES[x.dtype], _DTYPES[wdtype], act, eps))
     d = _lib.GroupNorm.from_buffer(args)
     y = torch.empty(shape, dtype=x.dtype, device=device)
     n = _workspace_bytes(lib, d, 0)
@@ -109,8 +108,9 @@ def _backward(args, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups: int, eps: float, act: int):
-        x, y, stats, ctx.args = _forward(x.detach(), groups, weight, bias, eps, act, True)
+    def forward(ctx, x, weight, bias, how):   # how: groups, eps, act
+        groups, eps, act = how
+        x, y, stats, ctx.args = _forward(x, groups, weight, bias, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
         return y
 
@@ -121,7 +121,7 @@ class _GroupNormAct(torch.autograd.Function):
 
 
 def _gradients(ctx, dy):
-    return (*_backward(ctx.args, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None, None, None)
+    return (*_backward(ctx.args, *ctx.saved_tensors, dy, *ctx.needs_input_grad[:3]), None)
 
 
 _differentiable_once = torch.autograd.function.once_differentiable(_gradients)
@@ -159,5 +159,5 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     bias = None if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _GroupNormAct.apply(x, weight, bias, num_groups, float(eps), _ACTS[act])
+        return _GroupNormAct.apply(x, weight, bias, (num_groups, float(eps), _ACTS[act]))
     return _forward(x, num_groups, weight, bias, float(eps), _ACTS[act], False)[1]

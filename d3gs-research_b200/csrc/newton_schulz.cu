@@ -1363,7 +1363,13 @@ int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig&
     return cfg.dtype == D3GS_DTYPE_F32 || !large(mats, count) ? 2 : 1;
 }
 constexpr size_t kHead = 256 + 1024;   // the failure word, the tickets
-size_t shared_bytes(const D3gsOrthoMatrix* mats, int32_t count) { return large(mats, count) ? kTickets * kSumBytes : 0; }
+// Column blocks of a long axis that each of the pairs sharing a tile should have at least; twice that in 16 bits.
+constexpr int kShare = 12;
+size_t shared_bytes(const D3gsOrthoMatrix* mats, int32_t count) {
+    int64_t longest = 0;
+    for (int32_t i = 0; i < count; ++i) longest = max(longest, max(mats[i].rows, mats[i].cols));
+    return large(mats, count) && div_up64(longest, kCols) >= 4 * kShare ? kTickets * kSumBytes : 0;
+}
 size_t workspace_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
     size_t need = 256 + kHead + shared_bytes(mats, count);   // (alignment)
     const int planes = planes_of(mats, count, cfg);
@@ -1492,7 +1498,7 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
         int longest = 0;
         for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);
         u.parts = 8;
-        while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? 12 : 24))) u.parts /= 2;
+        while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? kShare : 2 * kShare))) u.parts /= 2;
         if (u.parts >= 4)
             return launch(ns_pair_kernel<F32, MODE, RIGHT, 256, true>, "ns_pair_kernel", tiles * u.parts * 2, kPairThreads,
                           PairStages<L, RIGHT, 256>::kBytes, 2, st, u);

@@ -36,7 +36,8 @@ def _coefficients(what: str, coefficients: tuple, steps: int):
 
 
 def _config(what: str, dtype: int, coefficients, eps: float, steps: int) -> _lib.OrthoConfig:
-    values = _coefficients(what, tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients), int(steps))
+    values = _coefficients(what, tuple([tuple(map(float, c)) if isinstance(c, (tuple, list)) else float(c) for c in coefficients]),
+                           int(steps))
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"{what}: eps must be finite and positive, got {eps}")
     cfg = _lib.OrthoConfig()

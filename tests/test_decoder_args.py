@@ -129,6 +129,17 @@ def test_ortho_workspace():
     assert lib.d3gs_orthogonalize(mats, 2, C.byref(cfg), 256, 1 << 20, None) == 0
 
 
+def test_coefficients_are_taken_by_value():
+    from d3gs_research_b200 import muon
+    a = torch.tensor(1.5)
+    first = muon._config("x", 0, (a, -0.5, 0.0), 1e-7, 2)
+    a.fill_(2.0)
+    second = muon._config("x", 0, [[a, -0.5, 0.0]] * 2, 1e-7, 2)
+    assert first.coefficients[0][0] == first.coefficients[1][0] == 1.5
+    assert second.coefficients[0][0] == second.coefficients[1][0] == 2.0
+    assert first.coefficients[0][1] == -0.5 and first.steps == 2
+
+
 def test_muon_needs_gpu_tensors():
     from d3gs_research_b200 import GaussianMuon, muon_step, orthogonalize
     u = torch.zeros(4, 6)

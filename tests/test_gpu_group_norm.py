@@ -150,8 +150,9 @@ def test_background_before_the_object(cuda_device):
     check(x, dy, w, b, 8, "silu")
 
 
-def test_only_weight_or_only_bias(cuda_device):
-    x, dy, w, b = make((2, 9, 11, 24), 3, F32, F32)
+@pytest.mark.parametrize("size", [9, 90])
+def test_only_weight_or_only_bias(cuda_device, size):
+    x, dy, w, b = make((2, size, 11, 24), 3, F32, F32)
     for ww, bb in ((w, None), (None, b)):
         leaf = (ww if ww is not None else bb).detach().requires_grad_()
         y = group_norm_act(x, 3, leaf if ww is not None else None, leaf if bb is not None else None, eps=EPS)
@@ -161,32 +162,34 @@ def test_only_weight_or_only_bias(cuda_device):
         within(g, r[4] if ww is not None else r[5], 1e-5 * (r[6] if ww is not None else r[7]), "gradient")
 
 
+# a CTA an image, and several
+@pytest.mark.parametrize("h,w", [(13, 10), (83, 60)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_strided_inputs(cuda_device, dtype):
+def test_strided_inputs(cuda_device, dtype, h, w):
     """A slice of the channels, a view of a channels-first tensor, every other column, one pixel for all."""
-    x, dy, w, b = make((2, 13, 10, 40), 4, dtype, F32)
-    base, _ = check(x, dy, w, b, 4, "silu")
-    wide = torch.zeros(2, 13, 10, 56, dtype=dtype, device="cuda")
+    x, dy, gamma, beta = make((2, h, w, 40), 4, dtype, F32)
+    base, _ = check(x, dy, gamma, beta, 4, "silu")
+    wide = torch.zeros(2, h, w, 56, dtype=dtype, device="cuda")
     wide[..., 8:48] = x
-    wide_dy = torch.zeros(2, 13, 10, 47, dtype=dtype, device="cuda")
+    wide_dy = torch.zeros(2, h, w, 47, dtype=dtype, device="cuda")
     wide_dy[..., 3:43] = dy
-    check(wide[..., 8:48], wide_dy[..., 3:43], w, b, 4, "silu")
-    check(wide[..., 5:45], dy, w, b, 4, "silu")
+    check(wide[..., 8:48], wide_dy[..., 3:43], gamma, beta, 4, "silu")
+    check(wide[..., 5:45], dy, gamma, beta, 4, "silu")
     nchw = x.permute(0, 3, 1, 2).contiguous()
-    y, _ = check(nchw.permute(0, 2, 3, 1), dy.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1), w, b, 4, "silu")
+    y, _ = check(nchw.permute(0, 2, 3, 1), dy.permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1), gamma, beta, 4, "silu")
     assert torch.equal(y, base)
-    check(x[:, :, ::2], dy[:, :, ::2], w, b, 4, "silu")
-    check(x[:, 1:, 1:], dy[:, 1:, 1:], w, b, 4, "silu")
-    check(x, dy[:, :1, :1].expand(x.shape), w, b, 4, "silu")
-    check(x[:1].expand(x.shape), dy, w, b, 4, "silu")
-    nhwc = torch.empty(2, 40, 13, 10, device="cuda", dtype=dtype, memory_format=torch.channels_last)
+    check(x[:, :, ::2], dy[:, :, ::2], gamma, beta, 4, "silu")
+    check(x[:, 1:, 1:], dy[:, 1:, 1:], gamma, beta, 4, "silu")
+    check(x, dy[:, :1, :1].expand(x.shape), gamma, beta, 4, "silu")
+    check(x[:1].expand(x.shape), dy, gamma, beta, 4, "silu")
+    nhwc = torch.empty(2, 40, h, w, device="cuda", dtype=dtype, memory_format=torch.channels_last)
     nhwc.copy_(nchw)
-    y, _ = check(nhwc.permute(0, 2, 3, 1), dy, w, b, 4, "silu")
+    y, _ = check(nhwc.permute(0, 2, 3, 1), dy, gamma, beta, 4, "silu")
     assert torch.equal(y, base)
     # a scalar loss hands back a gradient without extent
     leaf = x.detach().requires_grad_()
-    (dx,) = torch.autograd.grad(group_norm_act(leaf, 4, w, b, eps=EPS).sum(), leaf)
-    r = reference(x, 4, w, b, "silu", torch.ones_like(x))
+    (dx,) = torch.autograd.grad(group_norm_act(leaf, 4, gamma, beta, eps=EPS).sum(), leaf)
+    r = reference(x, 4, gamma, beta, "silu", torch.ones_like(x))
     within(dx, r[2], 1e-4 * r[3].amax(), "dx of a sum")
 
 
@@ -201,8 +204,9 @@ def test_empty(cuda_device, shape):
     assert dx.shape == shape and not dw.any() and not db.any()
 
 
-def test_non_finite_values_stay_in_their_group(cuda_device):
-    x, dy, w, b = make((2, 21, 30, 16), 4, F32, F32)
+@pytest.mark.parametrize("width", [30, 300])
+def test_non_finite_values_stay_in_their_group(cuda_device, width):
+    x, dy, w, b = make((2, 21, width, 16), 4, F32, F32)
     clean = group_norm_act(x, 4, w, b, eps=EPS)
     for bad in (float("nan"), float("inf"), -float("inf")):
         z = x.clone()
@@ -310,6 +314,18 @@ def test_first_gradients_of_a_graph_that_is_kept(cuda_device, size):
     assert all(torch.equal(p, k) for p, k in zip(plain, kept))
     with pytest.raises(RuntimeError):
         torch.autograd.grad(kept[0].sum(), leaves[0])
+
+
+@pytest.mark.parametrize("size", [6, 70])
+def test_every_choice_of_wanted_gradients(cuda_device, size):
+    x, dy, w, b = make((2, size, 10, 24), 3, F32, F32)
+    everything = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(group_norm_act(everything[0], 3, everything[1], everything[2], eps=EPS), everything, dy)
+    for mask in range(1, 7):
+        leaves = [t.detach().requires_grad_(bool(mask >> k & 1)) for k, t in enumerate((x, w, b))]
+        wanted = [k for k in range(3) if mask >> k & 1]
+        got = torch.autograd.grad(group_norm_act(leaves[0], 3, leaves[1], leaves[2], eps=EPS), [leaves[k] for k in wanted], dy)
+        assert all(torch.equal(g, want[k]) for g, k in zip(got, wanted))
 
 
 def test_most_images(cuda_device):

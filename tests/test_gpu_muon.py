@@ -266,6 +266,31 @@ def test_optimizer(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(leaves, twin))
 
 
+def test_long_matrices_on_two_streams_and_in_graphs(cuda_device):
+    """Sums that CTAs leave to one another: two streams and two graphs at once, each several times."""
+    updates = [make(512, 8192, seed=1), make(8200, 400, seed=2)]
+    want = [orthogonalize(u) for u in updates]
+    graphs = []
+    for u in updates:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = orthogonalize(u)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in updates]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, u, (graph, out) in zip(streams, updates, graphs):
+            out.zero_()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(orthogonalize(u))
+                graph.replay()
+        torch.cuda.synchronize()
+        for g, (graph, out), w in zip(got, graphs, want):
+            assert torch.equal(g, w) and torch.equal(out, w)
+
+
 def test_streams_and_graphs(cuda_device):
     """The same bits on another stream and from a captured graph, replayed twice on changing gradients; two graphs at
     once on two streams."""

@@ -19,7 +19,8 @@
 //  * 16-bit matrices (large ones, see planes_of): A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
 //    and B lose turns X's singular directions by that much and no more.  What X loses is noise in all directions alike,
 //    and the next steps amplify it where X is small: with one value the result is 4e-3 off at 512 x 512 and 6e-3 at
-//    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.
+//    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.  So it is
+//    in the first one, where U times a power of two is exact (8 bits) and what is left of 1 / |U| goes into the scales.
 //
 // Working matrices are stored as the products read them: blocks of 128 rows x 64 columns, each the image of one shared
 // memory tile (128-byte rows, 16-byte pieces exchanged within groups of eight rows), hi and lo one after the other, zero
@@ -53,7 +54,7 @@ struct Matrix {
     int64_t src_stride;   // values between rows
     char *x[2], *a, *b;   // blocks of X (two buffers), A, B
     char* v;              // V's blocks on the diagonal: two for each block of rows
-    double* norms;        // sums of squares of the norm pass
+    double* norms;        // sums of squares of the norm pass; before them, as a float, the factor that `exact` leaves out
     int32_t rows, cols;
     int32_t m;            // short side
     int32_t mb, mk, nk;   // blocks: rows of all three, columns of A and B, columns of X
@@ -70,6 +71,7 @@ struct Table {
     float out_scale;      // of a product's result; of X in the first and the last pass
     float shift;          // added on the diagonal of V or B
     int32_t cubic;        // c = 0: the first product gives B
+    int32_t exact;        // X is U times a power of two, as one value (first pass and first step of large 16-bit matrices)
     uint32_t* fail;       // set when a bounded wait ran out: the last pass then writes NaN
     int32_t parts;        // how many pairs of CTAs share the sum of a tile
     uint32_t* tickets;    // how many of them have put their sums down: for both halves of every tile, zero between products
@@ -232,7 +234,16 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
     char* const out = m.x[0] + (int64_t)block * 2 * kPlane;
     let_next_start();
     wait_for_previous();
-    const float scale = inverse_norm(t, m) * t.out_scale;
+    float scale = inverse_norm(t, m) * t.out_scale;
+    if (t.exact) {
+        const uint32_t exponent = __float_as_uint(scale) & 0x7f800000u;
+        float rest = 1.0f;   // in [1, 2); scales without a power of two (zero, not finite) stay whole
+        if (exponent != 0 && exponent != 0x7f800000u) {
+            rest = scale / __uint_as_float(exponent);
+            scale = __uint_as_float(exponent);
+        }
+        if (block == 0 && threadIdx.x == 0) *reinterpret_cast<float*>(m.norms - 1) = rest;
+    }
 #pragma unroll 2
     for (int i = threadIdx.x; i < kRows * kCols / 8; i += kThreads) {
         // row and column within the block's part of U
@@ -251,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
         if (!tall) {
             const uint32_t o = block_offset(r, c);
             *reinterpret_cast<uint4*>(out + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(out + kPlane + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (!t.exact) *reinterpret_cast<uint4*>(out + kPlane + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -263,7 +274,8 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
     }
     if (!tall) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * (int)kPlane / 16; i += kThreads) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s)[i];
+    for (int i = threadIdx.x; i < (t.exact ? 1 : 2) * (int)kPlane / 16; i += kThreads)
+        reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(s)[i];
 }
 
 // Eight neighbouring values of the result: stored, or taken from the parameter.
@@ -460,7 +472,7 @@ __device__ __forceinline__ uint32_t instruction(bool across, uint32_t rows, uint
 enum { kGram = 0, kSquare = 1, kApply = 2 };
 
 // What the products of a mode of large matrices read: planes of the left and the right factor and of the result, and how
-// many planes lie between blocks of A and B.  RIGHT is 1 in the last step of 16-bit matrices.
+// many planes lie between blocks of A and B.  RIGHT is 1 in the first and the last step of 16-bit matrices.
 template <bool F32, int MODE, int RIGHT> struct Planes {
     static constexpr int kLeft = F32 ? 2 : 1;
     static constexpr int kRight = RIGHT;
@@ -1176,6 +1188,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         constexpr int kPart = N / 2;                     // columns of a thread; the warps' upper half takes the right ones
         const int half = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, r = threadIdx.x & 127;
+        float scale = t.out_scale;
+        if (!F32 && MODE != kSquare && t.exact) {   // what X leaves out of 1 / |U|
+            const float rest = *reinterpret_cast<const float*>(m.norms - 1);
+            scale *= MODE == kGram ? rest * rest : rest;
+        }
         float v[kPart];
 #pragma unroll
         for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
@@ -1254,10 +1271,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 const uint32_t o = block_offset(r, c % kCols);
                 uint32_t hi[4], lo[4];
                 const int in = row * kRows + (int)r, on = in < m.m ? in - (col * kCols + c) : -1;   // diagonal
-                finish(v + c, t.out_scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+                finish(v + c, scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
                 put<P::kOut == 2>(space + (c / kCols) * kOutBytes + o, hi, lo);
                 if (MODE == kGram && keeps_v) {
-                    finish(v + c, t.out_scale, t.shift, on, hi, lo);
+                    finish(v + c, scale, t.shift, on, hi, lo);
                     put<P::kOut == 2>((N == 256 ? space + kMine : smem + (2 + half) * kMine) + (c / kCols) * kOutBytes + o, hi, lo);
                 }
                 if (MODE != kApply && mirrored) {
@@ -1335,7 +1352,7 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.nk = (p.n + kCols - 1) / kCols;
     p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
-    p.norms = up256((size_t)div_up64(d.rows * ((d.cols + 7) / 8), kPieces) * 8);
+    p.norms = up256((size_t)div_up64(d.rows * ((d.cols + 7) / 8), kPieces) * 8 + 8);
     p.v = (size_t)p.mb * 2 * planes * kPlane;
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
@@ -1513,12 +1530,12 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
     return launch(ns_pair_kernel<F32, MODE, RIGHT, 128>, "ns_pair_kernel", narrow * 2, kPairThreads,
                   PairStages<L, RIGHT, 128>::kBytes, 2, st, t);
 }
-// one product of every matrix of the table; `blocks` writes its first_block
-template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table& t, bool last, B& blocks, cudaStream_t st) {
+// one product of every matrix of the table; `blocks` writes its first_block; one: X is one value
+template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table& t, bool one, B& blocks, cudaStream_t st) {
     if constexpr (!PAIR) return small_product<MODE>(t, blocks, st);
     else if constexpr (F32) return pair_product<true, MODE, 2>(t, blocks, st);
     else if constexpr (MODE == kApply)
-        return last ? pair_product<false, MODE, 1>(t, blocks, st) : pair_product<false, MODE, 2>(t, blocks, st);
+        return one ? pair_product<false, MODE, 1>(t, blocks, st) : pair_product<false, MODE, 2>(t, blocks, st);
     else return pair_product<false, MODE, 1>(t, blocks, st);
 }
 
@@ -1546,7 +1563,7 @@ void next_table(Table& t, const D3gsOrthoMatrix* mats, int32_t count, int32_t& i
         m.a = at + 2 * p.x;
         m.b = at + 2 * p.x + p.a;
         m.v = at + 2 * p.x + 2 * p.a;
-        m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a + p.v);
+        m.norms = reinterpret_cast<double*>(at + 2 * p.x + 2 * p.a + p.v) + 1;
         at += p.total;
     }
 }
@@ -1605,21 +1622,23 @@ int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int
         unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
         if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, t)) return rc;
         t.out_scale = sp.first;
+        t.exact = !F32;
         grid = blocks(every_block);
         if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, t)) return rc;
         for (int s = 0; s < sp.count; ++s) {
-            const bool last = s == sp.count - 1;
+            const bool one = s == 0 || s == sp.count - 1;
+            t.exact = !F32 && s == 0;
             t.cubic = sp.cubic >> s & 1;
             t.out_scale = sp.gram[s];
             t.shift = sp.gram_shift[s];
-            if (int32_t rc = product<F32, PAIR, kGram>(t, last, blocks, st)) return rc;
+            if (int32_t rc = product<F32, PAIR, kGram>(t, one, blocks, st)) return rc;
             if (!t.cubic) {
                 t.out_scale = sp.square[s];
                 t.shift = sp.square_shift[s];
-                if (int32_t rc = product<F32, PAIR, kSquare>(t, last, blocks, st)) return rc;
+                if (int32_t rc = product<F32, PAIR, kSquare>(t, one, blocks, st)) return rc;
             }
             t.out_scale = sp.apply[s];
-            if (int32_t rc = product<F32, PAIR, kApply>(t, last, blocks, st)) return rc;
+            if (int32_t rc = product<F32, PAIR, kApply>(t, one, blocks, st)) return rc;
             t.from ^= 1;
         }
         t.out_scale = sp.last;

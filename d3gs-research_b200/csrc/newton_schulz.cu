@@ -399,6 +399,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
         : "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tmem_store32(uint32_t at, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%"
+        "17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -1193,9 +1206,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             const float rest = *reinterpret_cast<const float*>(m.norms - 1);
             scale *= MODE == kGram ? rest * rest : rest;
         }
-        float v[kPart];
+        constexpr bool kAdds = F32 || SHARED;            // the sums pass through registers
+        float v[kAdds ? kPart : 1];
 #pragma unroll
-        for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
+        for (int c = 0; c < kPart && kAdds; ++c) v[c] = 0.0f;
         auto take = [&](uint32_t from) {
 #pragma unroll
             for (int c = 0; c < kPart; c += 32) {
@@ -1205,7 +1219,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 for (int i = 0; i < 32; ++i) v[c + i] += w[i];
             }
         };
-        if (F32)
+        if constexpr (F32)
             for (int k = 0; k < blocks; ++k) {
                 ok = __all_sync(~0u, wait_for(&s_sum[k % kSumBars], (k / kSumBars) & 1, polls));
                 if (!ok) break;
@@ -1217,7 +1231,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             }
         if (ok) ok = __all_sync(~0u, wait_for(&s_last, 0, polls));
         tc_fence_after();
-        if (ok && (!SHARED || blocks > 0)) take(F32 ? kSums * N : 0);
+        if constexpr (kAdds)
+            if (ok && (!SHARED || blocks > 0)) take(F32 ? kSums * N : 0);
         if (!ok) *t.fail = 1;
         // A tile that several pairs share: everyone puts its sums down, four columns of 128 rows after one another, the last
         // one to do so adds them up in the order of the parts and goes on.
@@ -1264,25 +1279,36 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         constexpr uint32_t kMine = kPart / kCols * kOutBytes, kSpace = MODE == kApply ? kMine : 2 * kMine;
         constexpr bool kTurns = 2 * kSpace > 196608u;
         char* const space = smem + (kTurns ? 0 : half * (N == 256 ? kSpace : kMine));
-        auto write = [&]() {
+        // What follows is a loop over TMEM: code that every CTA runs once is bound by fetching it.
+        if constexpr (kAdds) {
 #pragma unroll
-            for (int c = 0; c < kPart; c += 8) {
-                if (col + c / kCols >= wide || row >= m.mb) continue;
-                const uint32_t o = block_offset(r, c % kCols);
-                uint32_t hi[4], lo[4];
-                const int in = row * kRows + (int)r, on = in < m.m ? in - (col * kCols + c) : -1;   // diagonal
-                finish(v + c, scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
-                put<P::kOut == 2>(space + (c / kCols) * kOutBytes + o, hi, lo);
-                if (MODE == kGram && keeps_v) {
-                    finish(v + c, scale, t.shift, on, hi, lo);
-                    put<P::kOut == 2>((N == 256 ? space + kMine : smem + (2 + half) * kMine) + (c / kCols) * kOutBytes + o, hi, lo);
-                }
-                if (MODE != kApply && mirrored) {
-                    // N 256: rows of one block, columns of the two blocks that the rows r belong to.  N 128: a half's 64
-                    // columns are 64 rows of a block, the two halves' rows follow one another.
-                    char* const to = N == 256 ? space + kMine + (r / kCols) * kOutBytes
-                                              : smem + 2 * kMine + (r / kCols) * kOutBytes;
-                    write_mirrored<P::kOut == 2>(to, (N == 256 ? 0 : half * kCols) + c, r % kCols, hi, lo);
+            for (int c = 0; c < kPart; c += 32) tmem_store32(tmem + half * kPart + c + lanes, v + c);
+            tmem_wait_stored();
+        }
+        auto write = [&]() {
+#pragma unroll 1
+            for (int c0 = 0; c0 < kPart; c0 += 32) {
+                if (col + c0 / kCols >= wide || row >= m.mb) continue;
+                float w[32];
+                tmem_load32(tmem + half * kPart + c0 + lanes, w);
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    const int c = c0 + i;
+                    const uint32_t o = block_offset(r, c % kCols);
+                    uint32_t hi[4], lo[4];
+                    const int in = row * kRows + (int)r, on = in < m.m ? in - (col * kCols + c) : -1;   // diagonal
+                    finish(w + i, scale, t.shift, MODE == kSquare || (MODE == kGram && t.cubic) ? on : -1, hi, lo);
+                    put<P::kOut == 2>(space + (c / kCols) * kOutBytes + o, hi, lo);
+                    if (MODE == kGram && keeps_v) {
+                        finish(w + i, scale, t.shift, on, hi, lo);
+                        put<P::kOut == 2>((N == 256 ? space + kMine : smem + (2 + half) * kMine) + (c / kCols) * kOutBytes + o, hi, lo);
+                    }
+                    if (MODE != kApply && mirrored) {
+                        // N 256: rows of one block, columns of the two blocks that the rows r belong to.  N 128: a half's 64
+                        // columns are 64 rows of a block, the two halves' rows follow one another.
+                        char* const to = N == 256 ? space + kMine + (r / kCols) * kOutBytes : smem + 2 * kMine + (r / kCols) * kOutBytes;
+                        write_mirrored<P::kOut == 2>(to, (N == 256 ? 0 : half * kCols) + c, r % kCols, hi, lo);
+                    }
                 }
             }
             fence_proxy_async_smem();

@@ -1206,10 +1206,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             const float rest = *reinterpret_cast<const float*>(m.norms - 1);
             scale *= MODE == kGram ? rest * rest : rest;
         }
-        constexpr bool kAdds = F32 || SHARED;            // the sums pass through registers
-        float v[kAdds ? kPart : 1];
+        float v[F32 ? kPart : 1];
 #pragma unroll
-        for (int c = 0; c < kPart && kAdds; ++c) v[c] = 0.0f;
+        for (int c = 0; c < kPart && F32; ++c) v[c] = 0.0f;
         auto take = [&](uint32_t from) {
 #pragma unroll
             for (int c = 0; c < kPart; c += 32) {
@@ -1231,18 +1230,31 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             }
         if (ok) ok = __all_sync(~0u, wait_for(&s_last, 0, polls));
         tc_fence_after();
-        if constexpr (kAdds)
-            if (ok && (!SHARED || blocks > 0)) take(F32 ? kSums * N : 0);
         if (!ok) *t.fail = 1;
+        // What follows are loops over TMEM: code that every CTA runs once is bound by fetching it.
+        const uint32_t sums_at = tmem + half * kPart + lanes;
+        if constexpr (F32) {
+            if (ok && (!SHARED || blocks > 0)) take(kSums * N);
+#pragma unroll
+            for (int c = 0; c < kPart; c += 32) tmem_store32(sums_at + c, v + c);
+            tmem_wait_stored();
+        }
         // A tile that several pairs share: everyone puts its sums down, four columns of 128 rows after one another, the last
         // one to do so adds them up in the order of the parts and goes on.
         bool finishes = true;
         if constexpr (SHARED) {
             __shared__ uint32_t s_ticket;
-            float4* const sums = t.sums + (int64_t)(tile * 2 + rank) * parts * (kSumBytes / 16) + half * kPart * 32 + r;
+            constexpr int kNext = (int)(kSumBytes / 16);
+            float4* const sums = t.sums + (int64_t)(tile * 2 + rank) * parts * kNext + half * kPart * 32 + r;
+#pragma unroll 1
+            for (int c = 0; c < kPart; c += 32) {
+                float w[32];
+                tmem_load32(sums_at + c, w);
+                const bool some = F32 || blocks > 0;
 #pragma unroll
-            for (int c = 0; c < kPart; c += 4)
-                __stcg(sums + part * (int)(kSumBytes / 16) + c * 32, make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]));
+                for (int i = 0; i < 32; i += 4)
+                    __stcg(sums + part * kNext + (c + i) * 32, some ? make_float4(w[i], w[i + 1], w[i + 2], w[i + 3]) : make_float4(0, 0, 0, 0));
+            }
             __threadfence();
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (threadIdx.x == 0) {
@@ -1253,18 +1265,27 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             finishes = s_ticket == (uint32_t)parts - 1;
-            if (finishes) {
-#pragma unroll
-                for (int c = 0; c < kPart; ++c) v[c] = 0.0f;
 #pragma unroll 1
-                for (int q = 0; q < parts; ++q) {
+            for (int c = 0; c < kPart && finishes; c += 32) {
+                float w[32];
 #pragma unroll
-                    for (int c = 0; c < kPart; c += 4) {
-                        const float4 w = __ldcg(sums + q * (int)(kSumBytes / 16) + c * 32);
-                        v[c] += w.x, v[c + 1] += w.y, v[c + 2] += w.z, v[c + 3] += w.w;
-                    }
+                for (int i = 0; i < 32; ++i) w[i] = 0.0f;
+#pragma unroll 1
+                for (int q = 0; q < parts; q += 4) {   // (four or eight parts)
+                    float4 f[4][8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[k][i] = __ldcg(sums + (q + k) * kNext + (c + 4 * i) * 32);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            w[4 * i] += f[k][i].x, w[4 * i + 1] += f[k][i].y, w[4 * i + 2] += f[k][i].z, w[4 * i + 3] += f[k][i].w;
                 }
+                tmem_store32(sums_at + c, w);
             }
+            tmem_wait_stored();
         }
         // Every product has read its operands by now: their shared memory takes the finished blocks, from where they
         // leave as whole blocks.
@@ -1279,18 +1300,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
         constexpr uint32_t kMine = kPart / kCols * kOutBytes, kSpace = MODE == kApply ? kMine : 2 * kMine;
         constexpr bool kTurns = 2 * kSpace > 196608u;
         char* const space = smem + (kTurns ? 0 : half * (N == 256 ? kSpace : kMine));
-        // What follows is a loop over TMEM: code that every CTA runs once is bound by fetching it.
-        if constexpr (kAdds) {
-#pragma unroll
-            for (int c = 0; c < kPart; c += 32) tmem_store32(tmem + half * kPart + c + lanes, v + c);
-            tmem_wait_stored();
-        }
         auto write = [&]() {
 #pragma unroll 1
             for (int c0 = 0; c0 < kPart; c0 += 32) {
                 if (col + c0 / kCols >= wide || row >= m.mb) continue;
                 float w[32];
-                tmem_load32(tmem + half * kPart + c0 + lanes, w);
+                tmem_load32(sums_at + c0, w);
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     const int c = c0 + i;

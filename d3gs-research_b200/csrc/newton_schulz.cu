@@ -1422,7 +1422,7 @@ int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig&
 }
 constexpr size_t kHead = 256 + 1024;   // the failure word, the tickets
 // Column blocks of a long axis that each of the pairs sharing a tile should have at least; twice that in 16 bits.
-constexpr int kShare = 12;
+constexpr int kShare = 8;
 size_t shared_bytes(const D3gsOrthoMatrix* mats, int32_t count) {
     int64_t longest = 0;
     for (int32_t i = 0; i < count; ++i) longest = max(longest, max(mats[i].rows, mats[i].cols));
@@ -1547,11 +1547,10 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
         return MODE == kApply ? pairs * ((m.nk + 3) / 4) : pairs * (pairs + 1) / 2;
     });
     if constexpr (MODE == kGram) {
-        // Few tiles and a long axis: four or eight pairs a tile, with enough of the axis for each.  Two do not make up for
-        // the way of the sums through memory (10 us).  One pair a tile -> this: 512 x 3400 352 -> 332 us, 512 x 8192 628 ->
-        // 404, 512 x 32768 2162 -> 946, 1024 x 8192 829 -> 667; 512 x 6400 in 16 bits 294 -> 259.  (With two pairs: 2048 x
-        // 4096 891 -> 939.  With eight blocks each: 512 x 2048 278 -> 317, 1024 x 2304 357 -> 391; with 16 in 16 bits: 1024 x
-        // 4096 268 -> 275.)
+        // Few tiles and a long axis: four or eight pairs a tile, with enough of the axis for each; two do not make up for
+        // the way of the sums through memory.  One pair a tile -> this: 500 x 2600 302 -> 283 us, 1024 x 2304 350 -> 346,
+        // 512 x 8192 610 -> 355, 512 x 32768 2126 -> 833; in 16 bits 1024 x 4096 259 -> 253, 512 x 8192 309 -> 227.  (From
+        // twelve blocks a pair on, 24 in 16 bits, instead: 512 x 4608 317 instead of 297 us, in 16 bits 215 instead of 193.)
         Table u = t;
         int longest = 0;
         for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);

@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
 //
 // Measured: 4096 x 4096 in 16 bits 1.65 ms a call of five steps, 0.83 PFLOP/s, with X's second plane counted 1.08, where
 // the power limit leaves a plain product 1.40; tensor cores busy for 69 % of B X, 56 % of the others
-// (1.84 rounds of tiles on 74 pairs).  2048 x 2048 in 32 bits 0.52 to 0.58 ms: busy for 58 % of B X in 256-wide tiles, 38 %
+// (1.84 rounds of tiles on 74 pairs).  2048 x 2048 in 32 bits 0.51 to 0.58 ms: busy for 58 % of B X in 256-wide tiles, 38 %
 // of the others in 128-wide ones, which an SM takes 48 KB in for every 768 cycles of products.
 constexpr int kPairThreads = 320;
 template <int L, int R, int N> struct PairStages {

@@ -83,13 +83,26 @@ def _forward(x, groups, weight, bias, eps, act, keep: bool):
     return x, y, stats, args
 
 
+def _came_back(x, weight, bias, stats, dy, d):
+    """The saved tensors as the library reads them.  Hooks of the caller (``save_on_cpu``) may have put copies in their
+    place, laid out anew; ``d`` gets the strides of ``x`` as it is now."""
+    for t, like, dtype, shape in ((x, "x", d.dtype, dy.shape), (weight, "weight", d.weight_dtype, dy.shape[-1:]),
+                                  (bias, "bias", d.weight_dtype, dy.shape[-1:]), (stats, "statistics", 0, (d.batch, d.groups, 2))):
+        if t is not None and (t.shape != shape or t.device != dy.device or _DTYPES.get(t.dtype) != dtype):
+            raise RuntimeError(f"group_norm_act: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}: not the "
+                               f"{like} that the forward saved")
+    x, (d.x_batch_stride, d.x_pixel_stride) = _prepared(x)
+    return x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), stats.contiguous()
+
+
 def _backward(args, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b: bool):
-    device = x.device
+    device = dy.device
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _backward(args, x, weight, bias, stats, dy, need_x, need_w, need_b)
     lib = _lib.load()
     d = _lib.GroupNorm.from_buffer_copy(args)
+    x, weight, bias, stats = _came_back(x, weight, bias, stats, dy, d)
     dy, (d.dy_batch_stride, d.dy_pixel_stride) = _prepared(dy)
     empty = x.numel() == 0
     dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None

@@ -1,0 +1,108 @@
+"""What the decoder operators hand to the library, recorded on the CPU: a recorder stands in for the library's entries,
+CPU tensors for those on a GPU.  Nothing is computed."""
+import types
+
+import pytest
+import torch
+
+from d3gs_research_b200 import _lib, group_norm
+from d3gs_research_b200.group_norm import _GroupNormAct
+
+
+class Recorder:
+    """Takes the calls of the library: (entry, descriptor's fields where there is one, the other arguments)."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            fields = None
+            if hasattr(args[0], "_obj"):   # C.byref(descriptor)
+                fields = types.SimpleNamespace(**{k: getattr(args[0]._obj, k) for k, _ in args[0]._obj._fields_})
+            self.calls.append((name, fields, args))
+            return 256 if name.endswith("workspace_bytes") else 0
+        return entry
+
+    def last(self, name):
+        return next((f, a) for n, f, a in reversed(self.calls) if n == name)
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    rec = Recorder()
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)   # the index of a CPU tensor's device
+    return rec
+
+
+def reaches(at, image, pixel, d):
+    """One past the last value that the library reads of a tensor with these strides."""
+    return at + 4 * ((d.batch - 1) * image + (d.pixels - 1) * pixel + d.channels)
+
+
+def extent(t):
+    return t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def hooked(x, w, b, unpack):
+    """A backward whose saved tensors come back as ``unpack`` makes them, and those of the type's input shape."""
+    back = []
+
+    def keep(t):
+        back.append(unpack(t))
+        return back[-1]
+
+    leaves = [x.detach().requires_grad_(), w.detach().requires_grad_(), b.detach().requires_grad_()]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, keep):
+        y = _GroupNormAct.apply(*leaves, (4, 1e-5, 1))
+    torch.autograd.grad(y, leaves, torch.ones_like(y))
+    return back
+
+
+def spread(t):
+    """The same values, every second of a wider tensor."""
+    wide = torch.zeros(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype)
+    wide[..., ::2] = t
+    return wide[..., ::2]
+
+
+def padded(t):
+    """The same values with room behind every pixel's channels."""
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 24, dtype=t.dtype)
+    wide[..., 4:4 + t.shape[-1]] = t
+    return wide[..., 4:4 + t.shape[-1]]
+
+
+@pytest.mark.parametrize("view", [lambda t: t[..., 8:48], lambda t: t[:, :, ::2, :40], lambda t: t[:1, :, :, :40].expand(2, -1, -1, -1),
+                                  lambda t: t[..., :40].contiguous()])
+@pytest.mark.parametrize("unpack", [lambda t: t.clone(memory_format=torch.contiguous_format), padded, spread])
+def test_saved_tensors_that_come_back_with_other_strides(recorder, view, unpack):
+    """Saved-tensor hooks (``save_on_cpu`` among them) may return a copy laid out anew: the library gets the strides of
+    the tensor whose pointer it gets, and reads nothing behind its end."""
+    x = view(torch.arange(2 * 6 * 8 * 56, dtype=torch.float32).reshape(2, 6, 8, 56))
+    back = hooked(x, torch.ones(40), torch.zeros(40), unpack)
+    d, args = recorder.last("d3gs_group_norm_backward")
+    x_at, weight_at, bias_at, stats_at = args[1:5]
+    got = next(t for t in back if t.shape == x.shape)
+    if got.stride(-1) == 1:
+        assert x_at == got.data_ptr()
+        assert (d.x_batch_stride, d.x_pixel_stride) == group_norm._pixel_strides(got)
+        assert reaches(x_at, d.x_batch_stride, d.x_pixel_stride, d) <= extent(got)
+    else:                               # copied first
+        assert (d.x_batch_stride, d.x_pixel_stride) == (x[0].numel(), 40)
+    for at, t in ((weight_at, back[1]), (bias_at, back[2]), (stats_at, back[3])):
+        assert (at == t.data_ptr()) == t.is_contiguous()
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.double(), lambda t: t[:1], lambda t: t[..., :3]])
+def test_saved_tensors_that_come_back_as_something_else(recorder, unpack):
+    """Of another type or size they are refused: the library would read what is not there."""
+    x = torch.zeros(2, 6, 8, 40)
+    with pytest.raises(RuntimeError, match="group_norm_act: a saved tensor came back"):
+        hooked(x, torch.ones(40), torch.zeros(40), lambda t: unpack(t) if t.shape == x.shape else t)
+    for size in ((40,), (2, 4, 2)):
+        with pytest.raises(RuntimeError, match="group_norm_act: a saved tensor came back"):
+            hooked(x, torch.ones(40), torch.zeros(40), lambda t: t.double() if t.shape == size else t)
+    assert all(name != "d3gs_group_norm_backward" for name, *_ in recorder.calls)

@@ -12,6 +12,7 @@ import struct
 import torch
 
 from . import _lib
+from ._recording import refuse_recording
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"none": 0, "silu": 1, "gelu": 2}
@@ -148,7 +149,9 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     ``act`` is ``"none"``, ``"silu"`` or ``"gelu"`` (the erf form).  ``x`` is float32, bfloat16 or float16; ``weight``
     and ``bias`` ``[C]`` share one of these types, not necessarily that of ``x``.  Sums and statistics are float32.
     Channels that are not dense, or pixels that are not evenly spaced, are copied first.  The result is dense and has
-    the type of ``x``; gradients flow to ``x``, ``weight`` and ``bias`` (once)."""
+    the type of ``x``; gradients flow to ``x``, ``weight`` and ``bias`` (once).  Under ``torch.jit.trace`` or with inputs
+    that carry a forward-mode tangent the call is refused."""
+    refuse_recording("group_norm_act", (x, weight, bias))
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("group_norm_act: x must be a CUDA tensor")
     if x.dim() < 2 or x.dtype not in _DTYPES:

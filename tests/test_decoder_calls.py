@@ -106,3 +106,57 @@ def test_saved_tensors_that_come_back_as_something_else(recorder, unpack):
         with pytest.raises(RuntimeError, match="group_norm_act: a saved tensor came back"):
             hooked(x, torch.ones(40), torch.zeros(40), lambda t: t.double() if t.shape == size else t)
     assert all(name != "d3gs_group_norm_backward" for name, *_ in recorder.calls)
+
+
+def on_gpu(monkeypatch):
+    """CPU tensors that say they are on a GPU: the calls' own checks of their tensors come after those tested here."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+
+
+def calls():
+    from d3gs_research_b200 import group_norm_act, muon_step, orthogonalize
+
+    def step(t):
+        muon_step([t], [t.clone()], [t.clone()], lr=0.1)
+        return t
+
+    return {"group_norm_act": lambda t: group_norm_act(t, 2), "orthogonalize": lambda t: orthogonalize(t), "muon_step": step}
+
+
+@pytest.mark.parametrize("name", ["group_norm_act", "orthogonalize", "muon_step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_calls_under_a_tracer_are_refused(recorder, monkeypatch, name, grad):
+    """The trace would hold the allocation of the result and no kernel."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    on_gpu(monkeypatch)
+    call, x = calls()[name], torch.ones(4, 6)
+    if grad and name == "group_norm_act":
+        x.requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name}: cannot be traced"):
+        torch.jit.trace(call, x)
+    for pre in (False, True):
+        with pytest.raises(RuntimeError, match=f"{name}: cannot be traced"):
+            make_fx(call, pre_dispatch=pre)(x)
+    assert not recorder.calls
+    call(x.detach())                       # and no longer once the tracer has gone
+    assert recorder.calls
+
+
+@pytest.mark.parametrize("name", ["group_norm_act", "orthogonalize", "muon_step"])
+def test_tangents_are_refused(recorder, monkeypatch, name):
+    """Forward-mode differentiation would go on without them."""
+    import torch.autograd.forward_ad as forward_ad
+    from d3gs_research_b200 import group_norm_act
+    on_gpu(monkeypatch)
+    x = torch.ones(4, 6)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match=f"{name}: has no forward-mode"):
+            calls()[name](forward_ad.make_dual(x, x.clone()))
+        for k in range(2):
+            weights = [torch.ones(6), torch.ones(6)]
+            weights[k] = forward_ad.make_dual(weights[k], torch.ones(6))
+            with pytest.raises(RuntimeError, match="group_norm_act: has no forward-mode"):
+                group_norm_act(x, 2, *weights)
+        assert not recorder.calls
+        calls()[name](x)                   # inputs without one go through
+    assert recorder.calls

@@ -1,9 +1,9 @@
-"""The decoder operators in the calls around a training step: saved-tensor hooks.  Against the same call without them,
+"""The decoder operators in the calls around a training step: saved-tensor hooks, tracers, tangents.  Against the same call without them,
 and the formula in 64 bits."""
 import pytest
 import torch
 
-from d3gs_research_b200 import group_norm_act
+from d3gs_research_b200 import group_norm_act, muon_step, orthogonalize
 from test_gpu_group_norm import BF16, F32, check, make
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +36,25 @@ def test_saved_tensors_that_come_back_with_other_strides(cuda_device, dtype, h, 
                 _, got = check(x, dy, gamma, beta, 4, "silu")
             if x.is_contiguous() and unpack is not padded:
                 assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tracers_and_tangents_are_refused(cuda_device):
+    """Neither sees a kernel: a trace would hold the result's allocation alone, a tangent would be lost."""
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(t):
+        muon_step([t], [torch.ones_like(t)], [torch.ones_like(t)], lr=0.1)
+        return t
+
+    for call in (lambda t: group_norm_act(t, 2), lambda t: orthogonalize(t), step):
+        for grad in (False, True):
+            x = torch.randn(3, 5, 8, device="cuda")[0].requires_grad_(grad)
+            for trace in (lambda: torch.jit.trace(call, x), lambda: make_fx(call)(x)):
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    trace()
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+        before = torch.randn(5, 8, device="cuda")
+        after = call(before.clone())
+        assert torch.isfinite(after).all() and not torch.equal(after, before)

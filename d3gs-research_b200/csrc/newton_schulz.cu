@@ -459,6 +459,31 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint32_
     return false;
 }
 
+// A loading thread that has given up waits here until the copies number `from` to `to` - 1 have landed (number j in stage
+// j % count of `full`): the CTA must not end, nor its shared memory become another's, before.  The limit is this wait's
+// own, some 7 ms where a copy takes microseconds, and not the one that has just run out, which a test may have made short.
+// (It can run out itself where a stage's barrier also counts the other CTA's word, and that one has given up as well: by
+// then every copy has landed.)
+__device__ __forceinline__ void drain(uint64_t* full, int count, int from, int to) {
+    uint32_t left = 1u << 17;
+    for (int j = from; j < to; ++j) {
+        uint32_t landed = 0;
+        while (landed == 0 && left-- != 0)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(landed)
+                : "r"(smem_u32(full + j % count)), "r"((uint32_t)(j / count) & 1u)
+                : "memory");
+        if (landed == 0) return;
+    }
+}
+// What a test makes a CTA's loading thread withhold: everything (hold = the CTA's number), so that nothing of it is in
+// flight when waits run out, or the first copy alone (hold = -2 - number), so that the others are.
+__device__ __forceinline__ bool withholds_all(const Table& t) { return t.hooks.hold == (int)blockIdx.x; }
+__device__ __forceinline__ bool withholds_first(const Table& t) { return t.hooks.hold == -2 - (int)blockIdx.x; }
+
 // Shared-memory operand in 128-byte rows with the 16-byte pieces exchanged (swizzle mode 2).  Summed along the rows:
 // eight rows are 1024 bytes apart, `next` is not used.  Summed across the rows: the next eight summed rows are 1024
 // bytes apart, the next 64 columns `next`.  The low word holds the address: moving by n bytes adds n / 16 to it.
@@ -678,7 +703,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
         for (int k = 0; k < nk; k += 2, ++phase) {   // A = X X^T, two blocks a round
             next_phase();
             const int blocks = min(2, nk - k);
-            if (tid == 0 && !(t.hooks.hold == (int)blockIdx.x && phase == 0))   // (a test: the first products never come)
+            if (tid == 0 && !(withholds_all(t) && phase == 0))   // (a test: the first products never come)
                 issue(blocks, x0 + k * kNext, kNext, x0 + k * kNext, kNext, 2, square, k == 0);
             wait_done();
 #pragma unroll
@@ -838,14 +863,15 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
 
     if (warp == 8) {
         if (lane == 0) {
+            const int landing = withholds_first(t) ? 1 : 0;
             int k = 0;
-            for (; k < blocks; ++k) {
+            for (; k < blocks && !withholds_all(t); ++k) {
                 const int st = k % S::kCount;
                 if (k >= S::kCount) ok = wait_for(&s_empty[st], (k / S::kCount - 1) & 1, polls);
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
-                if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
+                if (k < landing) continue;   // a test: this copy never comes
                 const int kb = first + k;
                 if (MODE == kApply) {
                     const int wide = 2 * tj + 1 < m.nk ? 2 : 1;            // the last tile may be one block wide
@@ -866,9 +892,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                                       &s_full[st]);
                 }
             }
-            if (!ok)   // given up: what is on its way has to land before the CTA ends
-                for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
-                    wait_for(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+            if (!ok) drain(s_full, S::kCount, max(k - S::kCount, landing), k);
         }
     } else if (warp == 9) {
         if (lane == 0) {
@@ -1096,9 +1120,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
     if (warp == 8) {
         if (lane == 0) {
             // blocks behind the matrix's end are taken from its last ones; what they give is not written
-            const int lrow = min(row, m.mb - 1);
+            const int lrow = min(row, m.mb - 1), landing = withholds_first(t) ? 1 : 0;
             int k = 0;
-            for (; k < blocks; ++k) {
+            for (; k < blocks && !withholds_all(t); ++k) {
                 const int st = k % S::kCount;
                 if (k >= S::kCount) {
                     if (kOneCommit) {   // block k - kCount is done with when the block after it has been committed
@@ -1111,7 +1135,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                 if (!ok) break;
                 char* const a = smem + st * S::kStage;
                 char* const b = a + S::kLeft;
-                if (t.hooks.hold == (int)blockIdx.x && k == 0) continue;   // a test: this copy never comes
+                if (k < landing) continue;   // a test: this copy never comes
                 const int kb = first + k;
                 const bool shared = same && !(MODE == kSquare && kb >> 2 == tj);
                 mbar_arrive_expect_tx(&s_full[st], shared ? S::kLeft : S::kStage);
@@ -1137,9 +1161,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
                         bulk_copy_g2s(b + p * (kPlane / 2), from + p * kPlane + rank * (kPlane / 2), kPlane / 2, &s_full[st]);
                 }
             }
-            if (!ok)
-                for (int j = k > S::kCount ? k - S::kCount : 0; j < k; ++j)
-                    wait_for(&s_full[j % S::kCount], (j / S::kCount) & 1, polls);
+            if (!ok) drain(s_full, S::kCount, max(k - S::kCount, landing), k);
         }
     } else if (warp == 9) {
         if (lane == 0 && rank == 1) {

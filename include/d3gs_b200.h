@@ -163,7 +163,8 @@ uint64_t d3gs_kernel_launch_count(void);
 /* For tests of the error paths (no counterpart in the reference): every bounded wait of the kernels launched by this
  * process afterwards gives up after poll_limit polls (0 = the built-in limits), and the CTA / tile number `hold` (-1 =
  * none) withholds what a wait depends on -- its look-back flag in the scan and the sort, the bulk copy its own barrier
- * expects elsewhere.  The waiting code then sets its D3GS_STATUS_* bit and returns; nothing faults and nothing waits
+ * expects elsewhere.  hold = -2 - CTA: of several copies the first alone (the products of d3gs_orthogonalize; other
+ * kernels ignore it).  The waiting code then sets its D3GS_STATUS_* bit and returns; nothing faults and nothing waits
  * for ever.  d3gs_test_hooks(0, -1) restores normal operation. */
 void d3gs_test_hooks(uint32_t poll_limit, int32_t hold);
 /* sizeof() of the ABI structs, so a binding can verify its mirror: 0 D3gsCamera, 1 D3gsOpConfig,

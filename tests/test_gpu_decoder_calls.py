@@ -1,5 +1,5 @@
-"""The decoder operators in the calls around a training step: saved-tensor hooks, tracers, tangents.  Against the same call without them,
-and the formula in 64 bits."""
+"""The decoder operators in the calls around a training step: saved-tensor hooks, tracers, tangents; and waits that give
+up.  Against the same call without them, and the formula in 64 bits."""
 import pytest
 import torch
 
@@ -58,3 +58,24 @@ def test_tracers_and_tangents_are_refused(cuda_device):
         before = torch.randn(5, 8, device="cuda")
         after = call(before.clone())
         assert torch.isfinite(after).all() and not torch.equal(after, before)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,n", [(200, 300), (384, 3456), (500, 520), (500, 8200)])
+def test_a_wait_that_gives_up_with_copies_in_flight(cuda_device, dtype, m, n):
+    """One CTA's first tile never comes while its other copies are on their way, or another CTA of the cluster withholds
+    all of its own: the loading threads wait for what they asked for, the call returns, its result is NaN, and the next
+    call gives the bits it gave before."""
+    from d3gs_research_b200 import _lib
+    lib = _lib.load()
+    u = torch.randn(m, n, generator=torch.Generator(device="cuda").manual_seed(m), device="cuda").to(dtype)
+    want = orthogonalize(u)
+    for hold in (-2, -3, 1):
+        lib.d3gs_test_hooks(300, hold)
+        try:
+            got = orthogonalize(u)
+            torch.cuda.synchronize()
+        finally:
+            lib.d3gs_test_hooks(0, -1)
+        assert torch.isnan(got).all()
+        assert torch.equal(orthogonalize(u), want)

@@ -487,7 +487,15 @@ __device__ __forceinline__ bool withholds_first(const Table& t) { return t.hooks
 // Shared-memory operand in 128-byte rows with the 16-byte pieces exchanged (swizzle mode 2).  Summed along the rows:
 // eight rows are 1024 bytes apart, `next` is not used.  Summed across the rows: the next eight summed rows are 1024
 // bytes apart, the next 64 columns `next`.  The low word holds the address: moving by n bytes adds n / 16 to it.
-__device__ __forceinline__ uint32_t operand_low(uint32_t at, uint32_t next) { return (at >> 4) | ((next >> 4) << 16); }
+// In a cluster a CTA's own shared addresses carry its rank from bit 24 on (0x01000400 is 0x400 of CTA 1).  The address field
+// has no place for it: shifted in as it is, it would add 256 bytes a rank to `next`, and products that sum across the rows
+// would read past the end of shared memory.
+constexpr uint32_t kSharedOffset = 0x3ffffu;
+__host__ __device__ constexpr uint32_t operand_low(uint32_t at, uint32_t next) {
+    return ((at & kSharedOffset) >> 4) | ((next >> 4) << 16);
+}
+static_assert(operand_low(0x07000400u, 8192) == operand_low(0x400u, 8192) && operand_low(0x400u, 8192) == (0x40u | 512u << 16),
+              "an operand is addressed within its CTA, whatever the CTA's rank");
 __device__ __forceinline__ uint64_t operand(uint32_t low) {
     return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | low;
 }
@@ -801,6 +809,13 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
 // With few tiles the summed axis is what takes time, the long one of X X^T: there the CTAs of a cluster (1, 2, 4 or 8)
 // each sum a part of it, put their sums into shared memory and each finish a part of the columns, adding the parts in the
 // order of their ranks.  The other products sum over at most kPairFrom / 64 = 6 blocks, in one CTA.
+//
+// What orders the accesses of such a cluster, one by one: a stage is written by bulk copies and read by products, ordered by
+// s_full; the next copy into it by s_empty (a commit: the products have read it).  The sums are plain stores into the same
+// memory: behind s_last, the commit of all products, whose copies had landed before.  Other CTAs read them behind the first
+// cluster barrier (its arrival releases, its wait acquires for the cluster), and no CTA leaves before the second.  All ten
+// warps arrive at both, the two that load and issue after __syncwarp.  Results are plain stores to memory; bulk copies read
+// them in the next kernel, behind griddepcontrol.wait, which returns when this grid has ended and its stores are visible.
 // Nine convolution layers of 3 to 256 rows take 165 us, eighteen launches of 9 us with the tensor cores busy for 5 to 7 %:
 // what bounds them is one launch after another, each a wait for the last one's memory, a fill of the stages, the way out
 // through TMEM and shared memory.

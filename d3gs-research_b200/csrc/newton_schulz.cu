@@ -192,8 +192,23 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
     }
 }
 
+// What turns U into X: first / max(|U|, eps) as the product of two floats, since one alone does not hold it at the ends of
+// the range (a norm above 2^126, or one below 2^-114 with an eps as small).  A power of two goes onto U first; it is one
+// in between.  With both finite, zeros stay zeros whatever eps is.
+struct Factor {
+    float power, rest;
+    __device__ __forceinline__ float operator()(float u) const { return u * power * rest; }
+};
+__device__ __forceinline__ Factor factor_of(double sum_of_squares, float eps, float first) {
+    const double norm = sqrt(sum_of_squares), f = 1.0 / (norm < (double)eps ? (double)eps : norm) * first;   // a NaN stays one
+    Factor r;
+    r.power = f > 0x1p100 ? 0x1p100f : f < 0x1p-100 ? 0x1p-100f : 1.0f;
+    r.rest = (float)(f / (double)r.power);
+    return r;
+}
+
 // every CTA adds the sums up itself, in the same order
-__device__ __forceinline__ float inverse_norm(const Table& t, const Matrix& m) {
+__device__ __forceinline__ double sum_of_squares(const Matrix& m) {
     __shared__ double s[kThreads / 32];
     const int n = (int)(((int64_t)m.rows * ((m.cols + 7) / 8) + kPieces - 1) / kPieces);
     double sum = 0.0;
@@ -204,8 +219,7 @@ __device__ __forceinline__ float inverse_norm(const Table& t, const Matrix& m) {
     __syncthreads();
     sum = 0.0;
     for (int k = 0; k < kThreads / 32; ++k) sum += s[k];
-    const double norm = sqrt(sum);
-    return (float)(1.0 / (norm < (double)t.eps ? (double)t.eps : norm));   // a NaN stays one
+    return sum;
 }
 
 // byte of value (r, c) in a plane of a block
@@ -234,13 +248,13 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
     char* const out = m.x[0] + (int64_t)block * 2 * kPlane;
     let_next_start();
     wait_for_previous();
-    float scale = inverse_norm(t, m) * t.out_scale;
+    Factor scale = factor_of(sum_of_squares(m), t.eps, t.out_scale);
     if (t.exact) {
-        const uint32_t exponent = __float_as_uint(scale) & 0x7f800000u;
-        float rest = 1.0f;   // in [1, 2); scales without a power of two (zero, not finite) stay whole
+        const uint32_t exponent = __float_as_uint(scale.rest) & 0x7f800000u;
+        float rest = 1.0f;   // in [1, 2); factors without a power of two (zero, not finite) stay whole
         if (exponent != 0 && exponent != 0x7f800000u) {
-            rest = scale / __uint_as_float(exponent);
-            scale = __uint_as_float(exponent);
+            rest = scale.rest / __uint_as_float(exponent);
+            scale.rest = __uint_as_float(exponent);
         }
         if (block == 0 && threadIdx.x == 0) *reinterpret_cast<float*>(m.norms - 1) = rest;
     }
@@ -258,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) ns_load_kernel(const __grid_constant
         }
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split2(u[2 * j] * scale, u[2 * j + 1] * scale, hi[j], lo[j]);
+        for (int j = 0; j < 4; ++j) split2(scale(u[2 * j]), scale(u[2 * j + 1]), hi[j], lo[j]);
         if (!tall) {
             const uint32_t o = block_offset(r, c);
             *reinterpret_cast<uint4*>(out + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -637,8 +651,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
     tc_fence_after();
     sum = 0.0;
     for (int k = 0; k < kTinyThreads / 32; ++k) sum += s_norm[k];
-    const double norm = sqrt(sum);
-    const float scale = (float)(1.0 / (norm < (double)t.eps ? (double)t.eps : norm)) * sp.first;   // a NaN stays one
+    const Factor scale = factor_of(sum, t.eps, sp.first);
 #pragma unroll 2
     for (int i = tid; i < pieces; i += kTinyThreads) {   // (a thread reads the momentum that it wrote)
         int r, c;
@@ -646,7 +659,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
         load_piece(i, r, c, u, false);
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split2(u[2 * e] * scale, u[2 * e + 1] * scale, hi[e], lo[e]);
+        for (int e = 0; e < 4; ++e) split2(scale(u[2 * e]), scale(u[2 * e + 1]), hi[e], lo[e]);
         if (!tall) {   // (a piece's columns behind the matrix' end are zeros, as all that is not written)
             put<true>(x + (c / kCols) * (int)kBlock + block_offset(r, c % kCols), hi, lo);
         } else {

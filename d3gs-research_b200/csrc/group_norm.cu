@@ -837,9 +837,10 @@ int images_per_turn(const D3gsGroupNorm& d, bool backward) {
 // images 17 -> 22), 128 KB 13 -> 17.  Where there is an image for every SM one CTA also finds its image in L2 again:
 // 200 images of 16 KB 22 -> 14 and 24 -> 22, of 512 KB 80 -> 59 and 130 -> 110.  (Many channels would leave a CTA no
 // shared memory for their coefficients.)
+constexpr int kSmallChannels = 2048;
 bool one_cta(const D3gsGroupNorm& d, const Args& a, bool backward) {
     const int64_t vectors = a.elems / (a.L / a.P);   // what a thread loads at a time, 16 bytes in the figures above
-    return d.channels <= 2048 && vectors <= (d.batch >= 148 ? kSmallMany : backward ? kSmallGrad : kSmall);
+    return d.channels <= kSmallChannels && vectors <= (d.batch >= 148 ? kSmallMany : backward ? kSmallGrad : kSmall);
 }
 
 // Chunks of one image: as many CTAs in a turn as run at once (a CTA without a tile is not launched).
@@ -910,9 +911,11 @@ Args make_args(const D3gsGroupNorm& d, int v, bool backward, void* ws) {
     return a;
 }
 
+// most: the most dynamic shared memory that any call of this kernel asks for.  The attribute belongs to the kernel, not to
+// the call: set to what a call needs, another thread's smaller call could lower it between this one's two steps.
 template <typename K, typename... A>
-int32_t launch(K kernel, const char* name, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
-    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+int32_t launch(K kernel, const char* name, dim3 grid, unsigned threads, size_t smem, size_t most, cudaStream_t st, const A&... args) {
+    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     cudaLaunchConfig_t c{};
     c.gridDim = grid;
     c.blockDim = dim3(threads);
@@ -928,21 +931,30 @@ int32_t launch(K kernel, const char* name, dim3 grid, unsigned threads, size_t s
     return D3GS_OK;
 }
 
+// Dynamic shared memory: entries (values of the rows that a CTA takes at once), per-channel and per-group values.
+size_t entries(const Args& a) { return (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L; }
+constexpr size_t most_entries(int V, int channels) { return channels > kThreads * V ? channels : kThreads * V; }
+constexpr size_t small_bytes(size_t entries, size_t c, size_t g) { return entries * 12 + (c + g) * 8; }
+constexpr size_t small_grad_bytes(size_t entries, size_t c, size_t g) { return entries * 8 + c * 24 + g * 8; }
+
 template <typename T, int V, int ACT>
 int32_t run_forward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, false);
-    const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
+    const size_t slots = entries(a);
     if (one_cta(d, a, false)) {
         a.chunks = 1;
-        return launch(gn_small_kernel<T, V, ACT>, "gn_small_kernel", dim3(a.batch), kThreads, slots * 12 + (a.C + a.G) * 8, st, a);
+        return launch(gn_small_kernel<T, V, ACT>, "gn_small_kernel", dim3(a.batch), kThreads, small_bytes(slots, a.C, a.G),
+                      small_bytes(most_entries(V, kSmallChannels), kSmallChannels, kSmallChannels), st, a);
     }
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;
         const dim3 grid(a.chunks, images);
-        if (int32_t rc = launch(gn_stats_kernel<T, V>, "gn_stats_kernel", grid, kThreads, slots * 12, st, a)) return rc;
-        if (int32_t rc = launch(gn_stats_join_kernel, "gn_stats_join_kernel", dim3(images * a.G), kJoinThreads, 0, st, a)) return rc;
-        if (int32_t rc = launch(gn_apply_kernel<T, V, ACT>, "gn_apply_kernel", grid, kThreads, 0, st, a)) return rc;
+        if (int32_t rc = launch(gn_stats_kernel<T, V>, "gn_stats_kernel", grid, kThreads, slots * 12,
+                                most_entries(V, kMaxChannels) * 12, st, a))
+            return rc;
+        if (int32_t rc = launch(gn_stats_join_kernel, "gn_stats_join_kernel", dim3(images * a.G), kJoinThreads, 0, 0, st, a)) return rc;
+        if (int32_t rc = launch(gn_apply_kernel<T, V, ACT>, "gn_apply_kernel", grid, kThreads, 0, 0, st, a)) return rc;
     }
     return D3GS_OK;
 }
@@ -950,23 +962,26 @@ int32_t run_forward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
 template <typename T, int V, int ACT>
 int32_t run_backward(const D3gsGroupNorm& d, Args a, cudaStream_t st) {
     const int turn = images_per_turn(d, true);
-    const size_t slots = (size_t)(a.P <= kThreads ? kThreads / a.P : 1) * a.L;
+    const size_t slots = entries(a);
     if (one_cta(d, a, true)) {
         a.chunks = 1;
         if (int32_t rc = launch(gn_small_grad_kernel<T, V, ACT>, "gn_small_grad_kernel", dim3(a.batch), kThreads,
-                                slots * 8 + (size_t)a.C * 24 + a.G * 8, st, a))
+                                small_grad_bytes(slots, a.C, a.G),
+                                small_grad_bytes(most_entries(V, kSmallChannels), kSmallChannels, kSmallChannels), st, a))
             return rc;
         if (a.batch == 1 || !(a.dweight || a.dbias)) return D3GS_OK;
-        return launch(gn_params_kernel, "gn_params_kernel", dim3((a.C + kThreads - 1) / kThreads), kThreads, 0, st, a);
+        return launch(gn_params_kernel, "gn_params_kernel", dim3((a.C + kThreads - 1) / kThreads), kThreads, 0, 0, st, a);
     }
     for (int b = 0; b < a.batch; b += turn) {
         const int images = b + turn <= a.batch ? turn : a.batch - b;
         a.first = b;
         const dim3 grid(a.chunks, images);
-        if (int32_t rc = launch(gn_grad_sums_kernel<T, V, ACT>, "gn_grad_sums_kernel", grid, kThreads, slots * 8, st, a)) return rc;
-        if (int32_t rc = launch(gn_grad_join_kernel, "gn_grad_join_kernel", dim3(a.G, images), kJoinThreads, 0, st, a)) return rc;
+        if (int32_t rc = launch(gn_grad_sums_kernel<T, V, ACT>, "gn_grad_sums_kernel", grid, kThreads, slots * 8,
+                                most_entries(V, kMaxChannels) * 8, st, a))
+            return rc;
+        if (int32_t rc = launch(gn_grad_join_kernel, "gn_grad_join_kernel", dim3(a.G, images), kJoinThreads, 0, 0, st, a)) return rc;
         const int params = b + images == a.batch && (a.dweight || a.dbias);
-        if (int32_t rc = launch(gn_grad_apply_kernel<T, V, ACT>, "gn_grad_apply_kernel", grid, kThreads, 0, st, a, params))
+        if (int32_t rc = launch(gn_grad_apply_kernel<T, V, ACT>, "gn_grad_apply_kernel", grid, kThreads, 0, 0, st, a, params))
             return rc;
     }
     return D3GS_OK;

@@ -1551,10 +1551,13 @@ int32_t check(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     return D3GS_OK;
 }
 
+// most: the most dynamic shared memory that any call of this kernel asks for (0: all ask for the same).  The attribute
+// belongs to the kernel, not to the call: set to what a call needs, another thread's smaller call could lower it between
+// this one's two steps.
 template <typename K, typename... A>
-int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
+int32_t launch(K kernel, const char* name, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st, size_t most,
                const A&... args) {
-    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024) D3GS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(most ? most : smem)));
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(threads);
@@ -1585,7 +1588,7 @@ template <int MODE, typename B> int32_t small_product(const Table& t, B& blocks,
         for (int k = 0; k < t.count; ++k) longest = max(longest, t.mat[k].nk);
         while (parts < 8 && tiles * parts * 2 <= 148 && longest >= (int)parts * 2 * 4) parts *= 2;
     }
-    return launch(ns_small_kernel<MODE>, "ns_small_kernel", tiles * parts, kSmallThreads, SmallStages::kBytes, parts, st, t);
+    return launch(ns_small_kernel<MODE>, "ns_small_kernel", tiles * parts, kSmallThreads, SmallStages::kBytes, parts, st, 0, t);
 }
 template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const Table& t, B& blocks, cudaStream_t st) {
     constexpr int L = Planes<F32, MODE, RIGHT>::kLeft;
@@ -1608,17 +1611,17 @@ template <bool F32, int MODE, int RIGHT, typename B> int32_t pair_product(const 
         while (u.parts > 1 && ((int)tiles * 2 * u.parts > kTickets || longest < u.parts * (F32 ? kShare : 2 * kShare))) u.parts /= 2;
         if (u.parts >= 4)
             return launch(ns_pair_kernel<F32, MODE, RIGHT, 256, true>, "ns_pair_kernel", tiles * u.parts * 2, kPairThreads,
-                          PairStages<L, RIGHT, 256>::kBytes, 2, st, u);
+                          PairStages<L, RIGHT, 256>::kBytes, 2, st, 0, u);
     }
     if (tiles * 2 > 100)
         return launch(ns_pair_kernel<F32, MODE, RIGHT, 256>, "ns_pair_kernel", tiles * 2, kPairThreads,
-                      PairStages<L, RIGHT, 256>::kBytes, 2, st, t);
+                      PairStages<L, RIGHT, 256>::kBytes, 2, st, 0, t);
     const unsigned narrow = blocks([](const Matrix& m) {
         const int64_t pairs = (m.mb + 1) / 2;
         return MODE == kApply ? pairs * ((m.nk + 1) / 2) : pairs * (pairs + 1);
     });
     return launch(ns_pair_kernel<F32, MODE, RIGHT, 128>, "ns_pair_kernel", narrow * 2, kPairThreads,
-                  PairStages<L, RIGHT, 128>::kBytes, 2, st, t);
+                  PairStages<L, RIGHT, 128>::kBytes, 2, st, 0, t);
 }
 // one product of every matrix of the table; `blocks` writes its first_block; one: X is one value
 template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table& t, bool one, B& blocks, cudaStream_t st) {
@@ -1688,7 +1691,9 @@ int32_t run_tiny(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t
         if (t.count == 0) break;
         int blocks = 0;
         for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + 2 * t.mat[k].mk);
-        if (int32_t rc = launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st, t, sp)) return rc;
+        if (int32_t rc = launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st,
+                                kTinyBlocks * 2 * kPlane + 1024, t, sp))
+            return rc;
     }
     return D3GS_OK;
 }
@@ -1710,11 +1715,11 @@ int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int
         auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
         t.from = 0;
         unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
-        if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, t)) return rc;
+        if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
         t.out_scale = sp.first;
         t.exact = !F32;
         grid = blocks(every_block);
-        if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, t)) return rc;
+        if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
         for (int s = 0; s < sp.count; ++s) {
             const bool one = s == 0 || s == sp.count - 1;
             t.exact = !F32 && s == 0;
@@ -1733,7 +1738,7 @@ int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int
         }
         t.out_scale = sp.last;
         grid = blocks(every_block);
-        if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, t)) return rc;
+        if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
     }
     return D3GS_OK;
 }

@@ -1,5 +1,7 @@
-"""The decoder operators in the calls around a training step: saved-tensor hooks, tracers, tangents; and waits that give
-up.  Against the same call without them, and the formula in 64 bits."""
+"""The decoder operators in the calls around a training step: saved-tensor hooks, tracers, tangents, threads; and
+waits that give up.  Against the same call without them, and the formula in 64 bits."""
+import threading
+
 import pytest
 import torch
 
@@ -79,3 +81,76 @@ def test_a_wait_that_gives_up_with_copies_in_flight(cuda_device, dtype, m, n):
             lib.d3gs_test_hooks(0, -1)
         assert torch.isnan(got).all()
         assert torch.equal(orthogonalize(u), want)
+
+
+@pytest.mark.parametrize("op", ["group_norm", "group_norm_small", "orthogonalize"])
+def test_two_threads_with_different_sizes(cuda_device, op):
+    """The same kernel with much and with little shared memory, launched by two threads at once: neither call spoils the
+    other's launch, and every result has the bits of a call alone."""
+    if op == "orthogonalize":
+        inputs = [torch.randn(m, n, device="cuda") for m, n in ((64, 64), (128, 190))]
+        call = orthogonalize
+    else:
+        pixels, widths = (70, (16384, 8192)) if op == "group_norm" else (1, (2048, 1792))
+        inputs = [torch.randn(1, pixels, c, device="cuda").requires_grad_() for c in widths]
+
+        def call(x):
+            y = group_norm_act(x, 32)
+            return torch.cat([y.detach(), *torch.autograd.grad(y, x, torch.ones_like(y))])
+
+    want = [call(x) for x in inputs]
+    failures, start = [], threading.Barrier(2)
+
+    def work(x, w):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait()
+            with torch.cuda.stream(stream):
+                bad = sum((call(x) != w).any() for _ in range(1500)).item()
+            if bad:
+                failures.append(f"{bad} results differ")
+        except Exception as e:   # noqa: BLE001 (a thread's exception is lost otherwise)
+            failures.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=a) for a in zip(inputs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
+def test_launches_of_two_threads(cuda_device):
+    """The library's entry from two threads in tight loops (ctypes lets go of the interpreter lock), one with twice the
+    shared memory of the other: no launch fails."""
+    import ctypes as C
+    from d3gs_research_b200 import _lib
+    lib = _lib.load()
+    failures = []
+
+    def work(channels):
+        x = torch.randn(1, 70, channels, device="cuda")
+        y, stats = torch.empty_like(x), torch.empty(64, device="cuda")
+        d = _lib.GroupNorm(batch=1, pixels=70, x_batch_stride=70 * channels, x_pixel_stride=channels, channels=channels, groups=32,
+                           act=1, eps=EPS)
+        n = lib.d3gs_group_norm_workspace_bytes(C.byref(d), 0)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        failed = 0
+        for k in range(8000):
+            failed += lib.d3gs_group_norm_forward(C.byref(d), x.data_ptr(), None, None, y.data_ptr(), stats.data_ptr(),
+                                                  ws.data_ptr(), n, stream.cuda_stream) != 0
+            if k % 200 == 0:
+                stream.synchronize()
+        stream.synchronize()
+        if failed:
+            failures.append((channels, failed, _lib.last_error()))
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in (16384, 8192)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures

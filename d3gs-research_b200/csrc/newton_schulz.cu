@@ -16,7 +16,7 @@
 // hold every entry that matters.  One fp16 value keeps 11 bits, two of them, v = hi + lo, keep 22.
 //  * 32-bit matrices: all operands hi + lo, three products hi hi + hi lo + lo hi; the dropped lo lo is of the size of
 //    the last bit.  (Two bf16 values would hold 16 bits only, and three of them need six products.)
-//  * 16-bit matrices (large ones, see planes_of): A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
+//  * 16-bit matrices (large ones, see Batch): A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
 //    and B lose turns X's singular directions by that much and no more.  What X loses is noise in all directions alike,
 //    and the next steps amplify it where X is small: with one value the result is 4e-3 off at 512 x 512 and 6e-3 at
 //    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.  So it is
@@ -1448,41 +1448,70 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
 }
-// How the products of a list of matrices are cut: pairs of CTAs when the largest short side is above kPairFrom.  (Pairs
-// from 257 on instead: 320 x 320 155 us either way, 384 x 384 171 instead of 167, 384 x 3456 335 instead of 176.)
+// The ways through the products.  kLarge, pairs of CTAs: short sides above kPairFrom.  (Pairs from 257 on instead: 320 x
+// 320 155 us either way, 384 x 384 171 instead of 167, 384 x 3456 335 instead of 176.)  kTiny, a CTA a matrix: what fits
+// shared memory.  kSmall, tiles: the others.
 constexpr int kPairFrom = 384;
-bool large(const D3gsOrthoMatrix* mats, int32_t count) {
-    for (int32_t i = 0; i < count; ++i)
-        if ((mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols) > kPairFrom && mats[i].rows > 0 && mats[i].cols > 0) return true;
-    return false;
+enum { kNone = -1, kTiny = 0, kSmall = 1, kLarge = 2 };
+int way_of(const D3gsOrthoMatrix& d) {
+    const int64_t m = min(d.rows, d.cols), n = max(d.rows, d.cols);
+    if (m == 0) return kNone;
+    if (m > kPairFrom) return kLarge;
+    return m > kRows || n > kTinyCols || div_up64(n, kCols) + 2 * div_up64(m, kCols) > kTinyBlocks ? kSmall : kTiny;
 }
-// One CTA a matrix when all of them are that small.  (A list with one larger matrix goes the other way as a whole: the
-// small ones run beside it there, and cost nothing.)
-bool tiny(const D3gsOrthoMatrix* mats, int32_t count) {
-    for (int32_t i = 0; i < count; ++i) {
-        const int64_t m = min(mats[i].rows, mats[i].cols), n = max(mats[i].rows, mats[i].cols);
-        if (m > kRows || n > kTinyCols || div_up64(n, kCols) + 2 * div_up64(m, kCols) > kTinyBlocks) return false;
+// A list of matrices, cut into batches that share launches.  The largest come first, and a batch goes the way of its largest:
+// smaller ones run beside that and cost nothing.  (What is left of them when a batch is full goes its own way.)
+struct List {
+    const D3gsOrthoMatrix* mats;
+    int32_t count, dtype;
+    int32_t at = 0;
+    int way = kLarge;
+    const D3gsOrthoMatrix* next() {
+        for (; way > kNone; --way, at = 0)
+            while (at < count)
+                if (way_of(mats[at++]) == way) return &mats[at - 1];
+        return nullptr;
     }
-    return true;
-}
-// Planes of A and B.  Small matrices take two for 16-bit types too: with them it is not the products that take time, and
-// one plane would cost an 8 x 8 matrix up to twice the error of its own rounding.
-int planes_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
-    return cfg.dtype == D3GS_DTYPE_F32 || !large(mats, count) ? 2 : 1;
-}
+};
 constexpr size_t kHead = 256 + 1024;   // the failure word, the tickets
 // Column blocks of a long axis that each of the pairs sharing a tile should have at least; twice that in 16 bits.
 constexpr int kShare = 8;
-size_t shared_bytes(const D3gsOrthoMatrix* mats, int32_t count) {
+struct Batch {
+    const D3gsOrthoMatrix* mat[kMaxMatrices];
+    int count = 0, way = kNone;
+    // Planes of A and B.  Small matrices take two for 16-bit types too: with them it is not the products that take time, and
+    // one plane would cost an 8 x 8 matrix up to twice the error of its own rounding.
+    int planes = 2;
+    size_t sums = 0, bytes = 0;   // room for shared sums; all of the workspace
+};
+bool next_batch(List& list, Batch& b) {
+    b = Batch{};
     int64_t longest = 0;
-    for (int32_t i = 0; i < count; ++i) longest = max(longest, max(mats[i].rows, mats[i].cols));
-    return large(mats, count) && div_up64(longest, kCols) >= 4 * kShare ? kTickets * kSumBytes : 0;
+    while (b.count < kMaxMatrices) {
+        const D3gsOrthoMatrix* const d = list.next();
+        if (!d) break;
+        if (b.count == 0) {
+            b.way = way_of(*d);
+            b.planes = list.dtype != D3GS_DTYPE_F32 && b.way == kLarge ? 1 : 2;
+        }
+        b.mat[b.count++] = d;
+        longest = max(longest, max(d->rows, d->cols));
+        b.bytes += parts_of(*d, b.planes).total;
+    }
+    if (b.way == kTiny) b.bytes = 0;   // (all in shared memory)
+    else {
+        if (b.way == kLarge && div_up64(longest, kCols) >= 4 * kShare) b.sums = kTickets * kSumBytes;
+        b.bytes += kHead + b.sums;
+    }
+    return b.count > 0;
 }
+// Batches run one after another, each in the same workspace.
 size_t workspace_of(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig& cfg) {
-    size_t need = 256 + kHead + shared_bytes(mats, count);   // (alignment)
-    const int planes = planes_of(mats, count, cfg);
-    for (int32_t i = 0; i < count; ++i) need += parts_of(mats[i], planes).total;
-    return need;
+    List list{mats, count, cfg.dtype};
+    Batch b;
+    size_t most = 0;
+    while (next_batch(list, b)) most = max(most, b.bytes);
+    return 256 + most;   // (alignment)
 }
 
 // Scales of the operands.  The singular values of X lie in [0, x]: x = 1 at the start, and after a step the largest
@@ -1632,13 +1661,15 @@ template <bool F32, bool PAIR, int MODE, typename B> int32_t product(const Table
     else return pair_product<false, MODE, 1>(t, blocks, st);
 }
 
-// Fills the table with as many matrices as it takes, from number i on, and gives them their workspace.
-void next_table(Table& t, const D3gsOrthoMatrix* mats, int32_t count, int32_t& i, bool muon, int planes, char*& at) {
-    t.count = 0;
-    for (; i < count && t.count < kMaxMatrices; ++i) {
-        const D3gsOrthoMatrix& d = mats[i];
-        if (d.rows == 0 || d.cols == 0) continue;
-        const Parts p = parts_of(d, planes);
+// The table of a batch, whose workspace begins at `at`.
+void fill_table(Table& t, const Batch& b, bool muon, char* at) {
+    t.fail = reinterpret_cast<uint32_t*>(at);
+    t.tickets = reinterpret_cast<uint32_t*>(at + 256);
+    t.sums = reinterpret_cast<float4*>(at + kHead);
+    at += kHead + b.sums;
+    for (t.count = 0; t.count < b.count;) {
+        const D3gsOrthoMatrix& d = *b.mat[t.count];
+        const Parts p = parts_of(d, b.planes);
         Matrix& m = t.mat[t.count++];
         m.src = d.src;
         m.momentum = muon ? d.momentum : nullptr;
@@ -1685,61 +1716,51 @@ Steps steps_of(const D3gsOrthoConfig& cfg, const Scales& sc) {
 }
 
 // Tiny matrices: one launch, a CTA each.
-int32_t run_tiny(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t count, bool muon, char* at, cudaStream_t st) {
-    for (int32_t i = 0; i < count;) {
-        next_table(t, mats, count, i, muon, 2, at);
-        if (t.count == 0) break;
-        int blocks = 0;
-        for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + 2 * t.mat[k].mk);
-        if (int32_t rc = launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st,
-                                kTinyBlocks * 2 * kPlane + 1024, t, sp))
-            return rc;
-    }
-    return D3GS_OK;
+int32_t run_tiny(Table& t, const Steps& sp, cudaStream_t st) {
+    int blocks = 0;
+    for (int k = 0; k < t.count; ++k) blocks = max(blocks, t.mat[k].nk + 2 * t.mat[k].mk);
+    return launch(ns_tiny_kernel, "ns_tiny_kernel", t.count, kTinyThreads, blocks * 2 * kPlane + 1024, 1, st,
+                  kTinyBlocks * 2 * kPlane + 1024, t, sp);
 }
 
 template <bool F32, bool PAIR>
-int32_t run_products(Table& t, const Steps& sp, const D3gsOrthoMatrix* mats, int32_t count, bool muon, char* at, cudaStream_t st) {
-    for (int32_t i = 0; i < count;) {
-        next_table(t, mats, count, i, muon, F32 ? 2 : 1, at);
-        if (t.count == 0) break;
-        auto blocks = [&](auto per) {
-            int64_t b = 0;
-            for (int k = 0; k < t.count; ++k) {
-                t.first_block[k] = (int32_t)b;
-                b += per(t.mat[k]);
-            }
-            t.first_block[t.count] = (int32_t)b;
-            return (unsigned)b;
-        };
-        auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
-        t.from = 0;
-        unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
-        if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
-        t.out_scale = sp.first;
-        t.exact = !F32;
-        grid = blocks(every_block);
-        if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
-        for (int s = 0; s < sp.count; ++s) {
-            const bool one = s == 0 || s == sp.count - 1;
-            t.exact = !F32 && s == 0;
-            t.cubic = sp.cubic >> s & 1;
-            t.out_scale = sp.gram[s];
-            t.shift = sp.gram_shift[s];
-            if (int32_t rc = product<F32, PAIR, kGram>(t, one, blocks, st)) return rc;
-            if (!t.cubic) {
-                t.out_scale = sp.square[s];
-                t.shift = sp.square_shift[s];
-                if (int32_t rc = product<F32, PAIR, kSquare>(t, one, blocks, st)) return rc;
-            }
-            t.out_scale = sp.apply[s];
-            if (int32_t rc = product<F32, PAIR, kApply>(t, one, blocks, st)) return rc;
-            t.from ^= 1;
+int32_t run_products(Table& t, const Steps& sp, cudaStream_t st) {
+    auto blocks = [&](auto per) {
+        int64_t b = 0;
+        for (int k = 0; k < t.count; ++k) {
+            t.first_block[k] = (int32_t)b;
+            b += per(t.mat[k]);
         }
-        t.out_scale = sp.last;
-        grid = blocks(every_block);
-        if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
+        t.first_block[t.count] = (int32_t)b;
+        return (unsigned)b;
+    };
+    auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
+    t.from = 0;
+    unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
+    if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
+    t.out_scale = sp.first;
+    t.exact = !F32;
+    grid = blocks(every_block);
+    if (int32_t rc = launch(ns_load_kernel, "ns_load_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
+    for (int s = 0; s < sp.count; ++s) {
+        const bool one = s == 0 || s == sp.count - 1;
+        t.exact = !F32 && s == 0;
+        t.cubic = sp.cubic >> s & 1;
+        t.out_scale = sp.gram[s];
+        t.shift = sp.gram_shift[s];
+        if (int32_t rc = product<F32, PAIR, kGram>(t, one, blocks, st)) return rc;
+        if (!t.cubic) {
+            t.out_scale = sp.square[s];
+            t.shift = sp.square_shift[s];
+            if (int32_t rc = product<F32, PAIR, kSquare>(t, one, blocks, st)) return rc;
+        }
+        t.out_scale = sp.apply[s];
+        if (int32_t rc = product<F32, PAIR, kApply>(t, one, blocks, st)) return rc;
+        t.from ^= 1;
     }
+    t.out_scale = sp.last;
+    grid = blocks(every_block);
+    if (int32_t rc = launch(ns_store_kernel, "ns_store_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
     return D3GS_OK;
 }
 
@@ -1754,22 +1775,25 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
                  "%s: workspace missing, unaligned or smaller than d3gs_orthogonalize_workspace_bytes", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Steps sp = steps_of(*cfg, sc);
-    char* at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
+    char* const at = reinterpret_cast<char*>(up256((size_t)(uintptr_t)ws));
     Table t{};
-    t.fail = reinterpret_cast<uint32_t*>(at);
-    t.tickets = reinterpret_cast<uint32_t*>(at + 256);
-    t.sums = reinterpret_cast<float4*>(at + kHead);
-    at += kHead + shared_bytes(mats, count);
     t.bf16 = cfg->dtype == D3GS_DTYPE_BF16;
     t.eps = cfg->eps;
     t.mu = cfg->momentum;
     t.nesterov = cfg->nesterov;
     t.decay = cfg->decay;
     t.hooks = test_hooks();
-    if (tiny(mats, count)) return run_tiny(t, sp, mats, count, muon, at, st);
-    if (!large(mats, count)) return run_products<true, false>(t, sp, mats, count, muon, at, st);
-    return cfg->dtype == D3GS_DTYPE_F32 ? run_products<true, true>(t, sp, mats, count, muon, at, st)
-                                        : run_products<false, true>(t, sp, mats, count, muon, at, st);
+    List list{mats, count, cfg->dtype};
+    Batch b;
+    while (next_batch(list, b)) {
+        fill_table(t, b, muon, at);
+        const int32_t rc = b.way == kTiny                  ? run_tiny(t, sp, st)
+                           : b.way == kSmall               ? run_products<true, false>(t, sp, st)
+                           : cfg->dtype == D3GS_DTYPE_F32 ? run_products<true, true>(t, sp, st)
+                                                           : run_products<false, true>(t, sp, st);
+        if (rc) return rc;
+    }
+    return D3GS_OK;
 }
 
 }  // namespace

@@ -160,3 +160,30 @@ def test_tangents_are_refused(recorder, monkeypatch, name):
         assert not recorder.calls
         calls()[name](x)                   # inputs without one go through
     assert recorder.calls
+
+
+def workspace(shapes, dtype=0):
+    import ctypes as C
+    lib = _lib.load()
+    mats = (_lib.OrthoMatrix * len(shapes))()
+    for m, (rows, cols) in zip(mats, shapes):
+        m.src, m.dst, m.rows, m.cols, m.src_row_stride = 16, 16, rows, cols, cols
+    cfg = _lib.OrthoConfig()
+    cfg.dtype, cfg.steps, cfg.eps = dtype, 1, 1e-7
+    cfg.coefficients[0][:] = (3.4445, -4.775, 2.0315)
+    need = lib.d3gs_orthogonalize_workspace_bytes(mats, len(shapes), C.byref(cfg))
+    assert need > 0, _lib.last_error()
+    return need
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspace_is_that_of_the_largest_batch(dtype):
+    """Matrices that stay in shared memory need none; 32 at a time share launches, and all batches one workspace."""
+    tiny, wide = (8, 8), (2048, 2048)
+    assert workspace([tiny], dtype) == workspace([tiny] * 10000, dtype) <= 4096
+    assert workspace([wide] * 32, dtype) == workspace([wide] * 200, dtype) < 33 * workspace([wide], dtype)
+    # the large ones fill a batch of their own whatever their order, the small ones need no more
+    mixed = [tiny, wide] * 32
+    assert workspace(mixed, dtype) == workspace([wide] * 32, dtype)
+    assert workspace([wide, (0, 5), tiny, (100, 700)], dtype) <= workspace([wide, tiny, (100, 700)], dtype)
+    assert workspace([(0, 4)]) <= 4096

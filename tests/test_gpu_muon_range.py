@@ -1,10 +1,10 @@
-"""orthogonalize and muon_step at the ends of the floats' range: norms and eps whose reciprocals a 32-bit float does not
+"""orthogonalize and muon_step over long lists, and at the ends of the floats' range: norms and eps whose reciprocals a 32-bit float does not
 hold.  On every way through the products: a CTA a matrix, tiles, pairs of CTAs, shared sums."""
 import pytest
 import torch
 
 from d3gs_research_b200 import muon_step, orthogonalize
-from test_gpu_muon import BF16, F32, check, make
+from test_gpu_muon import BF16, F32, check, check_step, make, tensors
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,28 @@ def test_very_small_and_very_large_updates(cuda_device, m, n, dtype):
     check((u * 2.0 ** -126).to(dtype), eps=2.0 ** -112)      # far below eps
     check((u * 1.99 * 2.0 ** 127 * 0.99).to(dtype))
     check((u * 2.0 ** 100).to(dtype), eps=2.0 ** 120)
+
+
+def launches(call):
+    from d3gs_research_b200 import _lib
+    lib = _lib.load()
+    before = lib.d3gs_kernel_launch_count()
+    call()
+    return lib.d3gs_kernel_launch_count() - before
+
+
+def test_long_lists_take_their_workspace_and_their_way_a_batch(cuda_device):
+    """Eighty tiny matrices with one large among them, and forty large ones with tiny ones between: every result is that of
+    the formula, and what a batch of 32 has left of the tiny ones takes a launch a batch."""
+    for shapes, most in (([(8 + k % 5, 16 + k % 40) for k in range(80)] + [(500, 420)], 18 + 2),
+                         ([(400, 390 + k // 2) if k % 2 else (8, 16 + k) for k in range(80)], 2 * 18 + 1)):
+        run = tensors(shapes)
+        assert launches(lambda: check_step(*run)) == most
+    u = torch.stack([make(24, 40, seed=k) for k in range(100)])
+    assert launches(lambda: orthogonalize(u)) == 4
+    check(u)
+    for dtype in (F32, BF16):      # the workspace of one batch after another, no stale values in it
+        v = torch.stack([make(390 + 2, 500, seed=k) for k in range(40)]).to(dtype)
+        got = check(v)
+        assert torch.equal(orthogonalize(v[35]), orthogonalize(v[35:36])[0])
+        assert torch.equal(orthogonalize(v), got)

@@ -39,7 +39,8 @@ namespace {
 
 constexpr int kMaxMatrices = 32;   // per launch, a table of less than 4 KB; longer lists are cut
 constexpr int kThreads = 256;
-constexpr int kPieces = 1024;       // pieces of eight neighbouring columns per CTA of the norm pass
+constexpr int kPieces = 1024;       // pieces of eight neighbouring columns that a CTA of the norm pass takes at a time
+constexpr int kMaxNorms = 4096;     // sums of squares of a matrix: every CTA of the first pass adds them up
 constexpr int kMaxShort = 16384, kMaxLong = 1 << 24;
 constexpr int kRows = 128, kCols = 64;                 // one block
 constexpr uint32_t kPlane = kRows * kCols * 2;         // bytes of one fp16 plane of a block
@@ -147,6 +148,16 @@ __device__ __forceinline__ void load_src8(const Table& t, const Matrix& m, int64
     }
 }
 
+// How many times kPieces a CTA of the norm pass takes, so that there are at most kMaxNorms sums.  (Once, 64 x 16777216
+// in 32 bits: 155 -> 137 ms; all CTAs adding all sums is quadratic in the number of values.)
+__host__ __device__ __forceinline__ unsigned norm_rounds(int64_t rows, int64_t cols) {
+    return (unsigned)((rows * ((cols + 7) / 8) + (int64_t)kPieces * kMaxNorms - 1) / ((int64_t)kPieces * kMaxNorms));
+}
+__host__ __device__ __forceinline__ int norm_count(int64_t rows, int64_t cols) {
+    const int64_t each = (int64_t)kPieces * norm_rounds(rows, cols);   // (no empty matrix comes here)
+    return (int)((rows * ((cols + 7) / 8) + each - 1) / each);
+}
+
 // ---- new momentum, and the sum of squares of the update (in 64 bits: no value of a float overflows it) -----------
 __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant__ Table t) {
     __shared__ double s[kThreads / 32];
@@ -159,28 +170,32 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
     if (blockIdx.x == 0 && threadIdx.x == 0) *t.fail = 0;
     if (blockIdx.x == 0 && threadIdx.x < kTickets) t.tickets[threadIdx.x] = 0;
     double sum = 0.0;
-    float u[kPieces / kThreads][8], buf[kPieces / kThreads][8];
+    const unsigned rounds = norm_rounds(m.rows, m.cols);
+    for (unsigned round = 0; round < rounds; ++round) {
+        const unsigned first = ((unsigned)block * rounds + round) * kPieces;
+        float u[kPieces / kThreads][8], buf[kPieces / kThreads][8];
 #pragma unroll
-    for (int k = 0; k < kPieces / kThreads; ++k) {
-        const unsigned i = (unsigned)block * kPieces + k * kThreads + threadIdx.x;
-        const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
-        load_src8(t, m, n ? r * m.src_stride + c : 0, access.src, n, u[k]);
-        if (m.momentum) load8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < kPieces / kThreads; ++k) {
-        if (m.momentum) {
-            const unsigned i = (unsigned)block * kPieces + k * kThreads + threadIdx.x;
+        for (int k = 0; k < kPieces / kThreads; ++k) {
+            const unsigned i = first + k * kThreads + threadIdx.x;
             const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                buf[k][j] = fmaf(t.mu, buf[k][j], (1.0f - t.mu) * u[k][j]);
-                u[k][j] = update_of(t, u[k][j], buf[k][j]);
-            }
-            store8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
+            load_src8(t, m, n ? r * m.src_stride + c : 0, access.src, n, u[k]);
+            if (m.momentum) load8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += (double)u[k][j] * (double)u[k][j];
+        for (int k = 0; k < kPieces / kThreads; ++k) {
+            if (m.momentum) {
+                const unsigned i = first + k * kThreads + threadIdx.x;
+                const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    buf[k][j] = fmaf(t.mu, buf[k][j], (1.0f - t.mu) * u[k][j]);
+                    u[k][j] = update_of(t, u[k][j], buf[k][j]);
+                }
+                store8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += (double)u[k][j] * (double)u[k][j];
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -210,7 +225,7 @@ __device__ __forceinline__ Factor factor_of(double sum_of_squares, float eps, fl
 // every CTA adds the sums up itself, in the same order
 __device__ __forceinline__ double sum_of_squares(const Matrix& m) {
     __shared__ double s[kThreads / 32];
-    const int n = (int)(((int64_t)m.rows * ((m.cols + 7) / 8) + kPieces - 1) / kPieces);
+    const int n = norm_count(m.rows, m.cols);
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += kThreads) sum += m.norms[i];
 #pragma unroll
@@ -1443,7 +1458,7 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.nk = (p.n + kCols - 1) / kCols;
     p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
-    p.norms = up256((size_t)div_up64(d.rows * ((d.cols + 7) / 8), kPieces) * 8 + 8);
+    p.norms = up256((size_t)norm_count(d.rows, d.cols) * 8 + 8);
     p.v = (size_t)p.mb * 2 * planes * kPlane;
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
@@ -1736,7 +1751,7 @@ int32_t run_products(Table& t, const Steps& sp, cudaStream_t st) {
     };
     auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
     t.from = 0;
-    unsigned grid = blocks([](const Matrix& m) { return div_up64((int64_t)m.rows * ((m.cols + 7) / 8), kPieces); });
+    unsigned grid = blocks([](const Matrix& m) { return (int64_t)norm_count(m.rows, m.cols); });
     if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
     t.out_scale = sp.first;
     t.exact = !F32;

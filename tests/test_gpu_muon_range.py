@@ -68,3 +68,12 @@ def test_long_lists_take_their_workspace_and_their_way_a_batch(cuda_device):
         got = check(v)
         assert torch.equal(orthogonalize(v[35]), orthogonalize(v[35:36])[0])
         assert torch.equal(orthogonalize(v), got)
+
+
+@pytest.mark.parametrize("m,n,dtype", [(40, 1000003, F32), (1000003, 40, BF16), (500, 80000, F32)])
+def test_so_many_values_that_a_cta_takes_several_turns_of_the_norm(cuda_device, m, n, dtype):
+    check(make(m, n).to(dtype))
+
+
+def test_step_of_so_many_values(cuda_device):
+    check_step(*tensors([(40, 900001), (30, 20)]))

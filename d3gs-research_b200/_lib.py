@@ -118,7 +118,8 @@ class OrthoMatrix(C.Structure):
 
 class OrthoConfig(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("steps", C.c_int32), ("coefficients", C.c_float * 3 * NS_MAX_STEPS),
-                ("eps", C.c_float), ("momentum", C.c_float), ("decay", C.c_float), ("nesterov", C.c_int32)]
+                ("eps", C.c_float), ("decay", C.c_float), ("momentum", C.c_double), ("nesterov", C.c_int32),
+                ("reserved_", C.c_int32)]
 
 
 _STRUCTS = [Camera, OpConfig, Model, ModelGrad, SplatContext, AdamSegment, DensifyStats, PeerSet, RefineConfig,

@@ -66,7 +66,8 @@ struct Table {
     int32_t first_block[kMaxMatrices + 1];
     int32_t count;
     int32_t bf16;         // src and dst type (momentum and parameters are always 32 bits)
-    float eps, mu, decay;
+    float eps, decay;
+    float mu, fresh;      // weights of the old buffer and of the gradient; fresh is 1 - mu, rounded once
     int32_t nesterov;
     int32_t from;         // which of x[] holds X
     float out_scale;      // of a product's result; of X in the first and the last pass
@@ -99,7 +100,7 @@ __device__ __forceinline__ int find_matrix(const Table& t, int id, int& block) {
 
 // the update from gradient and NEW momentum
 __device__ __forceinline__ float update_of(const Table& t, float g, float buf) {
-    return t.nesterov ? fmaf(t.mu, buf, (1.0f - t.mu) * g) : buf;
+    return t.nesterov ? fmaf(t.mu, buf, t.fresh * g) : buf;
 }
 
 // Eight neighbouring columns of a row of U, of which `n` exist; where rows are so aligned, as vectors.
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
                 const int r = i / per_row, c = (i - r * per_row) * 8, n = i < pieces ? min(8, m.cols - c) : 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    buf[k][j] = fmaf(t.mu, buf[k][j], (1.0f - t.mu) * u[k][j]);
+                    buf[k][j] = fmaf(t.mu, buf[k][j], t.fresh * u[k][j]);
                     u[k][j] = update_of(t, u[k][j], buf[k][j]);
                 }
                 store8(m.momentum + (n ? (int64_t)r * m.cols + c : 0), access.state, n, buf[k]);
@@ -643,7 +644,7 @@ __global__ void __launch_bounds__(kTinyThreads, 1) ns_tiny_kernel(const __grid_c
             load8(m.momentum + r * m.cols + c, access.state, n, buf);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (update) buf[e] = fmaf(t.mu, buf[e], (1.0f - t.mu) * u[e]);
+                if (update) buf[e] = fmaf(t.mu, buf[e], t.fresh * u[e]);
                 u[e] = update_of(t, u[e], buf[e]);
             }
             if (update) store8(m.momentum + r * m.cols + c, access.state, n, buf);
@@ -1794,7 +1795,8 @@ int32_t entry(const D3gsOrthoMatrix* mats, int32_t count, const D3gsOrthoConfig*
     Table t{};
     t.bf16 = cfg->dtype == D3GS_DTYPE_BF16;
     t.eps = cfg->eps;
-    t.mu = cfg->momentum;
+    t.mu = (float)cfg->momentum;
+    t.fresh = (float)(1.0 - cfg->momentum);
     t.nesterov = cfg->nesterov;
     t.decay = cfg->decay;
     t.hooks = test_hooks();

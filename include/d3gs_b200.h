@@ -574,8 +574,10 @@ typedef struct D3gsOrthoConfig {
     int32_t steps;
     float coefficients[D3GS_NS_MAX_STEPS][3];   /* a, b, c of every step */
     float eps;
-    float momentum, decay;    /* d3gs_muon_step only: mu; 1 - lr * weight decay */
+    float decay;              /* d3gs_muon_step only: 1 - lr * weight decay */
+    double momentum;          /* d3gs_muon_step only: mu (in 64 bits: 1 - mu is taken from it) */
     int32_t nesterov;
+    int32_t reserved_;
 } D3gsOrthoConfig;
 size_t d3gs_orthogonalize_workspace_bytes(const D3gsOrthoMatrix* matrices, int32_t count, const D3gsOrthoConfig* cfg);
 int32_t d3gs_orthogonalize(const D3gsOrthoMatrix* matrices, int32_t count, const D3gsOrthoConfig* cfg, void* workspace,

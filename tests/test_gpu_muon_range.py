@@ -77,3 +77,25 @@ def test_so_many_values_that_a_cta_takes_several_turns_of_the_norm(cuda_device, 
 
 def test_step_of_so_many_values(cuda_device):
     check_step(*tensors([(40, 900001), (30, 20)]))
+
+
+@pytest.mark.parametrize("mu", [0.0, 0.3, 0.95, 0.999, 0.9999, 1 - 2.0 ** -20])
+@pytest.mark.parametrize("m,n", [(40, 60), (300, 200), (500, 420)])
+def test_the_gradients_weight_is_one_minus_the_momentum(cuda_device, m, n, mu):
+    """1 - mu as the difference of 64-bit numbers: the difference of 32-bit ones is 1e-3 off for a momentum near one.  Two
+    roundings of the new buffer: the weight's and the product's; with an old one, three, each of at most the terms' size."""
+    g, old = make(m, n, seed=1), make(m, n, seed=2)
+    for start in (torch.zeros_like(old), old):
+        buf = start.clone()
+        muon_step([torch.zeros(m, n, device="cuda")], [g], [buf], lr=0.1, momentum=mu)
+        kept, fresh = mu * start.double(), (1 - mu) * g.double()
+        assert ((buf.double() - kept - fresh).abs() <= 3 * 2.0 ** -24 * (kept.abs() + fresh.abs()) + 2.0 ** -149).all()
+
+
+def test_the_updates_weights_are_those_of_the_buffer(cuda_device):
+    """Nesterov: the update mu buffer + (1 - mu) g.  With an old buffer of zeros the update is (1 - mu^2) g, with a momentum of
+    zero g; with a buffer far from the gradient the weights show in the direction."""
+    for mu in (0.0, 0.95, 0.9999):
+        run = tensors([(40, 60), (300, 200), (500, 420)])
+        run[1][:] = [1e3 * g for g in run[1]]
+        check_step(*run, mu=mu)

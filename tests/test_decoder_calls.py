@@ -187,3 +187,41 @@ def test_workspace_is_that_of_the_largest_batch(dtype):
     assert workspace(mixed, dtype) == workspace([wide] * 32, dtype)
     assert workspace([wide, (0, 5), tiny, (100, 700)], dtype) <= workspace([wide, tiny, (100, 700)], dtype)
     assert workspace([(0, 4)]) <= 4096
+
+
+@pytest.mark.parametrize("name", ["group_norm_act", "orthogonalize", "muon_step"])
+def test_the_current_device_is_that_of_the_tensors(recorder, monkeypatch, name):
+    """With another device current, all calls of the library are made with the tensors' own, forward and backward."""
+    current = [7]
+
+    class on:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    seen = []
+    original = Recorder.__getattr__
+
+    def spy(self, entry):
+        call = original(self, entry)
+        return lambda *args: (seen.append((entry, current[-1])), call(*args))[1]
+
+    on_gpu(monkeypatch)
+    monkeypatch.setattr(Recorder, "__getattr__", spy)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[-1])
+    monkeypatch.setattr(torch.cuda, "device", on)
+    x = torch.ones(4, 6)
+    if name == "group_norm_act":
+        x.requires_grad_()
+        y = calls()[name](x)
+        torch.autograd.grad(y, x, torch.ones_like(y))
+        assert {entry for entry, _ in seen} >= {"d3gs_group_norm_forward", "d3gs_group_norm_backward"}
+    else:
+        calls()[name](x)
+    assert seen and all(device is None for _, device in seen)   # (a CPU tensor's device has no index)
+    assert current == [7]

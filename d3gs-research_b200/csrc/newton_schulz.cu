@@ -59,6 +59,7 @@ struct Matrix {
     int32_t rows, cols;
     int32_t m;            // short side
     int32_t mb, mk, nk;   // blocks: rows of all three, columns of A and B, columns of X
+    int32_t rounds, sums; // of the norm pass: how many times kPieces a CTA takes; sums of squares that gives
     float rate;
 };
 struct Table {
@@ -149,18 +150,9 @@ __device__ __forceinline__ void load_src8(const Table& t, const Matrix& m, int64
     }
 }
 
-// How many times kPieces a CTA of the norm pass takes, so that there are at most kMaxNorms sums.  (Once, 64 x 16777216
-// in 32 bits: 155 -> 137 ms; all CTAs adding all sums is quadratic in the number of values.)
-__host__ __device__ __forceinline__ unsigned norm_rounds(int64_t rows, int64_t cols) {
-    return (unsigned)((rows * ((cols + 7) / 8) + (int64_t)kPieces * kMaxNorms - 1) / ((int64_t)kPieces * kMaxNorms));
-}
-__host__ __device__ __forceinline__ int norm_count(int64_t rows, int64_t cols) {
-    const int64_t each = (int64_t)kPieces * norm_rounds(rows, cols);   // (no empty matrix comes here)
-    return (int)((rows * ((cols + 7) / 8) + each - 1) / each);
-}
-
 // ---- new momentum, and the sum of squares of the update (in 64 bits: no value of a float overflows it) -----------
-__global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant__ Table t) {
+// TURNS: a CTA may take several times kPieces.  (An instance of its own: the loop makes 8 x 2048 x 512 in 16 bits 17 us, not 13.)
+template <bool TURNS> __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant__ Table t) {
     __shared__ double s[kThreads / 32];
     int block;
     const Matrix& m = t.mat[find_matrix(t, (int)blockIdx.x, block)];
@@ -171,8 +163,8 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(const __grid_constant
     if (blockIdx.x == 0 && threadIdx.x == 0) *t.fail = 0;
     if (blockIdx.x == 0 && threadIdx.x < kTickets) t.tickets[threadIdx.x] = 0;
     double sum = 0.0;
-    const unsigned rounds = norm_rounds(m.rows, m.cols);
-    for (unsigned round = 0; round < rounds; ++round) {
+    const int rounds = TURNS ? m.rounds : 1;
+    for (int round = 0; round < rounds; ++round) {
         const unsigned first = ((unsigned)block * rounds + round) * kPieces;
         float u[kPieces / kThreads][8], buf[kPieces / kThreads][8];
 #pragma unroll
@@ -226,9 +218,8 @@ __device__ __forceinline__ Factor factor_of(double sum_of_squares, float eps, fl
 // every CTA adds the sums up itself, in the same order
 __device__ __forceinline__ double sum_of_squares(const Matrix& m) {
     __shared__ double s[kThreads / 32];
-    const int n = norm_count(m.rows, m.cols);
     double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += kThreads) sum += m.norms[i];
+    for (int i = threadIdx.x; i < m.sums; i += kThreads) sum += m.norms[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = sum;
@@ -1447,7 +1438,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) ns_pair_kernel(const __grid_c
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Parts {
-    int m, n, mb, mk, nk;
+    int m, n, mb, mk, nk, rounds, sums;
     size_t x, a, v, norms, total;   // bytes
 };
 Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
@@ -1459,7 +1450,12 @@ Parts parts_of(const D3gsOrthoMatrix& d, int planes) {
     p.nk = (p.n + kCols - 1) / kCols;
     p.x = (size_t)p.mb * p.nk * 2 * kPlane;
     p.a = (size_t)p.mb * p.mk * planes * kPlane;
-    p.norms = up256((size_t)norm_count(d.rows, d.cols) * 8 + 8);
+    // Every CTA of the first pass adds up all sums of squares of its matrix: at most kMaxNorms of them, since the work would be
+    // quadratic in the number of values.  (One each kPieces -> this, 64 x 16777216 in 32 bits: 155 -> 137 ms.)
+    const int64_t pieces = d.rows * ((d.cols + 7) / 8);
+    p.rounds = (int)div_up64(pieces, (int64_t)kPieces * kMaxNorms);
+    p.sums = p.rounds == 0 ? 0 : (int)div_up64(pieces, (int64_t)kPieces * p.rounds);
+    p.norms = up256((size_t)p.sums * 8 + 8);
     p.v = (size_t)p.mb * 2 * planes * kPlane;
     p.total = p.m == 0 ? 0 : 2 * p.x + 2 * p.a + p.v + p.norms;
     return p;
@@ -1697,6 +1693,8 @@ void fill_table(Table& t, const Batch& b, bool muon, char* at) {
         m.mb = p.mb;
         m.mk = p.mk;
         m.nk = p.nk;
+        m.rounds = p.rounds;
+        m.sums = p.sums;
         m.rate = d.rate;
         m.x[0] = at;
         m.x[1] = at + p.x;
@@ -1752,8 +1750,10 @@ int32_t run_products(Table& t, const Steps& sp, cudaStream_t st) {
     };
     auto every_block = [](const Matrix& m) { return (int64_t)m.mb * m.nk; };
     t.from = 0;
-    unsigned grid = blocks([](const Matrix& m) { return (int64_t)norm_count(m.rows, m.cols); });
-    if (int32_t rc = launch(ns_norm_kernel, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
+    unsigned grid = blocks([](const Matrix& m) { return (int64_t)m.sums; });
+    int rounds = 1;
+    for (int k = 0; k < t.count; ++k) rounds = max(rounds, t.mat[k].rounds);
+    if (int32_t rc = launch(rounds > 1 ? ns_norm_kernel<true> : ns_norm_kernel<false>, "ns_norm_kernel", grid, kThreads, 0, 1, st, 0, t)) return rc;
     t.out_scale = sp.first;
     t.exact = !F32;
     grid = blocks(every_block);

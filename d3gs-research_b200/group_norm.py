@@ -84,16 +84,29 @@ def _forward(x, groups, weight, bias, eps, act, keep: bool):
     return x, y, stats, args
 
 
+def _other(t, what: str) -> RuntimeError:
+    return RuntimeError(f"group_norm_act: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}: not the {what} "
+                        "that the forward saved")
+
+
 def _came_back(x, weight, bias, stats, dy, d):
     """The saved tensors as the library reads them.  Hooks of the caller (``save_on_cpu``) may have put copies in their
     place, laid out anew; ``d`` gets the strides of ``x`` as it is now."""
-    for t, like, dtype, shape in ((x, "x", d.dtype, dy.shape), (weight, "weight", d.weight_dtype, dy.shape[-1:]),
-                                  (bias, "bias", d.weight_dtype, dy.shape[-1:]), (stats, "statistics", 0, (d.batch, d.groups, 2))):
-        if t is not None and (t.shape != shape or t.device != dy.device or _DTYPES.get(t.dtype) != dtype):
-            raise RuntimeError(f"group_norm_act: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}: not the "
-                               f"{like} that the forward saved")
+    index, channels, wdtype = dy.get_device(), d.channels, d.weight_dtype
+    if x.shape != dy.shape or x.dtype is not dy.dtype or x.get_device() != index:
+        raise _other(x, "x")
+    if weight is not None:
+        if weight.numel() != channels or _DTYPES.get(weight.dtype) != wdtype or weight.get_device() != index:
+            raise _other(weight, "weight")
+        weight = weight.contiguous()
+    if bias is not None:
+        if bias.numel() != channels or _DTYPES.get(bias.dtype) != wdtype or bias.get_device() != index:
+            raise _other(bias, "bias")
+        bias = bias.contiguous()
+    if stats.numel() != 2 * d.batch * d.groups or stats.dtype is not torch.float32 or stats.get_device() != index:
+        raise _other(stats, "statistics")
     x, (d.x_batch_stride, d.x_pixel_stride) = _prepared(x)
-    return x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), stats.contiguous()
+    return x, weight, bias, stats.contiguous()
 
 
 def _backward(args, x, weight, bias, stats, dy, need_x: bool, need_w: bool, need_b: bool):
@@ -151,7 +164,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     Channels that are not dense, or pixels that are not evenly spaced, are copied first.  The result is dense and has
     the type of ``x``; gradients flow to ``x``, ``weight`` and ``bias`` (once).  Under ``torch.jit.trace`` or with inputs
     that carry a forward-mode tangent the call is refused."""
-    refuse_recording("group_norm_act", (x, weight, bias))
+    refuse_recording("group_norm_act", x, weight, bias)
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("group_norm_act: x must be a CUDA tensor")
     if x.dim() < 2 or x.dtype not in _DTYPES:

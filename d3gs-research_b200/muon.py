@@ -69,7 +69,7 @@ def orthogonalize(update: torch.Tensor, ns_coefficients: Sequence = NS_COEFFICIE
     same type out; every product is summed in 32 bits.  Rows that are not dense are copied first.  No gradient.
     Coefficients with which singular values in [0, 1] grow past 1024, or with ``0 < 1024 |c| < |b|``, are refused, and so
     are calls under ``torch.jit.trace`` or with a forward-mode tangent."""
-    refuse_recording("orthogonalize", (update,))
+    refuse_recording("orthogonalize", update)
     if not isinstance(update, torch.Tensor) or not update.is_cuda:
         raise ValueError("orthogonalize: update must be a CUDA tensor")
     if update.dim() < 2 or update.dtype not in (torch.float32, torch.bfloat16):
@@ -129,7 +129,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     ``sqrt(max(1, rows / columns))``, or with ``adjust_lr_fn="match_rms_adamw"`` ``0.2 sqrt(max(rows, columns))``.
     Parameters and buffers must be dense (contiguous or channels last) and must not overlap one another or a gradient."""
     params, grads, momentum_buffers = list(params), list(grads), list(momentum_buffers)
-    refuse_recording("muon_step", (*params, *grads, *momentum_buffers))
+    refuse_recording("muon_step", params, grads, momentum_buffers)
     if not len(params) == len(grads) == len(momentum_buffers):
         raise ValueError(f"muon_step: {len(params)} params, {len(grads)} grads, {len(momentum_buffers)} momentum_buffers")
     if adjust_lr_fn not in _ADJUST:

@@ -154,3 +154,20 @@ def test_launches_of_two_threads(cuda_device):
     for t in threads:
         t.join()
     assert not failures
+
+
+def test_under_torch_compile(cuda_device):
+    """The compiler does not see into the calls and leaves them as they are, with their gradients."""
+    def both(x, u):
+        return group_norm_act(x * 2, 4) + 1, orthogonalize(u + 0) * 2
+
+    x = torch.randn(2, 9, 11, 40, device="cuda").requires_grad_()
+    u = torch.randn(20, 30, device="cuda")
+    y, o = both(x, u)
+    (dx,) = torch.autograd.grad(y.sum(), x)
+    for backend in ("eager", "aot_eager"):
+        torch._dynamo.reset()
+        z, p = torch.compile(both, backend=backend)(x, u)
+        (dz,) = torch.autograd.grad(z.sum(), x)
+        assert torch.equal(y, z) and torch.equal(o, p) and torch.equal(dx, dz)
+    torch._dynamo.reset()

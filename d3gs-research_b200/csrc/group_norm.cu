@@ -133,7 +133,8 @@ template <typename T, int V> __device__ __forceinline__ void store_last(T* p, co
     __stcs(reinterpret_cast<R*>(p), *reinterpret_cast<const R*>(&v));
 }
 
-// The logistic function by ex2 and reciprocal of the special-function unit, about 2e-7 relative; u -> -inf gives 0.
+// The logistic function by ex2 and reciprocal of the special-function unit: 2e-7 relative near zero and 6e-8 |u| far from
+// it (the rounding of the exponent), where the product with u is off by at most 3e-8; u -> -inf gives 0.
 __device__ __forceinline__ Two logistic(Two u) {
     float2 e = split(mul2(u, both(-1.44269504f)));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
@@ -153,6 +154,8 @@ template <int ACT> __device__ __forceinline__ Two act_value(Two u) {
     if (ACT == kActGelu) return mul2(mul2(u, both(0.5f)), gauss2(u));
     return u;
 }
+// (__expf in GELU's slope: its error, 2 units of the last place and more for large arguments, is multiplied by a factor that
+// falls off as fast: below 1e-7 of the slope's largest value.)
 template <int ACT> __device__ __forceinline__ Two act_slope(Two u) {
     if (ACT == kActSilu) {
         const Two s = logistic(u);

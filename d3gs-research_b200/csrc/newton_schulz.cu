@@ -16,11 +16,16 @@
 // hold every entry that matters.  One fp16 value keeps 11 bits, two of them, v = hi + lo, keep 22.
 //  * 32-bit matrices: all operands hi + lo, three products hi hi + hi lo + lo hi; the dropped lo lo is of the size of
 //    the last bit.  (Two bf16 values would hold 16 bits only, and three of them need six products.)
-//  * 16-bit matrices (large ones, see Batch): A and B one value, X two of which A sees the first: A = Xhi Xhi^T, B X = B Xhi + B Xlo.  What A
-//    and B lose turns X's singular directions by that much and no more.  What X loses is noise in all directions alike,
-//    and the next steps amplify it where X is small: with one value the result is 4e-3 off at 512 x 512 and 6e-3 at
-//    4096 x 4096, three times its own rounding; with two 7e-4.  The last step amplifies little: there X is one value.  So it is
-//    in the first one, where U times a power of two is exact (8 bits) and what is left of 1 / |U| goes into the scales.
+//  * 16-bit matrices (large ones, see Batch): A, B and V one value, X two of which A sees the first: A = Xhi Xhi^T, B X =
+//    B Xhi + B Xlo.  What A and B lose turns X's singular directions by that much and no more.  What X loses is noise in all
+//    directions alike, and the next steps amplify it where X is small: with one value a result is 2.8e-3 off at 512 x 512
+//    and 5.1e-3 at 4096 x 4096 before its own rounding to bfloat16, which is 1.65e-3; with two, measured, 0.7e-3 at 2048 x
+//    512, 0.8e-3 at 512 x 512, 1.2e-3 at 2048 x 2048, 1.4e-3 at 4096 x 4096 (gradients with a few strong directions) and up
+//    to 1.5e-3 (a quarter of full rank).  The roundings themselves account for 1.1e-3 of the 1.4e-3, the bits that the
+//    tensor cores cut off running sums for the rest.  (Operands like those of 32-bit matrices would leave the output's
+//    rounding alone, for three products where there are now one or two.)  The last step amplifies little: there X is one
+//    value.  So it is in the first one, where U times a power of two is exact (8 bits) and what is left of 1 / |U| goes into
+//    the scales.
 //
 // Working matrices are stored as the products read them: blocks of 128 rows x 64 columns, each the image of one shared
 // memory tile (128-byte rows, 16-byte pieces exchanged within groups of eight rows), hi and lo one after the other, zero

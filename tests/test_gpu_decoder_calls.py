@@ -171,3 +171,18 @@ def test_under_torch_compile(cuda_device):
         (dz,) = torch.autograd.grad(z.sum(), x)
         assert torch.equal(y, z) and torch.equal(o, p) and torch.equal(dx, dz)
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_in_the_backward(cuda_device, reentrant):
+    """Under activation checkpointing the forward runs again in the backward: the same gradients, to the bit."""
+    from torch.utils.checkpoint import checkpoint
+    wide, _, gamma, beta = make((2, 31, 29, 56), 4, F32, F32)
+    gamma, beta = gamma[:40].contiguous().requires_grad_(), beta[:40].contiguous().requires_grad_()
+    wide.requires_grad_()
+    layer = lambda t: group_norm_act(group_norm_act(t[..., 8:48], 4, gamma, beta) * 2, 8)   # noqa: E731
+    want = torch.autograd.grad(layer(wide).square().sum(), (wide, gamma, beta))
+    for t in (wide, gamma, beta):
+        t.grad = None
+    checkpoint(layer, wide, use_reentrant=reentrant).square().sum().backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip((wide, gamma, beta), want))

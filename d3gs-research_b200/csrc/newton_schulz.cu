@@ -21,11 +21,11 @@
 //    directions alike, and the next steps amplify it where X is small: with one value a result is 2.8e-3 off at 512 x 512
 //    and 5.1e-3 at 4096 x 4096 before its own rounding to bfloat16, which is 1.65e-3; with two, measured, 0.7e-3 at 2048 x
 //    512, 0.8e-3 at 512 x 512, 1.2e-3 at 2048 x 2048, 1.4e-3 at 4096 x 4096 (gradients with a few strong directions) and up
-//    to 1.5e-3 (a quarter of full rank).  The roundings themselves account for 1.1e-3 of the 1.4e-3, the bits that the
-//    tensor cores cut off running sums for the rest.  (Operands like those of 32-bit matrices would leave the output's
-//    rounding alone, for three products where there are now one or two.)  The last step amplifies little: there X is one
-//    value.  So it is in the first one, where U times a power of two is exact (8 bits) and what is left of 1 / |U| goes into
-//    the scales.
+//    to 1.5e-3 (a quarter of full rank).  The same roundings done in 64 bits give these figures within 7 %; a third is that
+//    of V's diagonal, a value near b / c, behind which A V is no longer symmetric though one triangle stands for both.
+//    (Operands like those of 32-bit matrices would leave the output's rounding alone, for three products where there are
+//    now one or two.)  The last step amplifies little: there X is one value.  So it is in the first one, where U times a
+//    power of two is exact (8 bits) and what is left of 1 / |U| goes into the scales.
 //
 // Working matrices are stored as the products read them: blocks of 128 rows x 64 columns, each the image of one shared
 // memory tile (128-byte rows, 16-byte pieces exchanged within groups of eight rows), hi and lo one after the other, zero
